@@ -1,0 +1,142 @@
+// attn_capi.hip -- the extern "C" boundary of include/aih_attn.h: checks of
+// every argument that the host knows, the plan, the launches. What only the
+// device knows (lengths, positions, slots) the kernels bound themselves.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <string>
+
+#include "aih_device.h"
+#include "attn.h"
+#include "capi_util.h"
+
+namespace aih {
+namespace {
+
+constexpr uint64_t kMaxRow = 1u << 22;  // elements of a row stride: 128 rows stay within 32-bit byte offsets
+
+bool dt_ok(int32_t dt) { return dt == AIH_F32 || dt == AIH_F16 || dt == AIH_BF16; }
+uint32_t dt_bytes(int32_t dt) { return dt == AIH_F32 ? 4 : 2; }
+
+bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+std::string num(uint64_t v) { return std::to_string(v); }
+
+// A row stride in elements: 0 becomes `row`, anything else must hold a row in
+// whole 16-byte units.
+int take_stride(const char *what, uint64_t given, uint64_t row, int32_t dt, uint64_t *out) {
+  *out = given ? given : row;
+  if (*out < row) return api_fail(std::string(what) + " " + num(given) + " is shorter than a row of " + num(row));
+  if (*out * dt_bytes(dt) % 16) return api_fail(std::string(what) + " " + num(given) + " is not a whole number of 16-byte units");
+  if (*out > kMaxRow) return api_fail(std::string(what) + " " + num(*out) + " is above " + num(kMaxRow));
+  return AIH_OK;
+}
+
+int heads_ok(const char *fn, uint32_t hq, uint32_t hkv, uint32_t d, int32_t dt) {
+  if (!dt_ok(dt)) return api_fail(std::string(fn) + ": unknown dtype " + std::to_string(dt));
+  if (d == 0 || d % 8 || d > 256) return api_fail(std::string(fn) + ": d must be a multiple of 8, 8 to 256, not " + num(d));
+  if (hq == 0 || hq > 4096 || hkv > 4096) return api_fail(std::string(fn) + ": heads must be 1 to 4096");
+  return AIH_OK;
+}
+
+hipStream_t stream_of(aih_stream s) { return static_cast<hipStream_t>(s); }
+
+int launched(const char *fn, hipError_t e) {
+  if (e == hipSuccess) return AIH_OK;
+  return api_fail(std::string(fn) + ": launch failed: " + hipGetErrorString(e));
+}
+
+int check_attn(const aih_attn_desc *d, AttnArgs *a) {
+  if (!d) return api_fail("aih_attn: NULL descriptor");
+  if (int rc = heads_ok("aih_attn", d->hq, d->hkv, d->d, d->dt)) return rc;
+  if (d->hkv == 0 || d->hq % d->hkv) return api_fail("aih_attn: hq must be a multiple of hkv");
+  if (d->causal != 0 && d->causal != 1) return api_fail("aih_attn: causal must be 0 or 1");
+  if (d->nseq > 0x7fffffffu || d->tokens > 0x7fffffffu || d->rows > 0x7fffffffu || d->prefix > 0x7fffffffu)
+    return api_fail("aih_attn: counts must be below 2^31");
+  if ((uint64_t)d->tokens * d->hq > 0x7fffffffu) return api_fail("aih_attn: tokens * hq must be below 2^31");
+  if (d->scale != 0.0f && !(d->scale >= 1e-20f && d->scale <= 1e20f))
+    return api_fail("aih_attn: scale must be 0 or 1e-20 to 1e20");
+  *a = AttnArgs{};
+  a->nseq = d->nseq, a->tokens = d->tokens, a->rows = d->rows, a->prefix = d->prefix;
+  a->hq = d->hq, a->hkv = d->hkv, a->g = d->hq / d->hkv, a->d = d->d;
+  a->causal = (uint32_t)d->causal;
+  const double scale = d->scale != 0.0f ? (double)d->scale : 1.0 / std::sqrt((double)d->d);
+  a->scale_log2 = (float)(scale * 1.4426950408889634);
+  if (int rc = take_stride("aih_attn: q_stride", d->q_stride, (uint64_t)d->hq * d->d, d->dt, &a->qs)) return rc;
+  if (int rc = take_stride("aih_attn: o_stride", d->o_stride, (uint64_t)d->hq * d->d, d->dt, &a->os)) return rc;
+  if (int rc = take_stride("aih_attn: k_stride", d->k_stride, (uint64_t)d->hkv * d->d, d->dt, &a->ks)) return rc;
+  if (int rc = take_stride("aih_attn: v_stride", d->v_stride, (uint64_t)d->hkv * d->d, d->dt, &a->vs)) return rc;
+  if (int rc = take_stride("aih_attn: pk_stride", d->pk_stride, (uint64_t)d->hkv * d->d, d->dt, &a->pks)) return rc;
+  if (int rc = take_stride("aih_attn: pv_stride", d->pv_stride, (uint64_t)d->hkv * d->d, d->dt, &a->pvs)) return rc;
+  return AIH_OK;
+}
+
+}  // namespace
+}  // namespace aih
+
+using namespace aih;
+
+extern "C" int aih_qk_norm_rope(const aih_qk_norm_rope_desc *d, const void *x, const void *wq, const void *wk,
+                                const float *cosines, const float *sines, const int32_t *pos, const int32_t *slots,
+                                void *q, void *k, void *v, aih_stream stream) {
+  return api_guarded([&]() -> int {
+    if (!d) return api_fail("aih_qk_norm_rope: NULL descriptor");
+    if (int rc = heads_ok("aih_qk_norm_rope", d->hq, d->hkv, d->d, d->dt)) return rc;
+    if (d->rot % 4 || d->rot > d->d)
+      return api_fail("aih_qk_norm_rope: rot must be a multiple of 4, at most d, not " + num(d->rot));
+    if (d->pairs != 0 && d->pairs != 1) return api_fail("aih_qk_norm_rope: pairs must be 0 or 1");
+    if (!(d->eps >= 0.0f) || !std::isfinite(d->eps)) return api_fail("aih_qk_norm_rope: eps must be >= 0 and finite");
+    if (d->rot && d->positions == 0) return api_fail("aih_qk_norm_rope: the tables need at least one row");
+    if (d->tokens > 0x7fffffffu || d->rows > 0x7fffffffu)
+      return api_fail("aih_qk_norm_rope: counts must be below 2^31");
+    QkRopeArgs a{};
+    const uint64_t heads = (uint64_t)d->hq + 2 * (uint64_t)d->hkv;
+    if (int rc = take_stride("aih_qk_norm_rope: x_stride", d->x_stride, heads * d->d, d->dt, &a.xs)) return rc;
+    if (int rc = take_stride("aih_qk_norm_rope: q_stride", d->q_stride, (uint64_t)d->hq * d->d, d->dt, &a.qs)) return rc;
+    if (int rc = take_stride("aih_qk_norm_rope: k_stride", d->k_stride, (uint64_t)d->hkv * d->d, d->dt, &a.ks)) return rc;
+    if (int rc = take_stride("aih_qk_norm_rope: v_stride", d->v_stride, (uint64_t)d->hkv * d->d, d->dt, &a.vs)) return rc;
+    if (d->tokens == 0) return AIH_OK;
+    if (!x || !q || (d->hkv && !k)) return api_fail("aih_qk_norm_rope: x, q and k must not be NULL");
+    if (d->rot && (!cosines || !sines)) return api_fail("aih_qk_norm_rope: rot > 0 needs cosines and sines");
+    if (!aligned16(x) || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(wq) || !aligned16(wk) ||
+        !aligned16(cosines) || !aligned16(sines))
+      return api_fail("aih_qk_norm_rope: tensors must be aligned to 16 bytes");
+    a.x = x, a.wq = wq, a.wk = wk, a.cs = cosines, a.sn = sines, a.pos = pos, a.slots = slots;
+    a.q = q, a.k = k, a.v = v;
+    a.hq = d->hq, a.hkv = d->hkv, a.ht = d->hq + d->hkv + (v ? d->hkv : 0);
+    a.d = d->d, a.rot = d->rot, a.pairs = (uint32_t)d->pairs;
+    a.positions = d->positions, a.rows = d->rows;
+    a.items = (uint64_t)d->tokens * a.ht;
+    a.eps = d->eps, a.inv_d = 1.0f / (float)d->d;
+    return launched("aih_qk_norm_rope", launch_qk_norm_rope(a, d->dt, stream_of(stream)));
+  });
+}
+
+extern "C" int aih_attn_plan(const aih_attn_desc *d, aih_attn_plan_info *out) {
+  return api_guarded([&]() -> int {
+    AttnArgs a;
+    if (int rc = check_attn(d, &a)) return rc;
+    if (!out) return api_fail("aih_attn_plan: NULL output");
+    *out = aih_attn_plan_info{};
+    return AIH_OK;
+  });
+}
+
+extern "C" int aih_attn(const aih_attn_desc *d, const void *q, const void *k, const void *v, const int32_t *q_start,
+                        const int32_t *k_start, const int32_t *k_len, const void *prefix_k, const void *prefix_v,
+                        void *o, void *ws, size_t ws_bytes, aih_stream stream) {
+  return api_guarded([&]() -> int {
+    AttnArgs a;
+    if (int rc = check_attn(d, &a)) return rc;
+    if (d->nseq == 0 || d->tokens == 0) return AIH_OK;
+    if (!q || !o || !q_start || !k_start || !k_len) return api_fail("aih_attn: NULL tensor");
+    if (d->rows && (!k || !v)) return api_fail("aih_attn: k and v must not be NULL");
+    if (d->prefix && (!prefix_k || !prefix_v)) return api_fail("aih_attn: prefix > 0 needs prefix_k and prefix_v");
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(prefix_k) || !aligned16(prefix_v) ||
+        !aligned16(o) || !aligned16(ws))
+      return api_fail("aih_attn: tensors must be aligned to 16 bytes");
+    a.q = q, a.k = k, a.v = v, a.pk = prefix_k, a.pv = prefix_v, a.o = o, a.ws = static_cast<float *>(ws);
+    a.q_start = q_start, a.k_start = k_start, a.k_len = k_len;
+    return launched("aih_attn", launch_attn_simple(a, d->dt, stream_of(stream)));
+  });
+}
