@@ -26,18 +26,37 @@ struct QkRopeArgs {
 
 hipError_t launch_qk_norm_rope(const QkRopeArgs &a, int dt, hipStream_t st);
 
+// One launch of a tile kernel: either the sequences against their own keys,
+// or (k_start NULL) all rows as one sequence against the shared prefix.
 struct AttnArgs {
-  const void *q, *k, *v, *pk, *pv;
+  const void *q, *k, *v;
   void *o;
-  float *ws;
+  float *ws;  // partial results; NULL: the rows' keys are not cut, o is written
   const int32_t *q_start, *k_start, *k_len;
-  uint64_t qs, ks, vs, os, pks, pvs;  // row strides, elements
-  uint32_t nseq, tokens, rows, prefix;
+  uint64_t qs, ks, vs, os;  // row strides, elements
+  uint32_t nseq, tokens, rows;
   uint32_t hq, hkv, g, d;
   uint32_t causal;
   float scale_log2;  // scale * log2(e)
+  uint32_t tiles;    // row tiles of a key head, at most
+  uint32_t parts, chunk, part0;  // parts of this launch, keys of a part, first part's index in ws
+  uint32_t all_parts;
+  uint32_t nxcd;
 };
 
-hipError_t launch_attn_simple(const AttnArgs &a, int dt, hipStream_t st);
+// The workspace: O of every part [all_parts][tokens * hq][d] fp32, not yet
+// divided by the sum, then (maximum, sum) pairs [all_parts][tokens * hq][2].
+__host__ __device__ inline uint64_t attn_ws_ml(const AttnArgs &a) {
+  return (uint64_t)a.all_parts * a.tokens * a.hq * a.d;
+}
+
+// Rows of a tile (enum aih_attn_kernel).
+uint32_t attn_bm(int kernel, int dt, uint32_t d);
+
+hipError_t launch_attn(const AttnArgs &a, int kernel, int dt, hipStream_t st);
+hipError_t launch_attn_f32(const AttnArgs &a, int kernel, hipStream_t st);
+hipError_t launch_attn_f16(const AttnArgs &a, int kernel, hipStream_t st);
+hipError_t launch_attn_bf16(const AttnArgs &a, int kernel, hipStream_t st);
+hipError_t launch_attn_join(const AttnArgs &a, int dt, hipStream_t st);
 
 }  // namespace aih

@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cmath>
+#include <initializer_list>
 #include <string>
 
 #include "aih_device.h"
@@ -46,7 +47,44 @@ int launched(const char *fn, hipError_t e) {
   return api_fail(std::string(fn) + ": launch failed: " + hipGetErrorString(e));
 }
 
-int check_attn(const aih_attn_desc *d, AttnArgs *a) {
+// How a launch covers its rows and keys.
+struct Cover {
+  int32_t kernel;
+  uint32_t bm, tiles, parts, chunk;
+};
+
+uint32_t div_up(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
+
+// `nseq` sequences of `rows` (query, head of the group) rows altogether, each
+// against about `len` keys.
+Cover cover(uint32_t nseq, uint64_t rows, uint32_t len, uint32_t hkv, int32_t dt, uint32_t d) {
+  const uint32_t cus = device_cus();
+  Cover c{};
+  c.kernel = rows <= 32ull * nseq ? AIH_ATTN_KEYS : AIH_ATTN_ROWS;
+  c.bm = attn_bm(c.kernel, dt, d);
+  c.tiles = nseq == 1 ? div_up(rows, c.bm) : (uint32_t)(rows / c.bm) + nseq;
+  const uint64_t base = (uint64_t)c.tiles * hkv;
+  uint32_t chunk = 1024;
+  if (c.kernel == AIH_ATTN_KEYS) {
+    while (chunk > 256 && base * div_up(len, chunk) < 2 * cus) chunk /= 2;
+    c.parts = div_up(len, chunk);
+  } else {
+    c.parts = base >= 2 * cus ? 1 : div_up(2 * cus, base ? base : 1);
+    if (c.parts > div_up(len, 512)) c.parts = div_up(len, 512);
+    chunk = c.parts ? (div_up(len, c.parts) + 63) / 64 * 64 : 64;
+  }
+  if (c.parts == 0) c.parts = 1;
+  c.chunk = c.parts == 1 ? 0x7fffffe0u : chunk;
+  return c;
+}
+
+struct AttnPlan {
+  Cover own, pre;
+  uint32_t all_parts;
+  uint64_t ws_floats;
+};
+
+int check_attn(const aih_attn_desc *d, AttnArgs *a, AttnPlan *p) {
   if (!d) return api_fail("aih_attn: NULL descriptor");
   if (int rc = heads_ok("aih_attn", d->hq, d->hkv, d->d, d->dt)) return rc;
   if (d->hkv == 0 || d->hq % d->hkv) return api_fail("aih_attn: hq must be a multiple of hkv");
@@ -57,7 +95,8 @@ int check_attn(const aih_attn_desc *d, AttnArgs *a) {
   if (d->scale != 0.0f && !(d->scale >= 1e-20f && d->scale <= 1e20f))
     return api_fail("aih_attn: scale must be 0 or 1e-20 to 1e20");
   *a = AttnArgs{};
-  a->nseq = d->nseq, a->tokens = d->tokens, a->rows = d->rows, a->prefix = d->prefix;
+  *p = AttnPlan{};
+  a->nseq = d->nseq, a->tokens = d->tokens, a->rows = d->rows;
   a->hq = d->hq, a->hkv = d->hkv, a->g = d->hq / d->hkv, a->d = d->d;
   a->causal = (uint32_t)d->causal;
   const double scale = d->scale != 0.0f ? (double)d->scale : 1.0 / std::sqrt((double)d->d);
@@ -66,8 +105,21 @@ int check_attn(const aih_attn_desc *d, AttnArgs *a) {
   if (int rc = take_stride("aih_attn: o_stride", d->o_stride, (uint64_t)d->hq * d->d, d->dt, &a->os)) return rc;
   if (int rc = take_stride("aih_attn: k_stride", d->k_stride, (uint64_t)d->hkv * d->d, d->dt, &a->ks)) return rc;
   if (int rc = take_stride("aih_attn: v_stride", d->v_stride, (uint64_t)d->hkv * d->d, d->dt, &a->vs)) return rc;
-  if (int rc = take_stride("aih_attn: pk_stride", d->pk_stride, (uint64_t)d->hkv * d->d, d->dt, &a->pks)) return rc;
-  if (int rc = take_stride("aih_attn: pv_stride", d->pv_stride, (uint64_t)d->hkv * d->d, d->dt, &a->pvs)) return rc;
+  uint64_t s;
+  if (int rc = take_stride("aih_attn: pk_stride", d->pk_stride, (uint64_t)d->hkv * d->d, d->dt, &s)) return rc;
+  if (int rc = take_stride("aih_attn: pv_stride", d->pv_stride, (uint64_t)d->hkv * d->d, d->dt, &s)) return rc;
+  if (d->nseq == 0 || d->tokens == 0) return AIH_OK;
+  const uint64_t rows = (uint64_t)d->tokens * a->g;
+  p->own = cover(d->nseq, rows, d->max_len ? d->max_len : div_up(d->rows, d->nseq), d->hkv, d->dt, d->d);
+  p->all_parts = p->own.parts;
+  if (d->prefix) {
+    p->pre = cover(1, rows, d->prefix, d->hkv, d->dt, d->d);
+    p->all_parts += p->pre.parts;
+  }
+  for (const Cover *c : {&p->own, &p->pre})
+    if ((uint64_t)c->tiles * d->hkv * c->parts > 0x7fffffffu)
+      return api_fail("aih_attn: more than 2^31 - 1 workgroups");
+  if (p->all_parts > 1) p->ws_floats = (uint64_t)p->all_parts * d->tokens * d->hq * (d->d + 2);
   return AIH_OK;
 }
 
@@ -115,9 +167,16 @@ extern "C" int aih_qk_norm_rope(const aih_qk_norm_rope_desc *d, const void *x, c
 extern "C" int aih_attn_plan(const aih_attn_desc *d, aih_attn_plan_info *out) {
   return api_guarded([&]() -> int {
     AttnArgs a;
-    if (int rc = check_attn(d, &a)) return rc;
+    AttnPlan p;
+    if (int rc = check_attn(d, &a, &p)) return rc;
     if (!out) return api_fail("aih_attn_plan: NULL output");
     *out = aih_attn_plan_info{};
+    out->kernel = p.own.kernel, out->bm = p.own.bm, out->parts = p.own.parts;
+    out->chunk = p.own.parts > 1 ? p.own.chunk : 0;
+    out->prefix_kernel = p.pre.kernel, out->prefix_bm = p.pre.bm, out->prefix_parts = p.pre.parts;
+    out->prefix_chunk = p.pre.parts > 1 ? p.pre.chunk : 0;
+    out->grid = p.own.tiles * d->hkv * p.own.parts;
+    out->ws_bytes = p.ws_floats * 4;
     return AIH_OK;
   });
 }
@@ -127,7 +186,8 @@ extern "C" int aih_attn(const aih_attn_desc *d, const void *q, const void *k, co
                         void *o, void *ws, size_t ws_bytes, aih_stream stream) {
   return api_guarded([&]() -> int {
     AttnArgs a;
-    if (int rc = check_attn(d, &a)) return rc;
+    AttnPlan p;
+    if (int rc = check_attn(d, &a, &p)) return rc;
     if (d->nseq == 0 || d->tokens == 0) return AIH_OK;
     if (!q || !o || !q_start || !k_start || !k_len) return api_fail("aih_attn: NULL tensor");
     if (d->rows && (!k || !v)) return api_fail("aih_attn: k and v must not be NULL");
@@ -135,8 +195,25 @@ extern "C" int aih_attn(const aih_attn_desc *d, const void *q, const void *k, co
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(prefix_k) || !aligned16(prefix_v) ||
         !aligned16(o) || !aligned16(ws))
       return api_fail("aih_attn: tensors must be aligned to 16 bytes");
-    a.q = q, a.k = k, a.v = v, a.pk = prefix_k, a.pv = prefix_v, a.o = o, a.ws = static_cast<float *>(ws);
+    if (p.ws_floats && (!ws || ws_bytes < p.ws_floats * 4))
+      return api_fail("aih_attn: the workspace needs " + num(p.ws_floats * 4) + " bytes, not " + num(ws ? ws_bytes : 0));
+    const hipStream_t st = stream_of(stream);
+    a.q = q, a.k = k, a.v = v, a.o = o, a.ws = p.ws_floats ? static_cast<float *>(ws) : nullptr;
     a.q_start = q_start, a.k_start = k_start, a.k_len = k_len;
-    return launched("aih_attn", launch_attn_simple(a, d->dt, stream_of(stream)));
+    a.all_parts = p.all_parts;
+    a.nxcd = device_xcds();
+    if (d->prefix) {
+      AttnArgs b = a;
+      b.k = prefix_k, b.v = prefix_v, b.k_start = nullptr;
+      b.ks = d->pk_stride ? d->pk_stride : (uint64_t)d->hkv * d->d;
+      b.vs = d->pv_stride ? d->pv_stride : (uint64_t)d->hkv * d->d;
+      b.rows = d->prefix, b.causal = 0;
+      b.tiles = p.pre.tiles, b.parts = p.pre.parts, b.chunk = p.pre.chunk, b.part0 = 0;
+      if (int rc = launched("aih_attn", launch_attn(b, p.pre.kernel, d->dt, st))) return rc;
+    }
+    a.tiles = p.own.tiles, a.parts = p.own.parts, a.chunk = p.own.chunk, a.part0 = p.pre.parts;
+    if (int rc = launched("aih_attn", launch_attn(a, p.own.kernel, d->dt, st))) return rc;
+    if (!a.ws) return AIH_OK;
+    return launched("aih_attn", launch_attn_join(a, d->dt, st));
   });
 }

@@ -1,0 +1,10 @@
+// attn_f32.hip -- the f32 instances of the attention kernel (attn_impl.h).
+#include "attn_impl.h"
+
+namespace aih {
+
+hipError_t launch_attn_f32(const AttnArgs &a, int kernel, hipStream_t st) {
+  return at_launch_dt<DT_F32>(a, kernel, st);
+}
+
+}  // namespace aih
