@@ -158,6 +158,8 @@ class AttnSpec:
         n = self.workspace_bytes()
         if n:
             ws = conv._workspace(n, ws, conv._device_of(out))
+            if not isinstance(ws, int) and ws.numel() * ws.element_size() < n:
+                raise AihError(f"the workspace needs {n} bytes, not {ws.numel() * ws.element_size()}")
         p = conv._ptr
         conv._check(lib().aih_attn(C.byref(self._desc), p(q), p(k), p(v), p(q_start), p(k_start), p(k_len),
                                    p(prefix_k), p(prefix_v), p(out), p(ws) if n else None, n, conv._stream(stream)))

@@ -3,6 +3,7 @@
 // device knows (lengths, positions, slots) the kernels bound themselves.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <initializer_list>
 #include <string>
@@ -110,7 +111,8 @@ int check_attn(const aih_attn_desc *d, AttnArgs *a, AttnPlan *p) {
   if (int rc = take_stride("aih_attn: pv_stride", d->pv_stride, (uint64_t)d->hkv * d->d, d->dt, &s)) return rc;
   if (d->nseq == 0 || d->tokens == 0) return AIH_OK;
   const uint64_t rows = (uint64_t)d->tokens * a->g;
-  p->own = cover(d->nseq, rows, d->max_len ? d->max_len : div_up(d->rows, d->nseq), d->hkv, d->dt, d->d);
+  const uint32_t len = d->max_len ? std::min(d->max_len, d->rows) : div_up(d->rows, d->nseq);
+  p->own = cover(d->nseq, rows, len, d->hkv, d->dt, d->d);
   p->all_parts = p->own.parts;
   if (d->prefix) {
     p->pre = cover(1, rows, d->prefix, d->hkv, d->dt, d->d);
