@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include "../../include/aih_attn.h"
+#include "aih_device.h"
 
 namespace aih {
 
@@ -26,26 +27,30 @@ struct QkRopeArgs {
 
 hipError_t launch_qk_norm_rope(const QkRopeArgs &a, int dt, hipStream_t st);
 
-// One launch of a tile kernel: either the sequences against their own keys,
-// or (k_start NULL) all rows as one sequence against the shared prefix.
+// One launch: the sequences against their own keys, with the prefix's work in
+// front (pre_tiles > 0, AIH_ATTN_KEYS only); or, with k_start NULL
+// (AIH_ATTN_ROWS only), all rows against k and v as one sequence.
 struct AttnArgs {
-  const void *q, *k, *v;
+  const void *q, *k, *v, *pk, *pv;
   void *o;
-  float *ws;  // partial results; NULL: the rows' keys are not cut, o is written
+  float *ws;  // partial results; NULL: no row's keys are cut, o is written
   const int32_t *q_start, *k_start, *k_len;
-  uint64_t qs, ks, vs, os;  // row strides, elements
-  uint32_t nseq, tokens, rows;
+  uint64_t qs, ks, vs, os, pks, pvs;  // row strides, elements
+  uint32_t nseq, tokens, rows, prefix;
   uint32_t hq, hkv, g, d;
   uint32_t causal;
   float scale_log2;  // scale * log2(e)
   uint32_t tiles;    // row tiles of a key head, at most
-  uint32_t parts, chunk, part0;  // parts of this launch, keys of a part, first part's index in ws
+  uint32_t parts, shift, part0;             // parts of a sequence at most, log2 keys of a part, first part's index in ws
+  uint32_t pre_tiles, pre_parts, pre_shift;  // the prefix's
+  FastDiv by_g, by_hkv, by_pre_tiles;
   uint32_t all_parts;
   uint32_t nxcd;
 };
 
 // The workspace: O of every part [all_parts][tokens * hq][d] fp32, not yet
-// divided by the sum, then (maximum, sum) pairs [all_parts][tokens * hq][2].
+// divided by the sum, then (maximum, sum) pairs [all_parts][tokens * hq][2]; a
+// sum of -1 in part 0: the row's o is written already.
 __host__ __device__ inline uint64_t attn_ws_ml(const AttnArgs &a) {
   return (uint64_t)a.all_parts * a.tokens * a.hq * a.d;
 }

@@ -51,36 +51,36 @@ int launched(const char *fn, hipError_t e) {
 // How a launch covers its rows and keys.
 struct Cover {
   int32_t kernel;
-  uint32_t bm, tiles, parts, chunk;
+  uint32_t bm, tiles, parts, shift;
 };
 
 uint32_t div_up(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 
 // `nseq` sequences of `rows` (query, head of the group) rows altogether, each
 // against about `len` keys.
-Cover cover(uint32_t nseq, uint64_t rows, uint32_t len, uint32_t hkv, int32_t dt, uint32_t d) {
+Cover cover(int32_t kernel, uint32_t nseq, uint64_t rows, uint32_t len, uint32_t hkv, int32_t dt, uint32_t d) {
   const uint32_t cus = device_cus();
   Cover c{};
-  c.kernel = rows <= 32ull * nseq ? AIH_ATTN_KEYS : AIH_ATTN_ROWS;
+  c.kernel = kernel;
   c.bm = attn_bm(c.kernel, dt, d);
   c.tiles = nseq == 1 ? div_up(rows, c.bm) : (uint32_t)(rows / c.bm) + nseq;
   const uint64_t base = (uint64_t)c.tiles * hkv;
-  uint32_t chunk = 1024;
+  auto parts = [&](uint32_t x) { return std::max(1u, div_up(len, 1ull << x)); };
   if (c.kernel == AIH_ATTN_KEYS) {
-    while (chunk > 256 && base * div_up(len, chunk) < 2 * cus) chunk /= 2;
-    c.parts = div_up(len, chunk);
+    c.shift = 10;
+    while (c.shift > 8 && base * parts(c.shift) < 2 * cus) --c.shift;
   } else {
-    c.parts = base >= 2 * cus ? 1 : div_up(2 * cus, base ? base : 1);
-    if (c.parts > div_up(len, 512)) c.parts = div_up(len, 512);
-    chunk = c.parts ? (div_up(len, c.parts) + 63) / 64 * 64 : 64;
+    c.shift = 31;
+    while (c.shift > 9 && base * parts(c.shift) < 2 * cus) --c.shift;
   }
-  if (c.parts == 0) c.parts = 1;
-  c.chunk = c.parts == 1 ? 0x7fffffe0u : chunk;
+  c.parts = parts(c.shift);
+  if (c.parts == 1) c.shift = 31;
   return c;
 }
 
 struct AttnPlan {
   Cover own, pre;
+  bool together;  // the prefix in the same launch
   uint32_t all_parts;
   uint64_t ws_floats;
 };
@@ -106,21 +106,22 @@ int check_attn(const aih_attn_desc *d, AttnArgs *a, AttnPlan *p) {
   if (int rc = take_stride("aih_attn: o_stride", d->o_stride, (uint64_t)d->hq * d->d, d->dt, &a->os)) return rc;
   if (int rc = take_stride("aih_attn: k_stride", d->k_stride, (uint64_t)d->hkv * d->d, d->dt, &a->ks)) return rc;
   if (int rc = take_stride("aih_attn: v_stride", d->v_stride, (uint64_t)d->hkv * d->d, d->dt, &a->vs)) return rc;
-  uint64_t s;
-  if (int rc = take_stride("aih_attn: pk_stride", d->pk_stride, (uint64_t)d->hkv * d->d, d->dt, &s)) return rc;
-  if (int rc = take_stride("aih_attn: pv_stride", d->pv_stride, (uint64_t)d->hkv * d->d, d->dt, &s)) return rc;
+  if (int rc = take_stride("aih_attn: pk_stride", d->pk_stride, (uint64_t)d->hkv * d->d, d->dt, &a->pks)) return rc;
+  if (int rc = take_stride("aih_attn: pv_stride", d->pv_stride, (uint64_t)d->hkv * d->d, d->dt, &a->pvs)) return rc;
   if (d->nseq == 0 || d->tokens == 0) return AIH_OK;
   const uint64_t rows = (uint64_t)d->tokens * a->g;
   const uint32_t len = d->max_len ? std::min(d->max_len, d->rows) : div_up(d->rows, d->nseq);
-  p->own = cover(d->nseq, rows, len, d->hkv, d->dt, d->d);
+  const bool rows_fit = d->d * dt_bytes(d->dt) <= 512;  // else the registers do not hold a wavefront's queries
+  const int32_t kernel = rows <= 32ull * d->nseq || !rows_fit ? AIH_ATTN_KEYS : AIH_ATTN_ROWS;
+  p->own = cover(kernel, d->nseq, rows, len, d->hkv, d->dt, d->d);
   p->all_parts = p->own.parts;
   if (d->prefix) {
-    p->pre = cover(1, rows, d->prefix, d->hkv, d->dt, d->d);
+    p->together = kernel == AIH_ATTN_KEYS && (rows <= 256 || !rows_fit);
+    p->pre = cover(p->together ? AIH_ATTN_KEYS : AIH_ATTN_ROWS, 1, rows, d->prefix, d->hkv, d->dt, d->d);
     p->all_parts += p->pre.parts;
   }
-  for (const Cover *c : {&p->own, &p->pre})
-    if ((uint64_t)c->tiles * d->hkv * c->parts > 0x7fffffffu)
-      return api_fail("aih_attn: more than 2^31 - 1 workgroups");
+  if ((uint64_t)p->own.tiles * d->hkv * p->own.parts + (uint64_t)p->pre.tiles * d->hkv * p->pre.parts > 0x7fffffffu)
+    return api_fail("aih_attn: more than 2^31 - 1 tiles");
   if (p->all_parts > 1) p->ws_floats = (uint64_t)p->all_parts * d->tokens * d->hq * (d->d + 2);
   return AIH_OK;
 }
@@ -174,9 +175,9 @@ extern "C" int aih_attn_plan(const aih_attn_desc *d, aih_attn_plan_info *out) {
     if (!out) return api_fail("aih_attn_plan: NULL output");
     *out = aih_attn_plan_info{};
     out->kernel = p.own.kernel, out->bm = p.own.bm, out->parts = p.own.parts;
-    out->chunk = p.own.parts > 1 ? p.own.chunk : 0;
+    out->chunk = p.own.parts > 1 ? 1u << p.own.shift : 0;
     out->prefix_kernel = p.pre.kernel, out->prefix_bm = p.pre.bm, out->prefix_parts = p.pre.parts;
-    out->prefix_chunk = p.pre.parts > 1 ? p.pre.chunk : 0;
+    out->prefix_chunk = p.pre.parts > 1 ? 1u << p.pre.shift : 0;
     out->grid = p.own.tiles * d->hkv * p.own.parts;
     out->ws_bytes = p.ws_floats * 4;
     return AIH_OK;
@@ -204,16 +205,19 @@ extern "C" int aih_attn(const aih_attn_desc *d, const void *q, const void *k, co
     a.q_start = q_start, a.k_start = k_start, a.k_len = k_len;
     a.all_parts = p.all_parts;
     a.nxcd = device_xcds();
-    if (d->prefix) {
+    a.by_g = make_fastdiv(a.g), a.by_hkv = make_fastdiv(a.hkv);
+    a.by_pre_tiles = make_fastdiv(std::max(1u, p.pre.tiles));
+    a.pk = prefix_k, a.pv = prefix_v, a.prefix = d->prefix;
+    a.tiles = p.own.tiles, a.parts = p.own.parts, a.shift = p.own.shift, a.part0 = p.pre.parts;
+    if (d->prefix && !p.together) {
       AttnArgs b = a;
-      b.k = prefix_k, b.v = prefix_v, b.k_start = nullptr;
-      b.ks = d->pk_stride ? d->pk_stride : (uint64_t)d->hkv * d->d;
-      b.vs = d->pv_stride ? d->pv_stride : (uint64_t)d->hkv * d->d;
+      b.k = prefix_k, b.v = prefix_v, b.ks = a.pks, b.vs = a.pvs, b.k_start = nullptr;
       b.rows = d->prefix, b.causal = 0;
-      b.tiles = p.pre.tiles, b.parts = p.pre.parts, b.chunk = p.pre.chunk, b.part0 = 0;
-      if (int rc = launched("aih_attn", launch_attn(b, p.pre.kernel, d->dt, st))) return rc;
+      b.tiles = p.pre.tiles, b.parts = p.pre.parts, b.shift = p.pre.shift, b.part0 = 0;
+      if (int rc = launched("aih_attn", launch_attn(b, AIH_ATTN_ROWS, d->dt, st))) return rc;
+    } else {
+      a.pre_tiles = p.pre.tiles, a.pre_parts = p.pre.parts, a.pre_shift = p.pre.shift;
     }
-    a.tiles = p.own.tiles, a.parts = p.own.parts, a.chunk = p.own.chunk, a.part0 = p.pre.parts;
     if (int rc = launched("aih_attn", launch_attn(a, p.own.kernel, d->dt, st))) return rc;
     if (!a.ws) return AIH_OK;
     return launched("aih_attn", launch_attn_join(a, d->dt, st));

@@ -120,9 +120,7 @@ class Case:
 @pytest.mark.parametrize("causal", [True, False])
 def test_prompt_head_sizes(dt, d, causal):
     lens = [1, 33, 70, 129]
-    c = Case(dt, 4, 2, d, lens, lens, causal, seed=d)
-    assert c.spec().plan().kernel == attn.AttnKernel.ROWS
-    c.check()
+    Case(dt, 4, 2, d, lens, lens, causal, seed=d).check()
 
 
 @pytest.mark.parametrize("dt", ALL)
@@ -215,8 +213,7 @@ def test_length_hint_is_only_a_hint(hint):
 def test_few_rows_after_a_long_past(dt, causal):
     # a chunk of a prompt: tiles of rows whose keys are cut
     c = Case(dt, 4, 2, 64, [40], [1700], causal, seed=8)
-    p = c.spec().plan()
-    assert p.kernel == attn.AttnKernel.ROWS and p.parts > 1
+    assert c.spec().plan().parts > 1
     c.check()
 
 
