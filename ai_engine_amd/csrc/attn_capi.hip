@@ -66,7 +66,7 @@ Cover cover(int32_t kernel, uint32_t nseq, uint64_t rows, uint32_t len, uint32_t
   c.tiles = nseq == 1 ? div_up(rows, c.bm) : (uint32_t)(rows / c.bm) + nseq;
   const uint64_t base = (uint64_t)c.tiles * hkv;
   auto parts = [&](uint32_t x) { return std::max(1u, div_up(len, 1ull << x)); };
-  if (c.kernel == AIH_ATTN_KEYS) {
+  if (c.kernel == AIH_ATTN_KEYS && rows <= 32ull * nseq) {
     c.shift = 10;
     while (c.shift > 8 && base * parts(c.shift) < 2 * cus) --c.shift;
   } else {
@@ -112,7 +112,11 @@ int check_attn(const aih_attn_desc *d, AttnArgs *a, AttnPlan *p) {
   const uint64_t rows = (uint64_t)d->tokens * a->g;
   const uint32_t len = d->max_len ? std::min(d->max_len, d->rows) : div_up(d->rows, d->nseq);
   const bool rows_fit = d->d * dt_bytes(d->dt) <= 512;  // else the registers do not hold a wavefront's queries
-  const int32_t kernel = rows <= 32ull * d->nseq || !rows_fit ? AIH_ATTN_KEYS : AIH_ATTN_ROWS;
+  // fp32 prompts of few tiles: a wavefront's 32 rows against all keys are a chain
+  // of slow products that sets the time, so the keys go over the wavefronts
+  const uint64_t tiles = (uint64_t)d->hkv * (div_up(rows, attn_bm(AIH_ATTN_ROWS, d->dt, d->d)) + d->nseq / 2);
+  const bool chain = d->dt == AIH_F32 && tiles < (d->d <= 64 ? 4 : 2) * (uint64_t)device_cus();
+  const int32_t kernel = rows <= 32ull * d->nseq || !rows_fit || chain ? AIH_ATTN_KEYS : AIH_ATTN_ROWS;
   p->own = cover(kernel, d->nseq, rows, len, d->hkv, d->dt, d->d);
   p->all_parts = p->own.parts;
   if (d->prefix) {

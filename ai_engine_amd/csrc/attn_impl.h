@@ -105,20 +105,41 @@ __device__ __forceinline__ uint32_t at_vswz(uint32_t r) {
 // DMA of instructions i0 .. i0 + NI - 1 of a tile (1 KB, RPI rows each): lane ->
 // row i RPI + lane / PU, slot lane % PU. Rows past `rows` and units past the
 // head land as zeros.
+//
+// Written out, because the compiler makes every transposing LDS read wait for
+// all copies it knows of, those of the next stage too (it cannot tell their
+// places apart). The kernels wait for a stage's copies themselves
+// (at_wait_vm); no register is written, and a count that the compiler waits for
+// on behalf of its own loads only gets stricter by copies it does not know of.
 template <class T, int NI, bool V>
 __device__ __forceinline__ void at_dma(const char *base, uint32_t stride, uint32_t rows, uint32_t du, int i0, int lane,
                                        char *dst) {
-  const uint32_t len = rows ? (rows - 1) * stride + du * 16 : 0;
-  const __amdgpu_buffer_rsrc_t rs = at_rsrc(base, len);
+  const uint64_t at = reinterpret_cast<uint64_t>(base);
+  const u32x4 rs = {(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)at),
+                    (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32) & 0xffffu),
+                    (uint32_t)__builtin_amdgcn_readfirstlane(rows ? (rows - 1) * stride + du * 16 : 0), 0x00020000u};
   const uint32_t lr = lane / T::PU, ls = lane % T::PU;
   const uint32_t lu = ls ^ (V ? at_vswz<T>(lr) : at_kswz<T>(lr));
+  const uint32_t to = (uint32_t)(uintptr_t)(at_lds_void *)dst;
 #pragma unroll
   for (int k = 0; k < NI; ++k) {
     const uint32_t i = i0 + k;
     // rows i RPI and lr share no bit, so the XORs add up
     const uint32_t u = lu ^ (T::PU < 8 ? 0 : V ? at_vswz<T>(i * T::RPI) : at_kswz<T>(i * T::RPI));
     const uint32_t off = u < du ? u * 16 + (i * T::RPI + lr) * stride : kAtOob;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (at_lds_void *)(dst + i * 1024), 16, off, 0, 0, 0);
+    const uint32_t m0 = __builtin_amdgcn_readfirstlane(to + i * 1024);
+    // one wait state after m0; five after a vector instruction that may have
+    // written the descriptor
+    if (k == 0)
+      __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                       :
+                       : "s"(m0), "v"(off), "s"(rs)
+                       : "memory", "m0");
+    else
+      __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                       :
+                       : "s"(m0), "v"(off), "s"(rs)
+                       : "memory", "m0");
   }
 }
 

@@ -90,7 +90,8 @@ __global__ __launch_bounds__(64 * C::WK, C::WPE) void attn_keys_kernel(AttnArgs 
       const uint32_t at = item - base - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(n, l));
       const uint32_t rest = fdiv(at, a.by_hkv);
       hk = at - rest * a.hkv;
-      part = nt == 1 ? rest : rest / nt, tile = rest - part * nt;
+      part = nt == 1 ? rest : rest / nt;
+      tile = nt - 1 - (rest - part * nt);  // the last rows see the most keys: they go first
       shift = at_shift(a, s.len);
       causal = a.causal, gpart = a.part0 + part;
       kp = (const char *)a.k, vp = (const char *)a.v, ks = a.ks, vs = a.vs;
@@ -249,7 +250,11 @@ hipError_t at_launch_keys(const AttnArgs &a, uint32_t cus, hipStream_t st) {
       v = 1;
     return v;
   }();
-  const uint64_t room = (uint64_t)cus * occ;
+  // Uncut keys: one item a workgroup, handed out as others end. Cut ones: the
+  // items are many small ones, and of those that the host counts (the longest
+  // length for all) few may exist, so the workgroups that run at once share
+  // them.
+  const uint64_t room = a.parts == 1 ? items : (uint64_t)cus * occ;
   hipLaunchKernelGGL((attn_keys_kernel<C>), dim3((uint32_t)(items < room ? items : room)), dim3(64 * C::WK), C::LDS, st,
                      a);
   return hipGetLastError();

@@ -11,21 +11,21 @@ namespace {
 template <int DT, int DP, int WR_, int NQ, int KB>
 struct AtRowsCfg {
   using T = AtTile<DT, DP, NQ, KB>;
-  static constexpr int WR = WR_, NST = 2;
+  static constexpr int WR = WR_;
   static constexpr int BM = 32 * NQ * WR;
   static constexpr uint32_t HALF = T::KEYS * T::RB, STAGE = 2 * HALF;
-  static constexpr uint32_t LDS = NST * STAGE;
+  static constexpr uint32_t LDS = 2 * STAGE;
   static constexpr int NI = T::KEYS / T::RPI / WR;  // K instructions of a wavefront per stage, and as many of V
   // wavefronts a SIMD that the registers have to leave room for
-  static constexpr int WPE = DP <= 128 ? 2 : 1;
-  static_assert(NI >= 1 && 2 * NI * (NST - 2) < 64, "DMA instructions in flight");
+  static constexpr int WPE = DP <= 64 ? 3 : DP <= 128 ? 2 : 1;
+  static_assert(NI >= 1, "DMA instructions");
   static_assert(LDS <= 160 * 1024, "LDS");
 };
 
 template <class C>
 __global__ __launch_bounds__(64 * C::WR, C::WPE) void attn_rows_kernel(AttnArgs a) {
   using T = typename C::T;
-  constexpr int NQ = T::NQ, DB = T::DB, NST = C::NST, EB = T::EB;
+  constexpr int NQ = T::NQ, DB = T::DB, EB = T::EB;
   extern __shared__ __align__(16) char lds[];
 
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, lh = lane >> 5;
@@ -117,39 +117,50 @@ __global__ __launch_bounds__(64 * C::WR, C::WPE) void attn_rows_kernel(AttnArgs 
     for (int db = 0; db < DB; ++db) o[db][i] = f32x16{};
   }
 
-  auto compute = [&](uint32_t st, uint32_t b) {
+  // EDGE: a stage that some of the wavefront's rows see in part, or not at all
+  auto compute = [&](uint32_t st, uint32_t b, auto edge) {
+    constexpr bool EDGE = decltype(edge)::value;
     const uint32_t key = kbeg + st * T::KEYS;
-    if (key >= min(kend, wmax)) return;
+    if (EDGE && key >= min(kend, wmax)) return;
     const char *kt = lds + b * C::STAGE, *vt = kt + C::HALF;
     f32x16 sc[T::KB][NQ];
     u32x4 pb[T::KB][2][NQ];
     at_qk<T>(kt, [&](int i, int c) { return q[i][c]; }, sc, lane);
-    uint32_t to[NQ];
+    if constexpr (EDGE) {
+      uint32_t to[NQ];
 #pragma unroll
-    for (int i = 0; i < NQ; ++i) to[i] = max(min(kend, lim[i]), key) - key;
-    if (key + T::KEYS > min(kend, wmin)) at_mask<T>(sc, to, lane);
-    at_softmax<T>(sc, pb, m, l, o, a.scale_log2);
-    if (wmin < min(kend, key + T::KEYS) && at_spread_nonfinite<T>(vt, to, o, lane))
-      at_pv<T, true>(vt, sc, pb, o, lane);
-    else
-      at_pv<T, false>(vt, sc, pb, o, lane);
+      for (int i = 0; i < NQ; ++i) to[i] = max(min(kend, lim[i]), key) - key;
+      at_mask<T>(sc, to, lane);
+      at_softmax<T>(sc, pb, m, l, o, a.scale_log2);
+      if (wmin < min(kend, key + T::KEYS) && at_spread_nonfinite<T>(vt, to, o, lane)) {
+        at_pv<T, true>(vt, sc, pb, o, lane);
+        return;
+      }
+    } else {
+      at_softmax<T>(sc, pb, m, l, o, a.scale_log2);
+    }
+    at_pv<T, false>(vt, sc, pb, o, lane);
   };
 
   const uint32_t nst = kend > kbeg ? (kend - kbeg + T::KEYS - 1) / T::KEYS : 0;
-#pragma unroll
-  for (int i = 0; i < NST - 1; ++i) issue(i, i);
-  uint32_t bc = 0, bi = NST - 1;
-  for (uint32_t st = 0; st < nst; ++st) {
+  const uint32_t whole = min(kend, wmin);  // keys that every row of the wavefront sees
+  const uint32_t nfull = whole > kbeg ? (whole - kbeg) / T::KEYS : 0;
+  issue(0, 0);
+  // Every wavefront takes nst turns, some of them with other rows' stages whole
+  // and its own at the edge: the loop is cut in two per wavefront, the barriers
+  // are the same.
+  auto turn = [&](uint32_t st, auto edge) {
     // every wavefront's copies of the stage are in LDS, and every wavefront is
     // done reading the buffer that is requested next. A bare barrier:
     // __syncthreads() would also wait for the copies still in flight.
-    at_wait_vm<2 * C::NI *(NST - 2)>();
+    at_wait_vm<0>();
     __asm__ volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    issue(st + NST - 1, bi);
-    compute(st, bc);
-    bc = bc + 1 == NST ? 0 : bc + 1;
-    bi = bi + 1 == NST ? 0 : bi + 1;
-  }
+    issue(st + 1, (st + 1) & 1);
+    compute(st, st & 1, edge);
+  };
+  uint32_t st = 0;
+  for (; st < nfull; ++st) turn(st, std::false_type{});
+  for (; st < nst; ++st) turn(st, std::true_type{});
   at_wait_vm<0>();  // nothing may still be on its way into LDS at the end
 
   const uint64_t rows_all = (uint64_t)a.tokens * a.hq;
