@@ -342,13 +342,17 @@ __device__ __forceinline__ AtSeq at_seq_of(const AtSeq &s, int l) {
   return AtSeq{(uint32_t)__builtin_amdgcn_readlane(s.q0, l), (uint32_t)__builtin_amdgcn_readlane(s.lq, l),
                (uint32_t)__builtin_amdgcn_readlane(s.k0, l), (uint32_t)__builtin_amdgcn_readlane(s.len, l)};
 }
-__device__ __forceinline__ uint32_t at_scan(uint32_t v, uint32_t lane) {  // inclusive prefix sum of a wavefront
-#pragma unroll
-  for (uint32_t w = 1; w < 64; w <<= 1) {
-    const uint32_t o = __shfl_up(v, w);
-    if (lane >= w) v += o;
-  }
-  return v;
+// Inclusive prefix sum over a wavefront: within rows of 16 lanes by shifts, then
+// a row's total into the next row and the first half's into the second.
+__device__ __forceinline__ uint32_t at_scan(uint32_t v) {
+  int x = (int)v;
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);   // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);   // row_shr:2
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);   // row_shr:4
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);   // row_shr:8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
+  return (uint32_t)x;
 }
 
 // Keys that (query, head of the group) row `row` of a sequence sees.

@@ -11,22 +11,25 @@ namespace {
 // WK wavefronts, each with its own 32 keys of a stage in LDS. One buffer for
 // K and one for V: K's is free again after the scores, V's after the product,
 // so the next stage's K arrives during the softmax and the product, its V
-// during the next scores.
+// during the next scores. ONE: the two take turns in one buffer, where LDS would
+// otherwise hold one wavefront a SIMD: fp32 heads above 64 elements, whose long
+// products of one wavefront cover the waits and the softmax of another.
 template <int DT, int DP, int WK_>
 struct AtKeysCfg {
   using T = AtTile<DT, DP, 1, 1>;
   static constexpr int WK = WK_;
   static constexpr int KEYS = 32 * WK;
+  static constexpr bool ONE = T::RB >= 512 && T::F32;
   static constexpr uint32_t HALF = 32 * T::RB;   // K or V of a wavefront
+  static constexpr uint32_t MINE = ONE ? HALF : 2 * HALF;
   static constexpr int NI = 32 / T::RPI;         // DMA instructions of a half
   static constexpr int OPITCH = DP + 4;
   // the join of the wavefronts' results reuses the buffers
   static constexpr uint32_t JOIN = WK * 32u * OPITCH * 4 + WK * 64u * 4;
-  static constexpr uint32_t BUF = 2 * WK * HALF > JOIN ? 2 * WK * HALF : JOIN;
-  // fp32 heads of more than 128 elements: the queries in LDS, the registers
-  // hold the results
-  static constexpr bool QL = T::RB >= 1024;
-  static constexpr uint32_t LDS = BUF + (QL ? HALF : 0);
+  static constexpr uint32_t BUF = WK * MINE;
+  // then also the queries are in LDS: the registers hold the results
+  static constexpr bool QL = ONE;
+  static constexpr uint32_t LDS = BUF + (QL ? HALF : 0) > JOIN ? BUF + (QL ? HALF : 0) : JOIN;
   // workgroups of a CU, and with that wavefronts of a SIMD, that LDS has room for
   static constexpr int WPE = 2 * LDS <= 160 * 1024 ? 2 : 1;
   static_assert(NI >= 1 && NI < 64, "DMA instructions in flight");
@@ -46,7 +49,7 @@ __global__ __launch_bounds__(64 * C::WK, C::WPE) void attn_keys_kernel(AttnArgs 
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint64_t rows_all = (uint64_t)a.tokens * a.hq;
   const uint64_t ml0 = attn_ws_ml(a);
-  char *kt = lds + wave * 2 * C::HALF, *vt = kt + C::HALF;
+  char *kt = lds + wave * C::MINE, *vt = C::ONE ? kt : kt + C::HALF;
 
   // 64 sequences at a time, one a lane: items up to and including each
   const uint32_t pre_items = a.pre_tiles * a.pre_parts * a.hkv;
@@ -58,7 +61,7 @@ __global__ __launch_bounds__(64 * C::WK, C::WPE) void attn_keys_kernel(AttnArgs 
     const uint32_t x = at_shift(a, mine.len);
     parts = max(1u, (uint32_t)(((uint64_t)mine.len + (1ull << x) - 1) >> x));
     n = tiles * parts * a.hkv;
-    sum = at_scan(n, lane);
+    sum = at_scan(n);
   };
   count();
 
@@ -129,7 +132,7 @@ __global__ __launch_bounds__(64 * C::WK, C::WPE) void attn_keys_kernel(AttnArgs 
     }
     uint32_t key = kbeg + wave * 32;
     issue_k(key);
-    issue_v(key);
+    if constexpr (!C::ONE) issue_v(key);
     auto query = [&](int, int c) -> u32x4 {
       if constexpr (C::QL) return *reinterpret_cast<const u32x4 *>(ql + (((2 * c + lh) ^ at_kswz<T>(l32)) * 16));
       else return q[c];
@@ -144,23 +147,25 @@ __global__ __launch_bounds__(64 * C::WK, C::WPE) void attn_keys_kernel(AttnArgs 
     for (; key < kend; key += C::KEYS) {
       f32x16 sc[1][1];
       u32x4 pb[1][2][1];
-      at_wait_vm<C::NI>();  // K is there, V may still be on its way
+      at_wait_vm<C::ONE ? 0 : C::NI>();  // K is there, V may still be on its way
       __asm__ volatile("" ::: "memory");
       at_qk<T>(kt, query, sc, lane);
       // K's buffer is requested again: its reads are behind this wavefront
       __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      issue_k(key + C::KEYS);
+      if constexpr (C::ONE) issue_v(key);
+      else issue_k(key + C::KEYS);
       const uint32_t to[1] = {max(min(kend, lim), key) - key};
       if (key + 32 > min(kend, smin)) at_mask<T>(sc, to, lane);
       at_softmax<T>(sc, pb, m, l, o, a.scale_log2);
-      at_wait_vm<C::NI>();  // V is there, the next K on its way
+      at_wait_vm<C::ONE ? 0 : C::NI>();  // V is there, the next K on its way
       __asm__ volatile("" ::: "memory");
       if (smin < min(kend, key + 32) && at_spread_nonfinite<T>(vt, to, o, lane))
         at_pv<T, true>(vt, sc, pb, o, lane);
       else
         at_pv<T, false>(vt, sc, pb, o, lane);
       __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      issue_v(key + C::KEYS);
+      if constexpr (C::ONE) issue_k(key + C::KEYS);
+      else issue_v(key + C::KEYS);
     }
     at_wait_vm<0>();  // nothing is on its way into LDS any more
     l[0] = at_pair_sum(l[0]);
@@ -261,7 +266,7 @@ hipError_t at_launch_keys(const AttnArgs &a, uint32_t cus, hipStream_t st) {
 }
 
 template <int DT, int DP>
-using AtKeys = AtKeysCfg<DT, DP, (DP == 96 ? 128 : DP) * Storage<DT>::bytes >= 1024 ? 2 : 4>;
+using AtKeys = AtKeysCfg<DT, DP, 4>;
 
 }  // namespace
 }  // namespace aih

@@ -7,18 +7,18 @@
 namespace aih {
 namespace {
 
-// WR wavefronts of 32 NQ rows; stages of 32 KB keys, two of them in LDS.
-template <int DT, int DP, int WR_, int NQ, int KB>
+// WR wavefronts of 32 NQ rows; stages of 32 KB keys, NST of them in LDS.
+template <int DT, int DP, int WR_, int NQ, int KB, int NST_>
 struct AtRowsCfg {
   using T = AtTile<DT, DP, NQ, KB>;
-  static constexpr int WR = WR_;
+  static constexpr int WR = WR_, NST = NST_;
   static constexpr int BM = 32 * NQ * WR;
   static constexpr uint32_t HALF = T::KEYS * T::RB, STAGE = 2 * HALF;
-  static constexpr uint32_t LDS = 2 * STAGE;
+  static constexpr uint32_t LDS = NST * STAGE;
   static constexpr int NI = T::KEYS / T::RPI / WR;  // K instructions of a wavefront per stage, and as many of V
   // wavefronts a SIMD that the registers have to leave room for
   static constexpr int WPE = DP <= 64 ? 3 : DP <= 128 ? 2 : 1;
-  static_assert(NI >= 1, "DMA instructions");
+  static_assert(NI >= 1 && 2 * NI * (NST - 2) < 64, "DMA instructions in flight");
   static_assert(LDS <= 160 * 1024, "LDS");
 };
 
@@ -42,7 +42,7 @@ __global__ __launch_bounds__(64 * C::WR, C::WPE) void attn_rows_kernel(AttnArgs 
   auto count = [&](uint32_t b0) {
     mine = at_load_seq(a, b0 + lane);
     n = (mine.lq * a.g + C::BM - 1) / C::BM;  // tokens * hq is below 2^31
-    sum = at_scan(n, lane);
+    sum = at_scan(n);
   };
   if (a.k_start) {
     total = 0;
@@ -145,22 +145,25 @@ __global__ __launch_bounds__(64 * C::WR, C::WPE) void attn_rows_kernel(AttnArgs 
   const uint32_t nst = kend > kbeg ? (kend - kbeg + T::KEYS - 1) / T::KEYS : 0;
   const uint32_t whole = min(kend, wmin);  // keys that every row of the wavefront sees
   const uint32_t nfull = whole > kbeg ? (whole - kbeg) / T::KEYS : 0;
-  issue(0, 0);
+#pragma unroll
+  for (int i = 0; i < C::NST - 1; ++i) issue(i, i);
   // Every wavefront takes nst turns, some of them with other rows' stages whole
   // and its own at the edge: the loop is cut in two per wavefront, the barriers
   // are the same.
-  auto turn = [&](uint32_t st, auto edge) {
+  uint32_t st = 0, bc = 0, bi = C::NST - 1;
+  auto turn = [&](auto edge) {
     // every wavefront's copies of the stage are in LDS, and every wavefront is
     // done reading the buffer that is requested next. A bare barrier:
     // __syncthreads() would also wait for the copies still in flight.
-    at_wait_vm<0>();
+    at_wait_vm<2 * C::NI *(C::NST - 2)>();
     __asm__ volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    issue(st + 1, (st + 1) & 1);
-    compute(st, st & 1, edge);
+    issue(st + C::NST - 1, bi);
+    compute(st, bc, edge);
+    bc = bc + 1 == C::NST ? 0 : bc + 1;
+    bi = bi + 1 == C::NST ? 0 : bi + 1;
   };
-  uint32_t st = 0;
-  for (; st < nfull; ++st) turn(st, std::false_type{});
-  for (; st < nst; ++st) turn(st, std::true_type{});
+  for (; st < nfull; ++st) turn(std::false_type{});
+  for (; st < nst; ++st) turn(std::true_type{});
   at_wait_vm<0>();  // nothing may still be on its way into LDS at the end
 
   const uint64_t rows_all = (uint64_t)a.tokens * a.hq;
@@ -234,7 +237,8 @@ hipError_t at_launch_rows(const AttnArgs &a, hipStream_t st) {
 template <int DT, int DP>
 constexpr bool kAtRowsFit = DP * Storage<DT>::bytes <= 512;
 template <int DT, int DP>
-using AtRows = AtRowsCfg<DT, DP, 4, 1, (DP == 96 ? 128 : DP) * Storage<DT>::bytes >= 512 ? 1 : 2>;
+using AtRows = AtRowsCfg<DT, DP, 4, 1, (DP == 96 ? 128 : DP) * Storage<DT>::bytes >= 512 ? 1 : 2,
+                         DP * Storage<DT>::bytes <= 128 ? 3 : 2>;
 
 }  // namespace
 }  // namespace aih
