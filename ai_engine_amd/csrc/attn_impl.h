@@ -76,6 +76,17 @@ __device__ __forceinline__ uint32_t at_finite_only(uint32_t r) {
   else return r & ~((b >> 15) * 0xffffu);
 }
 
+// c + the two values in p: one instruction, subnormal f16 included. The sums are
+// of the probabilities as rounded for the product, so that the roundings cancel
+// in their quotient.
+template <int DT>
+__device__ __forceinline__ float at_dot_ones(uint32_t p, float c) {
+  if constexpr (DT == DT_F16)
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, p), f16x2{(_Float16)1.0f, (_Float16)1.0f}, c, false);
+  else
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, p), bf16x2{(__bf16)1.0f, (__bf16)1.0f}, c, false);
+}
+
 // A wavefront's tile: NQ blocks of 32 query rows, KB blocks of 32 keys, heads of
 // at most DP elements.
 template <int DT_, int DP_, int NQ_, int KB_>
@@ -221,7 +232,7 @@ __device__ __forceinline__ void at_softmax(f32x16 (&sc)[T::KB][T::NQ], u32x4 (&p
       for (int r = 0; r < 16; ++r) {
         const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb][n][r], scale, off));
         sc[kb][n][r] = p;
-        sum += p;
+        if constexpr (T::F32) sum += p;
       }
       if constexpr (!T::F32) {
 #pragma unroll
@@ -230,6 +241,10 @@ __device__ __forceinline__ void at_softmax(f32x16 (&sc)[T::KB][T::NQ], u32x4 (&p
                                pack2<T::DT>(sc[kb][n][8 * h + 2], sc[kb][n][8 * h + 3]),
                                pack2<T::DT>(sc[kb][n][8 * h + 4], sc[kb][n][8 * h + 5]),
                                pack2<T::DT>(sc[kb][n][8 * h + 6], sc[kb][n][8 * h + 7])};
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sum = at_dot_ones<T::DT>(pb[kb][h][n][e], sum);
       }
     }
     l[n] += sum;

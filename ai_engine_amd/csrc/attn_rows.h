@@ -7,18 +7,18 @@
 namespace aih {
 namespace {
 
-// WR wavefronts of 32 NQ rows; stages of 32 KB keys, NST of them in LDS.
-template <int DT, int DP, int WR_, int NQ, int KB, int NST_>
+// WR wavefronts of 32 NQ rows; stages of 32 KB keys, two of them in LDS.
+template <int DT, int DP, int WR_, int NQ, int KB>
 struct AtRowsCfg {
   using T = AtTile<DT, DP, NQ, KB>;
-  static constexpr int WR = WR_, NST = NST_;
+  static constexpr int WR = WR_;
   static constexpr int BM = 32 * NQ * WR;
   static constexpr uint32_t HALF = T::KEYS * T::RB, STAGE = 2 * HALF;
-  static constexpr uint32_t LDS = NST * STAGE;
+  static constexpr uint32_t LDS = 2 * STAGE;
   static constexpr int NI = T::KEYS / T::RPI / WR;  // K instructions of a wavefront per stage, and as many of V
   // wavefronts a SIMD that the registers have to leave room for
   static constexpr int WPE = DP <= 64 ? 3 : DP <= 128 ? 2 : 1;
-  static_assert(NI >= 1 && 2 * NI * (NST - 2) < 64, "DMA instructions in flight");
+  static_assert(NI >= 1, "DMA instructions");
   static_assert(LDS <= 160 * 1024, "LDS");
 };
 
@@ -145,22 +145,19 @@ __global__ __launch_bounds__(64 * C::WR, C::WPE) void attn_rows_kernel(AttnArgs 
   const uint32_t nst = kend > kbeg ? (kend - kbeg + T::KEYS - 1) / T::KEYS : 0;
   const uint32_t whole = min(kend, wmin);  // keys that every row of the wavefront sees
   const uint32_t nfull = whole > kbeg ? (whole - kbeg) / T::KEYS : 0;
-#pragma unroll
-  for (int i = 0; i < C::NST - 1; ++i) issue(i, i);
+  issue(0, 0);
   // Every wavefront takes nst turns, some of them with other rows' stages whole
   // and its own at the edge: the loop is cut in two per wavefront, the barriers
   // are the same.
-  uint32_t st = 0, bc = 0, bi = C::NST - 1;
+  uint32_t st = 0;
   auto turn = [&](auto edge) {
     // every wavefront's copies of the stage are in LDS, and every wavefront is
     // done reading the buffer that is requested next. A bare barrier:
     // __syncthreads() would also wait for the copies still in flight.
-    at_wait_vm<2 * C::NI *(C::NST - 2)>();
+    at_wait_vm<0>();
     __asm__ volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    issue(st + C::NST - 1, bi);
-    compute(st, bc, edge);
-    bc = bc + 1 == C::NST ? 0 : bc + 1;
-    bi = bi + 1 == C::NST ? 0 : bi + 1;
+    issue(st + 1, (st + 1) & 1);
+    compute(st, st & 1, edge);
   };
   for (; st < nfull; ++st) turn(std::false_type{});
   for (; st < nst; ++st) turn(std::true_type{});
@@ -237,8 +234,7 @@ hipError_t at_launch_rows(const AttnArgs &a, hipStream_t st) {
 template <int DT, int DP>
 constexpr bool kAtRowsFit = DP * Storage<DT>::bytes <= 512;
 template <int DT, int DP>
-using AtRows = AtRowsCfg<DT, DP, 4, 1, (DP == 96 ? 128 : DP) * Storage<DT>::bytes >= 512 ? 1 : 2,
-                         DP * Storage<DT>::bytes <= 128 ? 3 : 2>;
+using AtRows = AtRowsCfg<DT, DP, 4, 1, (DP == 96 ? 128 : DP) * Storage<DT>::bytes >= 512 ? 1 : 2>;
 
 }  // namespace
 }  // namespace aih
