@@ -38,17 +38,14 @@ struct AtKeysCfg {
 
 // Work items: first the prefix's (part, row tile, key head), then sequence by
 // sequence (part, row tile, key head): neighbours stream neighbouring heads of
-// the same rows. A workgroup takes every gridDim.x-th.
-template <class C>
+// the same rows. A workgroup takes one, or (MANY) every gridDim.x-th.
+template <class C, bool MANY>
 __global__ __launch_bounds__(64 * C::WK, C::WPE) void attn_keys_kernel(AttnArgs a) {
   using T = typename C::T;
   constexpr int WK = C::WK, DB = T::DB, EB = T::EB, DP = T::DP;
   extern __shared__ __align__(16) char lds[];
 
-  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, lh = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint64_t rows_all = (uint64_t)a.tokens * a.hq;
-  const uint64_t ml0 = attn_ws_ml(a);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   char *kt = lds + wave * C::MINE, *vt = C::ONE ? kt : kt + C::HALF;
 
   // 64 sequences at a time, one a lane: items up to and including each
@@ -56,7 +53,7 @@ __global__ __launch_bounds__(64 * C::WK, C::WPE) void attn_keys_kernel(AttnArgs 
   AtSeq mine{};
   uint32_t b0 = 0, base = pre_items, n = 0, sum = 0, tiles = 0, parts = 0;
   auto count = [&]() {
-    mine = at_load_seq(a, b0 + lane);
+    mine = at_load_seq(a, b0 + (threadIdx.x & 63));
     tiles = (mine.lq * a.g + 31) / 32;
     const uint32_t x = at_shift(a, mine.len);
     parts = max(1u, (uint32_t)(((uint64_t)mine.len + (1ull << x) - 1) >> x));
@@ -66,6 +63,11 @@ __global__ __launch_bounds__(64 * C::WK, C::WPE) void attn_keys_kernel(AttnArgs 
   count();
 
   for (uint32_t item = blockIdx.x;; item += gridDim.x) {
+    int tid = threadIdx.x;
+    // the lane's offsets are worked out again for every item: kept over the
+    // loop they would not fit the registers
+    if constexpr (MANY) __asm__ volatile("" : "+v"(tid));
+    const int lane = tid & 63, l32 = lane & 31, lh = lane >> 5;
     AtSeq s;
     const char *kp, *vp;
     uint64_t ks, vs;
@@ -190,6 +192,8 @@ __global__ __launch_bounds__(64 * C::WK, C::WPE) void attn_keys_kernel(AttnArgs 
         *reinterpret_cast<f32x4 *>(jo + (wave * 32 + l32) * C::OPITCH + 32 * db + 8 * r4 + 4 * lh) =
             f32x4{o[db][0][4 * r4], o[db][0][4 * r4 + 1], o[db][0][4 * r4 + 2], o[db][0][4 * r4 + 3]} * f;
     __syncthreads();
+    const uint64_t rows_all = (uint64_t)a.tokens * a.hq;
+    const uint64_t ml0 = attn_ws_ml(a);
     // rows whose keys are all in this part need no join with others
     const bool direct = !a.ws || (nparts == 1 && a.part0 == 0);
     for (uint32_t i = tid; i < 32 * (DP / 8); i += 64 * WK) {
@@ -236,33 +240,40 @@ __global__ __launch_bounds__(64 * C::WK, C::WPE) void attn_keys_kernel(AttnArgs 
         }
       }
     }
+    if constexpr (!MANY) return;
     __syncthreads();  // the next item's copies go where the results were read
   }
 }
 
+template <class C, bool MANY>
+hipError_t at_launch_items(const AttnArgs &a, uint64_t items, uint32_t cus, hipStream_t st) {
+  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(attn_keys_kernel<C, MANY>),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
+  if (attr != hipSuccess) return attr;
+  if constexpr (MANY) {
+    // workgroups of a CU that run at once
+    static const int occ = [] {
+      int v = 0;
+      if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&v, reinterpret_cast<const void *>(attn_keys_kernel<C, MANY>),
+                                                       64 * C::WK, C::LDS) != hipSuccess || v < 1)
+        v = 1;
+      return v;
+    }();
+    if (items > (uint64_t)cus * occ) items = (uint64_t)cus * occ;
+  }
+  hipLaunchKernelGGL((attn_keys_kernel<C, MANY>), dim3((uint32_t)items), dim3(64 * C::WK), C::LDS, st, a);
+  return hipGetLastError();
+}
+
+// Uncut keys: one item a workgroup, handed out as others end. Cut ones: the
+// items are many, and of those that the host counts (the longest length for
+// all) few may exist, so the workgroups that run at once share them.
 template <class C>
 hipError_t at_launch_keys(const AttnArgs &a, uint32_t cus, hipStream_t st) {
   const uint64_t items = (uint64_t)a.hkv * a.parts * a.tiles + (uint64_t)a.hkv * a.pre_parts * a.pre_tiles;
   if (items == 0 || items > 0x7fffffffu) return hipErrorInvalidValue;
-  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(attn_keys_kernel<C>),
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
-  if (attr != hipSuccess) return attr;
-  // workgroups of a CU that run at once
-  static const int occ = [] {
-    int v = 0;
-    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&v, reinterpret_cast<const void *>(attn_keys_kernel<C>),
-                                                     64 * C::WK, C::LDS) != hipSuccess || v < 1)
-      v = 1;
-    return v;
-  }();
-  // Uncut keys: one item a workgroup, handed out as others end. Cut ones: the
-  // items are many small ones, and of those that the host counts (the longest
-  // length for all) few may exist, so the workgroups that run at once share
-  // them.
-  const uint64_t room = a.parts == 1 ? items : (uint64_t)cus * occ;
-  hipLaunchKernelGGL((attn_keys_kernel<C>), dim3((uint32_t)(items < room ? items : room)), dim3(64 * C::WK), C::LDS, st,
-                     a);
-  return hipGetLastError();
+  if (a.parts > 1 && items > cus) return at_launch_items<C, true>(a, items, cus, st);
+  return at_launch_items<C, false>(a, items, cus, st);
 }
 
 template <int DT, int DP>
