@@ -104,8 +104,9 @@ class QkNormRopeSpec:
         """x [tokens, x_stride]; wq, wk [d] or None; cosines, sines [positions, rot/2] fp32; pos, slots int32
         [tokens] or None; q [tokens, hq, d]; k, v [rows, hkv, d] (v None: the values stay in x)."""
         p = conv._ptr
-        conv._check(lib().aih_qk_norm_rope(C.byref(self._desc), p(x), p(wq), p(wk), p(cosines), p(sines), p(pos),
-                                           p(slots), p(q), p(k), p(v), conv._stream(stream)))
+        if (_lib or lib()).aih_qk_norm_rope(C.byref(self._desc), p(x), p(wq), p(wk), p(cosines), p(sines), p(pos), p(slots),
+                                            p(q), p(k), p(v), conv._stream(stream)):
+            raise AihError(conv.last_error())
         return q, k, v
 
 
@@ -155,12 +156,13 @@ class AttnSpec:
     def run(self, q, k, v, q_start, k_start, k_len, out, prefix_k=None, prefix_v=None, ws=None, stream=None):
         """q, out [tokens, hq, d]; k, v [rows, hkv, d]; q_start [nseq + 1], k_start, k_len [nseq] int32;
         prefix_k, prefix_v [prefix, hkv, d]; ws: workspace_bytes() of device memory, made here if None."""
-        n = self.workspace_bytes()
+        n = self._ws if self._ws is not None else self.workspace_bytes()
         if n:
             ws = conv._workspace(n, ws, conv._device_of(out))
             if not isinstance(ws, int) and ws.numel() * ws.element_size() < n:
                 raise AihError(f"the workspace needs {n} bytes, not {ws.numel() * ws.element_size()}")
         p = conv._ptr
-        conv._check(lib().aih_attn(C.byref(self._desc), p(q), p(k), p(v), p(q_start), p(k_start), p(k_len),
-                                   p(prefix_k), p(prefix_v), p(out), p(ws) if n else None, n, conv._stream(stream)))
+        if (_lib or lib()).aih_attn(C.byref(self._desc), p(q), p(k), p(v), p(q_start), p(k_start), p(k_len), p(prefix_k),
+                                    p(prefix_v), p(out), p(ws) if n else None, n, conv._stream(stream)):
+            raise AihError(conv.last_error())
         return out

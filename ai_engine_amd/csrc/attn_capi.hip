@@ -125,7 +125,12 @@ int check_attn(const aih_attn_desc *d, AttnArgs *a, AttnPlan *p) {
   p->own = cover(kernel, d->nseq, rows, len, d->hkv, d->dt, d->d);
   p->all_parts = p->own.parts;
   if (d->prefix) {
-    p->together = kernel == AIH_ATTN_KEYS && (rows <= 256 || !rows_fit);
+    // The prefix's keys over the wavefronts re-read them for every 32 rows, but
+    // share a launch and leave few partial results: the faster as long as rows x
+    // keys are few. 16 own keys, 32/8 heads of 128, bf16, together | apart: 128
+    // streams behind 4096 keys 34 | 38 us, behind 16384 72 | 68; 256 behind 4096 59 |
+    // 63, behind 16384 146 | 117.
+    p->together = kernel == AIH_ATTN_KEYS && (rows * d->prefix <= 1u << 22 || !rows_fit);
     p->pre = cover(p->together ? AIH_ATTN_KEYS : AIH_ATTN_ROWS, 1, rows, d->prefix, d->hkv, d->dt, d->d);
     p->all_parts += p->pre.parts;
   }
