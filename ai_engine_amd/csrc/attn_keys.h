@@ -120,6 +120,9 @@ __global__ __launch_bounds__(64 * C::WK, C::WPE) void attn_keys_kernel(AttnArgs 
       at_dma<T, C::NI, true>(vbase + (rem ? (uint64_t)key * vstr : 0), vstr, rem, du, 0, lane, vt);
     };
 
+    uint32_t key = kbeg + wave * 32;
+    issue_k(key);
+    if constexpr (!C::ONE) issue_v(key);
     u32x4 q[C::QL ? 1 : T::NC];
     char *ql = lds + C::BUF + l32 * T::RB;
     const AtQuery<T> src(a, s, hk, row0, l32);
@@ -132,9 +135,6 @@ __global__ __launch_bounds__(64 * C::WK, C::WPE) void attn_keys_kernel(AttnArgs 
 #pragma unroll
       for (int c = 0; c < T::NC; ++c) q[c] = src.unit(a, 0, 2 * c + lh);
     }
-    uint32_t key = kbeg + wave * 32;
-    issue_k(key);
-    if constexpr (!C::ONE) issue_v(key);
     auto query = [&](int, int c) -> u32x4 {
       if constexpr (C::QL) return *reinterpret_cast<const u32x4 *>(ql + (((2 * c + lh) ^ at_kswz<T>(l32)) * 16));
       else return q[c];

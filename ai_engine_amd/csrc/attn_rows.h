@@ -82,6 +82,19 @@ __global__ __launch_bounds__(64 * C::WR, C::WPE) void attn_rows_kernel(AttnArgs 
   const uint32_t kend = (uint32_t)min((uint64_t)at_limit(a, a.causal, s, min(row0 + C::BM, nrows) - 1),
                                       kbeg64 + (1ull << shift));
 
+  const uint32_t kstr = (uint32_t)a.ks * EB, vstr = (uint32_t)a.vs * EB, du = a.d / T::UE;
+  const char *kbase = (const char *)a.k + ((uint64_t)s.k0 * a.ks + (uint64_t)hk * a.d) * EB;
+  const char *vbase = (const char *)a.v + ((uint64_t)s.k0 * a.vs + (uint64_t)hk * a.d) * EB;
+  auto issue = [&](uint32_t st, uint32_t b) {
+    const uint32_t key = kbeg + st * T::KEYS;
+    const uint32_t rem = key < kend ? min(kend - key, (uint32_t)T::KEYS) : 0;
+    char *dst = lds + b * C::STAGE;
+    at_dma<T, C::NI, false>(kbase + (rem ? (uint64_t)key * kstr : 0), kstr, rem, du, wave * C::NI, lane, dst);
+    at_dma<T, C::NI, true>(vbase + (rem ? (uint64_t)key * vstr : 0), vstr, rem, du, wave * C::NI, lane, dst + C::HALF);
+  };
+
+  issue(0, 0);  // on its way while the rest is set up
+
   const uint32_t wrow = row0 + wave * 32 * NQ;
   uint32_t lim[NQ];
   u32x4 q[NQ][T::NC];
@@ -95,17 +108,6 @@ __global__ __launch_bounds__(64 * C::WR, C::WPE) void attn_rows_kernel(AttnArgs 
   // the first row of a wavefront sees the fewest keys, its last one the most
   const uint32_t wmin = wrow < nrows ? at_limit(a, a.causal, s, wrow) : 0;
   const uint32_t wmax = wrow < nrows ? at_limit(a, a.causal, s, min(wrow + 32 * NQ, nrows) - 1) : 0;
-
-  const uint32_t kstr = (uint32_t)a.ks * EB, vstr = (uint32_t)a.vs * EB, du = a.d / T::UE;
-  const char *kbase = (const char *)a.k + ((uint64_t)s.k0 * a.ks + (uint64_t)hk * a.d) * EB;
-  const char *vbase = (const char *)a.v + ((uint64_t)s.k0 * a.vs + (uint64_t)hk * a.d) * EB;
-  auto issue = [&](uint32_t st, uint32_t b) {
-    const uint32_t key = kbeg + st * T::KEYS;
-    const uint32_t rem = key < kend ? min(kend - key, (uint32_t)T::KEYS) : 0;
-    char *dst = lds + b * C::STAGE;
-    at_dma<T, C::NI, false>(kbase + (rem ? (uint64_t)key * kstr : 0), kstr, rem, du, wave * C::NI, lane, dst);
-    at_dma<T, C::NI, true>(vbase + (rem ? (uint64_t)key * vstr : 0), vstr, rem, du, wave * C::NI, lane, dst + C::HALF);
-  };
 
   f32x16 o[DB][NQ];
   float m[NQ], l[NQ];
@@ -145,7 +147,6 @@ __global__ __launch_bounds__(64 * C::WR, C::WPE) void attn_rows_kernel(AttnArgs 
   const uint32_t nst = kend > kbeg ? (kend - kbeg + T::KEYS - 1) / T::KEYS : 0;
   const uint32_t whole = min(kend, wmin);  // keys that every row of the wavefront sees
   const uint32_t nfull = whole > kbeg ? (whole - kbeg) / T::KEYS : 0;
-  issue(0, 0);
   // Every wavefront takes nst turns, some of them with other rows' stages whole
   // and its own at the edge: the loop is cut in two per wavefront, the barriers
   // are the same.
