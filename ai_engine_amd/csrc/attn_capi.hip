@@ -57,8 +57,10 @@ struct Cover {
 uint32_t div_up(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 
 // `nseq` sequences of `rows` (query, head of the group) rows altogether, each
-// against about `len` keys.
-Cover cover(int32_t kernel, uint32_t nseq, uint64_t rows, uint32_t len, uint32_t hkv, int32_t dt, uint32_t d) {
+// against about `len` keys. Keys are cut until the work items fill the CUs
+// twice; those of few rows at 1024 anyway, since lengths may differ a lot.
+Cover cover(int32_t kernel, uint32_t nseq, uint64_t rows, uint32_t len, uint32_t hkv, int32_t dt, uint32_t d,
+            bool split) {
   const uint32_t cus = device_cus();
   Cover c{};
   c.kernel = kernel;
@@ -71,7 +73,7 @@ Cover cover(int32_t kernel, uint32_t nseq, uint64_t rows, uint32_t len, uint32_t
     while (c.shift > 8 && base * parts(c.shift) < 2 * cus) --c.shift;
   } else {
     c.shift = 31;
-    while (c.shift > 9 && base * parts(c.shift) < 2 * cus) --c.shift;
+    while (split && c.shift > 9 && base * parts(c.shift) < 2 * cus) --c.shift;
   }
   c.parts = parts(c.shift);
   if (c.parts == 1) c.shift = 31;
@@ -122,7 +124,7 @@ int check_attn(const aih_attn_desc *d, AttnArgs *a, AttnPlan *p) {
   const uint64_t cus = device_cus();
   const bool chain = d->dt == AIH_F32 ? tiles < 4 * cus : 2 * tiles < 3 * cus && len >= 256;
   const int32_t kernel = rows <= 32ull * d->nseq || !rows_fit || chain ? AIH_ATTN_KEYS : AIH_ATTN_ROWS;
-  p->own = cover(kernel, d->nseq, rows, len, d->hkv, d->dt, d->d);
+  p->own = cover(kernel, d->nseq, rows, len, d->hkv, d->dt, d->d, kernel == AIH_ATTN_KEYS);
   p->all_parts = p->own.parts;
   if (d->prefix) {
     // The prefix's keys over the wavefronts re-read them for every 32 rows, but
@@ -131,7 +133,7 @@ int check_attn(const aih_attn_desc *d, AttnArgs *a, AttnPlan *p) {
     // streams behind 4096 keys 34 | 38 us, behind 16384 72 | 68; 256 behind 4096 59 |
     // 63, behind 16384 146 | 117.
     p->together = kernel == AIH_ATTN_KEYS && (rows * d->prefix <= 1u << 22 || !rows_fit);
-    p->pre = cover(p->together ? AIH_ATTN_KEYS : AIH_ATTN_ROWS, 1, rows, d->prefix, d->hkv, d->dt, d->d);
+    p->pre = cover(p->together ? AIH_ATTN_KEYS : AIH_ATTN_ROWS, 1, rows, d->prefix, d->hkv, d->dt, d->d, true);
     p->all_parts += p->pre.parts;
   }
   if ((uint64_t)p->own.tiles * d->hkv * p->own.parts + (uint64_t)p->pre.tiles * d->hkv * p->pre.parts > 0x7fffffffu)
@@ -218,7 +220,6 @@ extern "C" int aih_attn(const aih_attn_desc *d, const void *q, const void *k, co
     a.q = q, a.k = k, a.v = v, a.o = o, a.ws = p.ws_floats ? static_cast<float *>(ws) : nullptr;
     a.q_start = q_start, a.k_start = k_start, a.k_len = k_len;
     a.all_parts = p.all_parts;
-    a.nxcd = device_xcds();
     a.by_g = make_fastdiv(a.g), a.by_hkv = make_fastdiv(a.hkv);
     a.by_pre_tiles = make_fastdiv(std::max(1u, p.pre.tiles));
     a.pk = prefix_k, a.pv = prefix_v, a.prefix = d->prefix;
