@@ -116,13 +116,14 @@ int check_attn(const aih_attn_desc *d, AttnArgs *a, AttnPlan *p) {
   const bool rows_fit = d->d * dt_bytes(d->dt) <= 512;  // else the registers do not hold a wavefront's queries
   // Prompts of few tiles: a wavefront's 32 rows against all keys are a chain
   // that sets the time while others have nothing to do, so the keys go over
-  // the wavefronts. Measured, rows | keys over the wavefronts: fp32, 4096 tokens,
-  // 16/4 heads of 96 (512 tiles) 645 | 460 us, 32/8 heads (1024) 862 | 928; f16,
-  // 720 tokens, 32/8 heads of 64 (184 tiles) 25 | 17 us, four of them (752) 24 | 45;
-  // 16 of 100 tokens, 8/2 heads of 128 (132) 9.9 | 11.5: too short to share.
+  // the wavefronts. Measured, rows | keys over the wavefronts: fp32 causal, 4096
+  // tokens, 16/4 heads of 96 (512 tiles) 564 | 436 us, 4 x 2048 tokens (1040) 573 |
+  // 487, 16 x 720 (1504) 293 | 321; 16 bit, 2880 tokens, 8/2 heads of 64 (180) 41 |
+  // 25, 16/4 heads (360) 44.6 | 43.6, of 128 63 | 70; 40 x 100 tokens, 8/2 heads of
+  // 128 (330) 14 | 19: too short to share.
   const uint64_t tiles = (uint64_t)d->hkv * (div_up(rows, attn_bm(AIH_ATTN_ROWS, d->dt, d->d)) + d->nseq / 2);
   const uint64_t cus = device_cus();
-  const bool chain = d->dt == AIH_F32 ? tiles < 4 * cus : 2 * tiles < 3 * cus && len >= 256;
+  const bool chain = d->dt == AIH_F32 ? tiles < 5 * cus : tiles < cus && len >= 256;
   const int32_t kernel = rows <= 32ull * d->nseq || !rows_fit || chain ? AIH_ATTN_KEYS : AIH_ATTN_ROWS;
   p->own = cover(kernel, d->nseq, rows, len, d->hkv, d->dt, d->d, kernel == AIH_ATTN_KEYS);
   p->all_parts = p->own.parts;
