@@ -2,7 +2,7 @@
 
 Every translation unit is compiled by hipcc for gfx950 only, in parallel,
 into ai_engine_amd/_build/, then linked into a shared library that exports the
-C ABI of include/aih_conv.h.  Run `python -m ai_engine_amd.build`.
+C ABI of include/.  Run `python -m ai_engine_amd.build`.
 """
 from __future__ import annotations
 
