@@ -172,6 +172,7 @@ EXPORTS = (
     "aih_conv_noalloc", "aih_conv_stem_f32in", "aih_conv_dwpw_plan", "aih_conv_dwpw",
     "aih_ir_block_stem_plan", "aih_ir_block_stem",
     "aih_ir_block_head_plan", "aih_ir_block_head",
+    "aih_qk_norm_rope", "aih_attn_plan", "aih_attn",  # bound in attn.py
 )
 
 _lib = None
