@@ -56,11 +56,20 @@ struct Cover {
 
 uint32_t div_up(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 
+enum class Use { OWN, PREFIX };
+
 // `nseq` sequences of `rows` (query, head of the group) rows altogether, each
-// against about `len` keys. Keys are cut until the work items fill the CUs
-// twice; those of few rows at 1024 anyway, since lengths may differ a lot.
-Cover cover(int32_t kernel, uint32_t nseq, uint64_t rows, uint32_t len, uint32_t hkv, int32_t dt, uint32_t d,
-            bool split) {
+// against about `len` keys. What cutting the keys gains in spread it pays for
+// with partial results and a launch that joins them, which the prefix needs
+// anyway. Measured with AIH_ATTN_KEYS (16 bit; heads, keys: whole | cut):
+//   1 stream, 32/8 heads of 128: 512 8.0 | 9.3 us, 1024 11.7 | 9.6, 4096 24 | 10.5
+//   16 streams: 1024 14.5 | 18.9 us, 2048 in 2 parts 34.6, in 8 36.9
+//   a prompt of 1500, 4/4 heads of 64 (188 items) 11.8 | 16.9 us
+// fp32, 1 stream, 8/2 heads of 64: 384 10.9 | 11.5 us, 512 13.1 | 11.6; a prompt of
+// 1024, 4/4 heads (128 items) 22.7 | 18.8. Few rows are cut at 1024 anyway, since
+// the sequences' lengths may differ a lot. 64 streams behind a prefix of 4096,
+// 32/8 heads of 128: 8 parts 29.2 us, 4 parts 25.1.
+Cover cover(int32_t kernel, uint32_t nseq, uint64_t rows, uint32_t len, uint32_t hkv, int32_t dt, uint32_t d, Use use) {
   const uint32_t cus = device_cus();
   Cover c{};
   c.kernel = kernel;
@@ -68,12 +77,14 @@ Cover cover(int32_t kernel, uint32_t nseq, uint64_t rows, uint32_t len, uint32_t
   c.tiles = nseq == 1 ? div_up(rows, c.bm) : (uint32_t)(rows / c.bm) + nseq;
   const uint64_t base = (uint64_t)c.tiles * hkv;
   auto parts = [&](uint32_t x) { return std::max(1u, div_up(len, 1ull << x)); };
-  if (c.kernel == AIH_ATTN_KEYS && rows <= 32ull * nseq) {
-    c.shift = 10;
-    while (c.shift > 8 && base * parts(c.shift) < 2 * cus) --c.shift;
-  } else {
-    c.shift = 31;
-    while (split && c.shift > 9 && base * parts(c.shift) < 2 * cus) --c.shift;
+  const bool few = rows <= 32ull * nseq;
+  const uint32_t whole = use == Use::PREFIX ? 0 : kernel == AIH_ATTN_ROWS ? len : dt == AIH_F32 ? 384 : 768;
+  const uint32_t items = use == Use::PREFIX || dt == AIH_F32 ? cus : cus / 2;
+  const uint32_t least = few && use == Use::OWN ? 8 : 9;
+  c.shift = 31;
+  if (len > whole) {
+    if (few && use == Use::OWN) c.shift = 10;
+    while (c.shift > least && base * parts(c.shift) < items) --c.shift;
   }
   c.parts = parts(c.shift);
   if (c.parts == 1) c.shift = 31;
@@ -125,7 +136,7 @@ int check_attn(const aih_attn_desc *d, AttnArgs *a, AttnPlan *p) {
   const uint64_t cus = device_cus();
   const bool chain = d->dt == AIH_F32 ? tiles < 5 * cus : tiles < cus && len >= 256;
   const int32_t kernel = rows <= 32ull * d->nseq || !rows_fit || chain ? AIH_ATTN_KEYS : AIH_ATTN_ROWS;
-  p->own = cover(kernel, d->nseq, rows, len, d->hkv, d->dt, d->d, kernel == AIH_ATTN_KEYS);
+  p->own = cover(kernel, d->nseq, rows, len, d->hkv, d->dt, d->d, Use::OWN);
   p->all_parts = p->own.parts;
   if (d->prefix) {
     // The prefix's keys over the wavefronts re-read them for every 32 rows, but
@@ -134,7 +145,7 @@ int check_attn(const aih_attn_desc *d, AttnArgs *a, AttnPlan *p) {
     // streams behind 4096 keys 34 | 38 us, behind 16384 72 | 68; 256 behind 4096 59 |
     // 63, behind 16384 146 | 117.
     p->together = kernel == AIH_ATTN_KEYS && (rows * d->prefix <= 1u << 22 || !rows_fit);
-    p->pre = cover(p->together ? AIH_ATTN_KEYS : AIH_ATTN_ROWS, 1, rows, d->prefix, d->hkv, d->dt, d->d, true);
+    p->pre = cover(p->together ? AIH_ATTN_KEYS : AIH_ATTN_ROWS, 1, rows, d->prefix, d->hkv, d->dt, d->d, Use::PREFIX);
     p->all_parts += p->pre.parts;
   }
   if ((uint64_t)p->own.tiles * d->hkv * p->own.parts + (uint64_t)p->pre.tiles * d->hkv * p->pre.parts > 0x7fffffffu)

@@ -239,8 +239,11 @@ hipError_t at_launch_rows(const AttnArgs &a, hipStream_t st) {
 // The heads of more than 128 fp32 elements leave no registers for this kernel.
 template <int DT, int DP>
 constexpr bool kAtRowsFit = DP * Storage<DT>::bytes <= 512;
+// Stages of 64 keys, or of 32 where two of 64 leave no room: fp32 heads above 64
+// elements (at 256 16-bit elements 64 keys beat 32 by 2 to 7 %, one workgroup a
+// CU either way).
 template <int DT, int DP>
-using AtRows = AtRowsCfg<DT, DP, 4, 1, (DP == 96 ? 128 : DP) * Storage<DT>::bytes >= 512 ? 1 : 2>;
+using AtRows = AtRowsCfg<DT, DP, 4, 1, (DT == DT_F32 && DP > 64) ? 1 : 2>;
 
 }  // namespace
 }  // namespace aih

@@ -194,7 +194,7 @@ def test_large_scores(dt):
 # ---------------------------------------------------------------- keys cut into parts
 
 @pytest.mark.parametrize("dt", ALL)
-@pytest.mark.parametrize("lens", [[255, 256, 257], [1023, 0, 2049], [3000, 1, 513]])
+@pytest.mark.parametrize("lens", [[1300, 256, 257], [1023, 0, 2049], [3000, 1, 513]])
 def test_cut_keys(dt, lens):
     c = Case(dt, 4, 2, 64, [1] * 3, lens, seed=6)
     p = c.spec(max_len=3000).plan()
