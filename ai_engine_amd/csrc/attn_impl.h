@@ -24,6 +24,7 @@ namespace {
 typedef __attribute__((address_space(3))) void at_lds_void;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4 at_lds_s16x4;
 
 constexpr uint32_t kAtOob = 0x80000000u;  // a byte offset past every buffer
@@ -302,20 +303,33 @@ __device__ __forceinline__ void at_pv(const char *vt, const f32x16 (&sc)[T::KB][
   }
 }
 
-// Keys that some rows of a tile see and others do not: 0 * NaN or 0 * inf of an
-// unseen value must not reach a row. If the tile holds such values they are
-// added to the rows that see them (keys below to[n]) one by one, and the
-// product runs without them. True: it holds some.
-template <class T>
-__device__ __forceinline__ bool at_spread_nonfinite(const char *vt, const uint32_t (&to)[T::NQ],
-                                                    f32x16 (&o)[T::DB][T::NQ], int lane) {
-  uint32_t bad = 0;
-  for (int i = lane; i < T::KEYS * T::PU; i += 64) {
-    const u32x4 v = *reinterpret_cast<const u32x4 *>(vt + i * 16);
+// The larger magnitude, per value, of a running maximum and of four words of V.
+template <int DT>
+__device__ __forceinline__ uint32_t at_max_abs(uint32_t m, u32x4 v) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) bad |= at_nonfinite<T::DT>(v[e]);
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (DT == DT_F32) {
+      m = max(m, v[e] & 0x7fffffffu);
+    } else {
+      const u16x2 x = __builtin_bit_cast(u16x2, v[e] & 0x7fff7fffu), y = __builtin_bit_cast(u16x2, m);
+      m = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(x, y));
+    }
   }
-  if (!__any(bad != 0)) return false;
+  return m;
+}
+
+// Keys that some rows of a tile see and others do not: 0 * NaN or 0 * inf of an
+// unseen value must not reach a row. If keys `from` .. `end` - 1 of the tile,
+// which hold all of those, have such values, the tile's are added to the rows
+// that see them (keys below to[n]) one by one, and the product runs without
+// them. True: it has some.
+template <class T>
+__device__ __forceinline__ bool at_spread_nonfinite(const char *vt, uint32_t from, uint32_t end,
+                                                    const uint32_t (&to)[T::NQ], f32x16 (&o)[T::DB][T::NQ], int lane) {
+  uint32_t big = 0;
+  for (uint32_t i = from * T::PU + lane; i < end * T::PU; i += 64)
+    big = at_max_abs<T::DT>(big, *reinterpret_cast<const u32x4 *>(vt + i * 16));
+  if (!__any(at_nonfinite<T::DT>(big) != 0)) return false;
   const uint32_t lh = lane >> 5;
   for (uint32_t j = 0; j < T::KEYS; ++j) {
 #pragma unroll

@@ -161,7 +161,8 @@ __global__ __launch_bounds__(64 * C::WK, C::WPE) void attn_keys_kernel(AttnArgs 
       at_softmax<T>(sc, pb, m, l, o, a.scale_log2);
       at_wait_vm<C::ONE ? 0 : C::NI>();  // V is there, the next K on its way
       __asm__ volatile("" ::: "memory");
-      if (smin < min(kend, key + 32) && at_spread_nonfinite<T>(vt, to, o, lane))
+      const uint32_t end = min(kend, key + 32);
+      if (smin < end && at_spread_nonfinite<T>(vt, max(smin, key) - key, end - key, to, o, lane))
         at_pv<T, true>(vt, sc, pb, o, lane);
       else
         at_pv<T, false>(vt, sc, pb, o, lane);

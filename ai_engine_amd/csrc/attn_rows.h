@@ -139,7 +139,8 @@ __global__ __launch_bounds__(64 * C::WR, C::WPE) void attn_rows_kernel(AttnArgs 
       for (int i = 0; i < NQ; ++i) to[i] = max(min(kend, lim[i]), key) - key;
       at_mask<T>(sc, to, lane);
       at_softmax<T>(sc, pb, m, l, o, a.scale_log2);
-      if (wmin < min(kend, key + T::KEYS) && at_spread_nonfinite<T>(vt, to, o, lane)) {
+      const uint32_t end = min(kend, key + T::KEYS);
+      if (wmin < end && at_spread_nonfinite<T>(vt, max(wmin, key) - key, end - key, to, o, lane)) {
         at_pv<T, true>(vt, sc, pb, o, lane);
         return;
       }
