@@ -25,6 +25,7 @@ __global__ __launch_bounds__(64 * (NW == 1 ? kWaves : NW)) void attn_join_kernel
   const uint64_t row = NW == 1 ? (uint64_t)blockIdx.x * kWaves + w : blockIdx.x;
   if (row >= rows_all) return;
   const f32x2 *ml = reinterpret_cast<const f32x2 *>(a.ws + attn_ws_ml(a)) + row;
+  const int q0 = a.q_start[0], q1 = a.q_start[a.nseq];
 
   // (maximum, sum) of the part that this lane's next vector belongs to
   const uint32_t subs = NW * (64u >> ldim), sub = wave * (64u >> ldim) + (lane >> ldim);
@@ -52,6 +53,8 @@ __global__ __launch_bounds__(64 * (NW == 1 ? kWaves : NW)) void attn_join_kernel
     sum = sum * __builtin_amdgcn_exp2f(mx - mn) + t.y * __builtin_amdgcn_exp2f(t.x - mn);
     mx = mn;
   }
+  const uint64_t t = row / a.hq, h = row - t * a.hq;
+  done |= (int64_t)t < q0 || (int64_t)t >= q1;  // of no sequence: no part holds anything
   if (__any(done)) return;  // the whole row's wavefronts find the same
   float all = mx;
 #pragma unroll
@@ -84,7 +87,6 @@ __global__ __launch_bounds__(64 * (NW == 1 ? kWaves : NW)) void attn_join_kernel
   }
   if (lane < (1u << ldim) && dim < a.d) {
     x *= sum == 0.0f ? 0.0f : 1.0f / sum;
-    const uint64_t t = row / a.hq, h = row - t * a.hq;
     const uint64_t e = t * a.os + h * a.d + dim;
     if constexpr (DT == DT_F32) *reinterpret_cast<f32x4 *>((float *)a.o + e) = x;
     else *reinterpret_cast<u32x2 *>((uint16_t *)a.o + e) = pack4<DT>(x);

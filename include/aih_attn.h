@@ -108,9 +108,9 @@ typedef struct {
 
 int aih_attn_plan(const aih_attn_desc *d, aih_attn_plan_info *out);
 
-/* q_start [nseq + 1], k_start and k_len [nseq]: int32 device arrays; starts
- * and lengths that reach past the tensors are cut there, and a row of o that
- * no sequence covers is not written. prefix_k / prefix_v are read when
+/* q_start [nseq + 1] (not descending), k_start and k_len [nseq]: int32 device
+ * arrays; starts and lengths that reach past the tensors are cut there, and a
+ * row of o that no sequence covers is not written. prefix_k / prefix_v are read when
  * d->prefix > 0. ws: plan.ws_bytes of device memory, aligned to 16 bytes (may
  * be NULL when 0). */
 int aih_attn(const aih_attn_desc *d, const void *q, const void *k, const void *v, const int32_t *q_start,

@@ -347,6 +347,23 @@ def test_rows_of_no_sequence_are_not_written():
     assert (out[:10] == 5.0).all() and (out[80:] == 5.0).all()
 
 
+@pytest.mark.parametrize("prefix", [0, 700])
+@pytest.mark.parametrize("lq", [1, 40])
+def test_rows_of_no_sequence_are_not_written_by_a_join(prefix, lq):
+    lens = [3000, 1, 1500]
+    c = Case(DType.F16, 4, 2, 64, [lq] * 3, lens, prefix=prefix, seed=19)
+    out = torch.full((c.tokens + 30, 4, 64), 5.0, dtype=torch.float16, device=DEV)
+    q = torch.ones(c.tokens + 30, 4, 64, dtype=torch.float16)
+    q[10:-20] = c.q
+    spec = c.spec(tokens=c.tokens + 30)
+    assert spec.workspace_bytes() > 0
+    ws = torch.ones(spec.workspace_bytes() // 4, device=DEV)
+    spec.run(q.to(DEV), c.k.to(DEV), c.v.to(DEV), i32([10 + s for s in c.q_starts]), i32(c.k_starts), i32(c.k_lens),
+             out, prefix_k=c.pk.to(DEV) if prefix else None, prefix_v=c.pv.to(DEV) if prefix else None, ws=ws)
+    c.check(got=out[10:-20].cpu())
+    assert (out[:10] == 5.0).all() and (out[-20:] == 5.0).all()
+
+
 @pytest.mark.parametrize("lq", [1, 40])
 def test_a_cache_beyond_32_bit_offsets(lq):
     # 2^31 elements and 4 GiB lie before the sequence's rows
