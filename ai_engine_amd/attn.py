@@ -74,6 +74,17 @@ def _u32(name, v, lo=0):
     return v
 
 
+def _workspace_on(nbytes, device, stream):
+    """Device memory of the stream it is used on: torch gives a freed block to that stream's next allocation only."""
+    device = device or "cuda"  # a raw address has none
+    if stream is None:
+        return conv._workspace(nbytes, None, device)
+    import torch
+
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device) if isinstance(stream, int) else stream):
+        return conv._workspace(nbytes, None, device)
+
+
 @dataclass(frozen=True)
 class QkNormRopeSpec:
     """Head norms and rotation; fields of aih_qk_norm_rope_desc (strides in elements, 0 = dense)."""
@@ -158,7 +169,8 @@ class AttnSpec:
         prefix_k, prefix_v [prefix, hkv, d]; ws: workspace_bytes() of device memory, made here if None."""
         n = self._ws if self._ws is not None else self.workspace_bytes()
         if n:
-            ws = conv._workspace(n, ws, conv._device_of(out))
+            if ws is None:
+                ws = _workspace_on(n, conv._device_of(out), stream)
             if not isinstance(ws, int) and ws.numel() * ws.element_size() < n:
                 raise AihError(f"the workspace needs {n} bytes, not {ws.numel() * ws.element_size()}")
         p = conv._ptr

@@ -414,6 +414,37 @@ def test_on_another_stream_and_with_its_own_workspace():
     assert torch.equal(out.cpu(), want)
 
 
+def test_raw_addresses():
+    c = Case(DType.F16, 8, 2, 64, [1] * 4, [5000, 3000, 10, 0], seed=23)
+    spec = c.spec()
+    args = [t.to(DEV) for t in (c.q, c.k, c.v)] + [i32(c.q_starts), i32(c.k_starts), i32(c.k_lens)]
+    out = torch.full((4, 8, 64), float("nan"), dtype=torch.float16, device=DEV)
+    assert spec.workspace_bytes() > 0
+    spec.run(*[t.data_ptr() for t in args], out.data_ptr())
+    c.check(got=out.cpu())
+
+
+@pytest.mark.parametrize("raw", [False, True])
+def test_a_workspace_made_by_the_call_belongs_to_its_stream(raw):
+    c = Case(DType.F16, 8, 2, 64, [1] * 4, [5000, 3000, 10, 0], seed=23)
+    want = c.run()
+    spec = c.spec()
+    args = [t.to(DEV) for t in (c.q, c.k, c.v)] + [i32(c.q_starts), i32(c.k_starts), i32(c.k_lens)]
+    out = torch.full((4, 8, 64), float("nan"), dtype=torch.float16, device=DEV)
+    n = spec.workspace_bytes() // 4
+    a = torch.randn(4096, 4096, device=DEV)
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(st):
+        for _ in range(8):  # keeps the stream busy while the host goes on
+            a @ a
+    spec.run(*args, out, stream=st.cuda_stream if raw else st)
+    others = [torch.full((n,), 7.0, device=DEV) for _ in range(3)]  # on the current stream, at once
+    torch.cuda.synchronize()
+    assert torch.equal(out.cpu(), want)
+    assert all(bool((o == 7.0).all()) for o in others)
+
+
 def test_graph_replay():
     c = Case(DType.F16, 8, 2, 64, [1] * 4, [5000, 3000, 10, 0], prefix=200, seed=24)
     spec = c.spec()
