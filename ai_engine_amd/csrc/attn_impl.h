@@ -31,13 +31,15 @@ constexpr uint32_t kAtOob = 0x80000000u;  // a byte offset past every buffer
 constexpr float kAtLowest = -3.402823466e38f;
 // A row's maximum is left stale until a score exceeds it by 2^8, so that the
 // accumulators are rescaled a few times per row instead of once per stage; p
-// stays below 2^8, exact enough in every type. For 16-bit heads of at most 64
-// elements, where the vector instructions and not the products set the time,
-// the maximum is not even looked for until a tile's probabilities, whose sum
-// is at hand before they are used, add up to 2^15 (AtTile::LAZY; 4096 tokens,
-// 16/4 heads causal: of 32 elements 50.0 -> 43.4 us, of 64 62.0 -> 58.9, of 96
-// and 256 nothing gained, of 128 2 % lost: the exponentials then wait for the check
-// instead of running beside the next product). A row goes by its own values
+// stays below 2^8, exact enough in every type. LAZY tiles do not even look for
+// the maximum before a block's probabilities, whose sum is at hand before they
+// are used, add up to 2^15: 16-bit heads of at most 64 elements, whose vector
+// instructions set the time (4096 tokens, 16/4 heads causal: of 32 elements
+// 50.0 -> 43.4 us, of 64 62.0 -> 58.9), and of more than 128, whose steps are
+// written out (at_step) and have nothing to wait for. At 96 and 128 elements the
+// exponentials then wait for the check instead of running beside the next
+// product (2 to 3 % lost), fp32's few long ones lose it (3 to 5 % of a short
+// call: a row's first block is always taken twice). A row goes by its own values
 // alone: what others in the wavefront hold does not change its rounding.
 constexpr float kAtSlack = 8.0f;
 constexpr float kAtMost = 32768.0f;
@@ -96,20 +98,21 @@ __device__ __forceinline__ float at_dot_ones(uint32_t p, float c) {
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, p), bf16x2{(__bf16)1.0f, (__bf16)1.0f}, c, false);
 }
 
-// A wavefront's tile: NQ blocks of 32 query rows, KB blocks of 32 keys, heads of
-// at most DP elements.
-template <int DT_, int DP_, int NQ_, int KB_>
+// A wavefront's tile: 32 query rows, 32 keys, heads of at most DP elements.
+template <int DT_, int DP_>
 struct AtTile {
-  static constexpr int DT = DT_, DP = DP_, NQ = NQ_, KB = KB_;
+  static constexpr int DT = DT_, DP = DP_;
   static constexpr bool F32 = DT == DT_F32;
-  static constexpr bool LAZY = !F32 && DP <= 64;
+  static constexpr bool LAZY = !F32 && (DP <= 64 || DP > 128);  // see kAtMost
   static constexpr int EB = Storage<DT>::bytes, UE = 16 / EB;
   static constexpr int U = DP / UE;                   // 16-byte units of a head
   static constexpr int PU = DP == 96 ? 128 / UE : U;  // units of an LDS row: a power of two
   static constexpr int RB = PU * 16;
   static constexpr int NC = U / 2, DB = DP / 32;
   static constexpr int RPI = 64 / PU;                 // rows of a DMA instruction (1 KB)
-  static constexpr int KEYS = 32 * KB;
+  // probabilities of 32 keys: as they are, or packed, 16 keys an operand
+  struct Packed { u32x4 h[2]; };
+  using Probs = std::conditional_t<F32, f32x16, Packed>;
 };
 
 // LDS layout of a tile of rows: unit u of row r at slot u ^ swz(r) of its PU
@@ -164,167 +167,193 @@ __device__ __forceinline__ void at_dma(const char *base, uint32_t stride, uint32
   }
 }
 
-// S^T = K Q^T of a tile; q(n, c): units 2c + h (lane half h) of this lane's row of
-// block n.
-template <class T, class Q>
-__device__ __forceinline__ void at_qk(const char *kt, Q q, f32x16 (&sc)[T::KB][T::NQ], int lane) {
-  const uint32_t l32 = lane & 31, lh = lane >> 5, sw = at_kswz<T>(l32);
-#pragma unroll
-  for (int kb = 0; kb < T::KB; ++kb) {
-#pragma unroll
-    for (int n = 0; n < T::NQ; ++n) sc[kb][n] = f32x16{};
-#pragma unroll
-    for (int c = 0; c < T::NC; ++c) {
-      const u32x4 k = *reinterpret_cast<const u32x4 *>(kt + (32 * kb + l32) * T::RB + (((2 * c + lh) ^ sw) * 16));
-#pragma unroll
-      for (int n = 0; n < T::NQ; ++n) {
-        const u32x4 qn = q(n, c);
-        if constexpr (T::F32) {
-          const f32x4 k4 = __builtin_bit_cast(f32x4, k), q4 = __builtin_bit_cast(f32x4, qn);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[kb][n] = __builtin_amdgcn_mfma_f32_32x32x2f32(k4[e], q4[e], sc[kb][n], 0, 0, 0);
-        } else if constexpr (T::DT == DT_F16) {
-          sc[kb][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, k),
-                                                             __builtin_bit_cast(f16x8, qn), sc[kb][n], 0, 0, 0);
-        } else {
-          sc[kb][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, k),
-                                                              __builtin_bit_cast(bf16x8, qn), sc[kb][n], 0, 0, 0);
-        }
-      }
-    }
-  }
+// c + A B of 16-bit operands
+template <class T>
+__device__ __forceinline__ f32x16 at_mfma(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (T::DT == DT_F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// Key of result register r in block kb, relative to the tile.
-__device__ __forceinline__ uint32_t at_key(int kb, int r, uint32_t lh) { return 32 * kb + 8 * (r / 4) + 4 * lh + r % 4; }
+// S^T = K Q^T of N tiles; q(c): units 2c + h (lane half h) of this lane's row.
+template <class T, int N, class Q>
+__device__ __forceinline__ void at_qk(const char *kt, Q q, f32x16 (&sc)[N], int lane) {
+  const uint32_t l32 = lane & 31, lh = lane >> 5, sw = at_kswz<T>(l32);
+#pragma unroll
+  for (int i = 0; i < N; ++i) sc[i] = f32x16{};
+#pragma unroll
+  for (int c = 0; c < T::NC; ++c)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const u32x4 k = *reinterpret_cast<const u32x4 *>(kt + (32 * i + l32) * T::RB + (((2 * c + lh) ^ sw) * 16)), qc = q(c);
+      if constexpr (T::F32) {
+        const f32x4 k4 = __builtin_bit_cast(f32x4, k), q4 = __builtin_bit_cast(f32x4, qc);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(k4[e], q4[e], sc[i], 0, 0, 0);
+      } else {
+        sc[i] = at_mfma<T>(k, qc, sc[i]);
+      }
+    }
+}
 
-// Keys from to[n] on (relative to the tile) do not count.
-template <class T>
-__device__ __forceinline__ void at_mask(f32x16 (&sc)[T::KB][T::NQ], const uint32_t (&to)[T::NQ], int lane) {
-  const uint32_t lh = lane >> 5;
+// Keys from `to` on (relative to the tile) do not count: result register r is key
+// 8 (r / 4) + r % 4 + 4 h.
+__device__ __forceinline__ void at_mask(f32x16 &sc, uint32_t to, int lane) {
+  const int mine = (int)min(to, 32u) - 4 * (lane >> 5);
 #pragma unroll
-  for (int n = 0; n < T::NQ; ++n)
-#pragma unroll
-    for (int kb = 0; kb < T::KB; ++kb)
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (at_key(kb, r, lh) >= to[n]) sc[kb][n][r] = -__builtin_huge_valf();
+  for (int r = 0; r < 16; ++r)
+    if (8 * (r / 4) + r % 4 >= mine) sc[r] = -__builtin_huge_valf();
 }
 
 // Scores -> probabilities 2^(scale s - m + bias) with the running maximum m (in
-// the exponent's units) and this lane's share of the sum l. 16-bit types get
-// them packed for the product, 16 keys an operand.
+// the exponent's units); returns `sum` plus this lane's. Words w0 .. w1 - 1, two
+// keys each.
 template <class T>
-__device__ __forceinline__ void at_softmax(f32x16 (&sc)[T::KB][T::NQ], u32x4 (&pb)[T::KB][2][T::NQ], float (&m)[T::NQ],
-                                           float (&l)[T::NQ], f32x16 (&o)[T::DB][T::NQ], float scale) {
+__device__ __forceinline__ float at_probs(const f32x16 &sc, typename T::Probs &p, float m, float scale, int w0 = 0,
+                                          int w1 = 8, float sum = 0.0f) {
+  const float off = kAtBias<T::DT> - m;
 #pragma unroll
-  for (int n = 0; n < T::NQ; ++n) {
-    // the row's maximum over this tile, in the exponent's units
-    auto top = [&]() {
-      float mx = sc[0][n][0];
-#pragma unroll
-      for (int kb = 0; kb < T::KB; ++kb)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[kb][n][r]);
-      return at_pair_max(mx) * scale;
-    };
-    auto raise = [&](float mx, bool need) {
-      const float mn = need ? fmaxf(m[n], mx) : m[n], al = __builtin_amdgcn_exp2f(m[n] - mn);
-      m[n] = mn;
-      l[n] *= al;
-#pragma unroll
-      for (int db = 0; db < T::DB; ++db)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[db][n][r] *= al;
-    };
-    // p of all keys; their sum
-    auto probs = [&]() -> float {
-      const float off = kAtBias<T::DT> - m[n];
-      float sum = 0.0f;
-#pragma unroll
-      for (int kb = 0; kb < T::KB; ++kb)
-#pragma unroll
-        for (int r = 0; r < 16; r += 2) {
-          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb][n][r], scale, off));
-          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb][n][r + 1], scale, off));
-          if constexpr (T::F32) {
-            sc[kb][n][r] = p0, sc[kb][n][r + 1] = p1;
-            sum += p0 + p1;
-          } else {
-            const uint32_t p = pack2<T::DT>(p0, p1);
-            pb[kb][r / 8][n][r % 8 / 2] = p;
-            sum = at_dot_ones<T::DT>(p, sum);
-          }
-        }
-      return sum;
-    };
-    float sum;
-    if constexpr (T::LAZY) {
-      sum = probs();
-      const bool big = !(sum < kAtMost);
-      if (__any(big)) {
-        raise(top(), at_pair_max(big ? 1.0f : 0.0f) != 0.0f);
-        sum = probs();
-      }
+  for (int w = w0; w < w1; ++w) {
+    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * w], scale, off));
+    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * w + 1], scale, off));
+    if constexpr (T::F32) {
+      p[2 * w] = p0, p[2 * w + 1] = p1;
+      sum += p0 + p1;
     } else {
-      const float mx = top();
-      const bool need = mx > m[n] + kAtSlack;
-      if (__any(need)) raise(mx, need);
-      sum = probs();
+      const uint32_t x = pack2<T::DT>(p0, p1);
+      p.h[w / 4][w % 4] = x;
+      sum = at_dot_ones<T::DT>(x, sum);
     }
-    l[n] += sum;
   }
+  return sum;
+}
+// The rows' maximum over N blocks, in the exponent's units.
+template <class T, int N>
+__device__ __forceinline__ float at_top(const f32x16 (&sc)[N], float scale) {
+  float mx = sc[0][0];
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[i][r]);
+  return at_pair_max(mx) * scale;
+}
+// The rows that need it (`row`) get the larger maximum.
+template <class T>
+__device__ __forceinline__ void at_raise(float mx, bool row, float &m, float &l, f32x16 (&o)[T::DB]) {
+  const float mn = row ? fmaxf(m, mx) : m, al = __builtin_amdgcn_exp2f(m - mn);
+  m = mn;
+  l *= al;
+#pragma unroll
+  for (int db = 0; db < T::DB; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[db][r] *= al;
+}
+// `sum` is at_probs' of N blocks: the rows that it is too large for get their
+// maximum found and their probabilities again.
+template <class T, int N>
+__device__ __forceinline__ void at_settle(const f32x16 (&sc)[N], typename T::Probs (&p)[N], float sum, float &m,
+                                          float &l, f32x16 (&o)[T::DB], float scale) {
+  const bool big = !(sum < kAtMost);
+  if (__any(big)) {
+    at_raise<T>(at_top<T>(sc, scale), at_pair_max(big ? 1.0f : 0.0f) != 0.0f, m, l, o);
+    sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum = at_probs<T>(sc[i], p[i], m, scale, 0, 8, sum);
+  }
+  l += sum;
+}
+// The softmax of N blocks: p, the maximum m and this lane's share of the sum l.
+template <class T, int N>
+__device__ __forceinline__ void at_softmax(const f32x16 (&sc)[N], typename T::Probs (&p)[N], float &m, float &l,
+                                           f32x16 (&o)[T::DB], float scale) {
+  if constexpr (!T::LAZY) {
+    const float mx = at_top<T>(sc, scale);
+    const bool row = mx > m + kAtSlack;
+    if (__any(row)) at_raise<T>(mx, row, m, l, o);
+  }
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) sum = at_probs<T>(sc[i], p[i], m, scale, 0, 8, sum);
+  if constexpr (T::LAZY) at_settle<T>(sc, p, sum, m, l, o, scale);
+  else l += sum;
 }
 
 // O^T += V^T P^T; CLEAN: infinite and NaN values of V count as zero.
 template <class T, bool CLEAN>
-__device__ __forceinline__ void at_pv(const char *vt, const f32x16 (&sc)[T::KB][T::NQ],
-                                      const u32x4 (&pb)[T::KB][2][T::NQ], f32x16 (&o)[T::DB][T::NQ], int lane) {
+__device__ __forceinline__ void at_pv(const char *vt, const typename T::Probs &pb, f32x16 (&o)[T::DB], int lane) {
   const uint32_t l32 = lane & 31, lh = lane >> 5;
   if constexpr (T::F32) {
     const char *p = vt + 4 * lh * T::RB + l32 * 4;
 #pragma unroll
-    for (int kb = 0; kb < T::KB; ++kb)
+    for (int r = 0; r < 16; ++r)
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-#pragma unroll
-        for (int db = 0; db < T::DB; ++db) {
-          uint32_t v = *reinterpret_cast<const uint32_t *>(p + (32 * kb + 8 * (r / 4) + r % 4) * T::RB + 128 * db);
-          if constexpr (CLEAN) v = at_finite_only<T::DT>(v);
-#pragma unroll
-          for (int n = 0; n < T::NQ; ++n)
-            o[db][n] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(v), sc[kb][n][r], o[db][n], 0, 0, 0);
-        }
+      for (int db = 0; db < T::DB; ++db) {
+        uint32_t v = *reinterpret_cast<const uint32_t *>(p + (8 * (r / 4) + r % 4) * T::RB + 128 * db);
+        if constexpr (CLEAN) v = at_finite_only<T::DT>(v);
+        o[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(v), pb[r], o[db], 0, 0, 0);
+      }
   } else {
     // a transposing read: 16 lanes read 4 rows x 16 columns, 8 bytes each
     // (row lane / 4, columns 4 (lane % 4) ..), and lane i gets column i
     const uint32_t row = 4 * lh + ((lane & 15) >> 2), sw = at_vswz<T>(row);
 #pragma unroll
-    for (int kb = 0; kb < T::KB; ++kb)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int db = 0; db < T::DB; ++db) {
+        const uint32_t unit = (4 * db + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ sw;
+        const char *p = vt + (16 * h + row) * T::RB + unit * 16 + (lane & 1) * 8;
+        const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_lds_s16x4 *)p);
+        const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_lds_s16x4 *)(p + 8 * T::RB));
+        u32x4 v = __builtin_bit_cast(u32x4, s16x8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]});
+        if constexpr (CLEAN) {
 #pragma unroll
-        for (int db = 0; db < T::DB; ++db) {
-          const uint32_t unit = (4 * db + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ sw;
-          const char *p = vt + (32 * kb + 16 * h + row) * T::RB + unit * 16 + (lane & 1) * 8;
-          const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_lds_s16x4 *)p);
-          const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_lds_s16x4 *)(p + 8 * T::RB));
-          u32x4 v = __builtin_bit_cast(u32x4, s16x8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]});
-          if constexpr (CLEAN) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = at_finite_only<T::DT>(v[e]);
-          }
-#pragma unroll
-          for (int n = 0; n < T::NQ; ++n) {
-            if constexpr (T::DT == DT_F16)
-              o[db][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                  __builtin_bit_cast(f16x8, v), __builtin_bit_cast(f16x8, pb[kb][h][n]), o[db][n], 0, 0, 0);
-            else
-              o[db][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                  __builtin_bit_cast(bf16x8, v), __builtin_bit_cast(bf16x8, pb[kb][h][n]), o[db][n], 0, 0, 0);
-          }
+          for (int e = 0; e < 4; ++e) v[e] = at_finite_only<T::DT>(v[e]);
         }
+        o[db] = at_mfma<T>(v, pb.h[h], o[db]);
+      }
   }
+}
+
+// A step of 16-bit heads: the scores of the next block (K at kt; they replace
+// sc), the product of the last block's probabilities (V at vt; p) and the
+// probabilities of the block in between (sc; they replace p). None waits for
+// another: a product of each kind and a share of the exponentials at a time, the
+// operands of the next two on their way. The compiler on its own puts each
+// product behind the wait for its operand, and the exponentials after them.
+template <class T, class Q>
+__device__ __forceinline__ void at_step(const char *kt, const char *vt, Q q, f32x16 (&sc)[1], typename T::Probs (&p)[1],
+                                        float &m, float &l, f32x16 (&o)[T::DB], float scale, int lane) {
+  constexpr int N = T::NC, FIRST = 2;  // products of each kind; operands on their way
+  const uint32_t l32 = lane & 31, lh = lane >> 5, sw = at_kswz<T>(l32);
+  const uint32_t row = 4 * lh + ((lane & 15) >> 2), vsw = at_vswz<T>(row);
+  u32x4 kk[N], vv[N];
+  auto load = [&](int i) __attribute__((always_inline)) {
+    kk[i] = *reinterpret_cast<const u32x4 *>(kt + l32 * T::RB + (((2 * i + lh) ^ sw) * 16));
+    const int h = i / T::DB, db = i % T::DB;
+    const uint32_t unit = (4 * db + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ vsw;
+    const char *at = vt + (16 * h + row) * T::RB + unit * 16 + (lane & 1) * 8;
+    const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_lds_s16x4 *)at);
+    const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_lds_s16x4 *)(at + 8 * T::RB));
+    vv[i] = __builtin_bit_cast(u32x4, s16x8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]});
+  };
+  f32x16 next{};
+  typename T::Probs pn[1];
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < FIRST; ++i) load(i);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    __builtin_amdgcn_sched_barrier(0);
+    if (i + FIRST < N) load(i + FIRST);
+    sum = at_probs<T>(sc[0], pn[0], m, scale, 8 * i / N, 8 * (i + 1) / N, sum);
+    next = at_mfma<T>(kk[i], q(i), next);
+    o[i % T::DB] = at_mfma<T>(vv[i], p[0].h[i / T::DB], o[i % T::DB]);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  p[0] = pn[0];
+  at_settle<T>(sc, p, sum, m, l, o, scale);
+  sc[0] = next;
 }
 
 // The larger magnitude, per value, of a running maximum and of four words of V.
@@ -345,17 +374,18 @@ __device__ __forceinline__ uint32_t at_max_abs(uint32_t m, u32x4 v) {
 // Keys that some rows of a tile see and others do not: 0 * NaN or 0 * inf of an
 // unseen value must not reach a row. If keys `from` .. `end` - 1 of the tile,
 // which hold all of those, have such values, the tile's are added to the rows
-// that see them (keys below to[n]) one by one, and the product runs without
+// that see them (keys below `to`) one by one, and the product runs without
 // them. True: it has some.
 template <class T>
 __device__ __forceinline__ bool at_spread_nonfinite(const char *vt, uint32_t from, uint32_t end,
-                                                    const uint32_t (&to)[T::NQ], f32x16 (&o)[T::DB][T::NQ], int lane) {
+                                                    uint32_t to, f32x16 (&o)[T::DB], int lane) {
   uint32_t big = 0;
+  end = min(end, 32u);
   for (uint32_t i = from * T::PU + lane; i < end * T::PU; i += 64)
     big = at_max_abs<T::DT>(big, *reinterpret_cast<const u32x4 *>(vt + i * 16));
   if (!__any(at_nonfinite<T::DT>(big) != 0)) return false;
   const uint32_t lh = lane >> 5;
-  for (uint32_t j = 0; j < T::KEYS; ++j) {
+  for (uint32_t j = 0; j < 32; ++j) {
 #pragma unroll
     for (int db = 0; db < T::DB; ++db)
 #pragma unroll
@@ -367,9 +397,7 @@ __device__ __forceinline__ bool at_spread_nonfinite(const char *vt, uint32_t fro
         else v = unpack4<T::DT>(*reinterpret_cast<const u32x2 *>(p));
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int n = 0; n < T::NQ; ++n)
-            if (at_nonfinite<DT_F32>(__float_as_uint(v[e])) && j < to[n]) o[db][n][4 * r4 + e] += v[e];
+          if (at_nonfinite<DT_F32>(__float_as_uint(v[e])) && j < to) o[db][4 * r4 + e] += v[e];
       }
   }
   return true;
@@ -422,23 +450,20 @@ __device__ __forceinline__ uint32_t at_shift(const AttnArgs &a, uint32_t len) {
   return x;
 }
 
-// The query rows of a wavefront from row0 on: unit u of block n's row l32, zero
-// where there is none. Offsets from the first row's token fit 32 bits.
+// The query rows of a wavefront from row0 on: unit u of row l32, zero where there
+// is none. Offsets from the first row's token fit 32 bits.
 template <class T>
 struct AtQuery {
   __amdgpu_buffer_rsrc_t rs;
-  uint32_t off[T::NQ];
+  uint32_t off;
   __device__ __forceinline__ AtQuery(const AttnArgs &a, const AtSeq &s, uint32_t hk, uint32_t row0, uint32_t l32) {
     const uint32_t nrows = s.lq * a.g, tok0 = fdiv(min(row0, nrows - 1), a.by_g);
     rs = at_rsrc((const char *)a.q + ((uint64_t)(s.q0 + tok0) * a.qs + (uint64_t)hk * a.g * a.d) * T::EB, 0x7fffffffu);
-#pragma unroll
-    for (int n = 0; n < T::NQ; ++n) {
-      const uint32_t row = row0 + 32 * n + l32, tok = fdiv(row, a.by_g);
-      off[n] = row < nrows ? ((tok - tok0) * (uint32_t)a.qs + (row - tok * a.g) * a.d) * T::EB : kAtOob;
-    }
+    const uint32_t row = row0 + l32, tok = fdiv(row, a.by_g);
+    off = row < nrows ? ((tok - tok0) * (uint32_t)a.qs + (row - tok * a.g) * a.d) * T::EB : kAtOob;
   }
-  __device__ __forceinline__ u32x4 unit(const AttnArgs &a, int n, uint32_t u) const {
-    const uint32_t o = u * T::UE < a.d ? off[n] + u * 16 : kAtOob;
+  __device__ __forceinline__ u32x4 unit(const AttnArgs &a, uint32_t u) const {
+    const uint32_t o = u * T::UE < a.d ? off + u * 16 : kAtOob;
     return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, o, 0, 0));
   }
 };

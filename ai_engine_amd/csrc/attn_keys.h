@@ -16,7 +16,7 @@ namespace {
 // products of one wavefront cover the waits and the softmax of another.
 template <int DT, int DP, int WK_>
 struct AtKeysCfg {
-  using T = AtTile<DT, DP, 1, 1>;
+  using T = AtTile<DT, DP>;
   static constexpr int WK = WK_;
   static constexpr int KEYS = 32 * WK;
   static constexpr bool ONE = T::RB >= 512 && T::F32;
@@ -129,69 +129,69 @@ __global__ __launch_bounds__(64 * C::WK, C::WPE) void attn_keys_kernel(AttnArgs 
     if constexpr (C::QL) {  // row l32 in LDS as a row of K, the wavefronts sharing the units
 #pragma unroll 4
       for (int c = wave; c < T::NC; c += WK)
-        *reinterpret_cast<u32x4 *>(ql + (((2 * c + lh) ^ at_kswz<T>(l32)) * 16)) = src.unit(a, 0, 2 * c + lh);
+        *reinterpret_cast<u32x4 *>(ql + (((2 * c + lh) ^ at_kswz<T>(l32)) * 16)) = src.unit(a, 2 * c + lh);
       __syncthreads();
     } else {
 #pragma unroll
-      for (int c = 0; c < T::NC; ++c) q[c] = src.unit(a, 0, 2 * c + lh);
+      for (int c = 0; c < T::NC; ++c) q[c] = src.unit(a, 2 * c + lh);
     }
-    auto query = [&](int, int c) -> u32x4 {
+    auto query = [&](int c) -> u32x4 {
       if constexpr (C::QL) return *reinterpret_cast<const u32x4 *>(ql + (((2 * c + lh) ^ at_kswz<T>(l32)) * 16));
       else return q[c];
     };
     const uint32_t lim = at_limit(a, causal, s, row0 + l32);
 
-    f32x16 o[DB][1];
-    float m[1] = {kAtLowest}, l[1] = {0.0f};
+    f32x16 o[DB];
+    float m = kAtLowest, l = 0.0f;
 #pragma unroll
-    for (int db = 0; db < DB; ++db) o[db][0] = f32x16{};
+    for (int db = 0; db < DB; ++db) o[db] = f32x16{};
 
     for (; key < kend; key += C::KEYS) {
-      f32x16 sc[1][1];
-      u32x4 pb[1][2][1];
       at_wait_vm<C::ONE ? 0 : C::NI>();  // K is there, V may still be on its way
       __asm__ volatile("" ::: "memory");
+      f32x16 sc[1];
+      typename T::Probs p[1];
       at_qk<T>(kt, query, sc, lane);
       // K's buffer is requested again: its reads are behind this wavefront
       __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       if constexpr (C::ONE) issue_v(key);
       else issue_k(key + C::KEYS);
-      const uint32_t to[1] = {max(min(kend, lim), key) - key};
-      if (key + 32 > min(kend, smin)) at_mask<T>(sc, to, lane);
-      at_softmax<T>(sc, pb, m, l, o, a.scale_log2);
+      const uint32_t to = max(min(kend, lim), key) - key;
+      if (key + 32 > min(kend, smin)) at_mask(sc[0], to, lane);
+      at_softmax<T>(sc, p, m, l, o, a.scale_log2);
       at_wait_vm<C::ONE ? 0 : C::NI>();  // V is there, the next K on its way
       __asm__ volatile("" ::: "memory");
       const uint32_t end = min(kend, key + 32);
       if (smin < end && at_spread_nonfinite<T>(vt, max(smin, key) - key, end - key, to, o, lane))
-        at_pv<T, true>(vt, sc, pb, o, lane);
+        at_pv<T, true>(vt, p[0], o, lane);
       else
-        at_pv<T, false>(vt, sc, pb, o, lane);
+        at_pv<T, false>(vt, p[0], o, lane);
       __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       if constexpr (C::ONE) issue_k(key + C::KEYS);
       else issue_v(key + C::KEYS);
     }
     at_wait_vm<0>();  // nothing is on its way into LDS any more
-    l[0] = at_pair_sum(l[0]);
+    l = at_pair_sum(l);
 
     // join the wavefronts' keys: a common maximum, scaled sums through LDS
     float *jo = reinterpret_cast<float *>(lds);
     float *jml = jo + WK * 32 * C::OPITCH;
     __syncthreads();
     if (lh == 0) {
-      jml[wave * 64 + l32] = m[0];
-      jml[wave * 64 + 32 + l32] = l[0];
+      jml[wave * 64 + l32] = m;
+      jml[wave * 64 + 32 + l32] = l;
     }
     __syncthreads();
     float mm = jml[l32];
 #pragma unroll
     for (int w = 1; w < WK; ++w) mm = fmaxf(mm, jml[w * 64 + l32]);
-    const float f = __builtin_amdgcn_exp2f(m[0] - mm);
+    const float f = __builtin_amdgcn_exp2f(m - mm);
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4)
         *reinterpret_cast<f32x4 *>(jo + (wave * 32 + l32) * C::OPITCH + 32 * db + 8 * r4 + 4 * lh) =
-            f32x4{o[db][0][4 * r4], o[db][0][4 * r4 + 1], o[db][0][4 * r4 + 2], o[db][0][4 * r4 + 3]} * f;
+            f32x4{o[db][4 * r4], o[db][4 * r4 + 1], o[db][4 * r4 + 2], o[db][4 * r4 + 3]} * f;
     __syncthreads();
     const uint64_t rows_all = (uint64_t)a.tokens * a.hq;
     const uint64_t ml0 = attn_ws_ml(a);
