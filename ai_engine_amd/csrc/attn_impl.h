@@ -116,14 +116,18 @@ struct AtTile {
 };
 
 // LDS layout of a tile of rows: unit u of row r at slot u ^ swz(r) of its PU
-// slots, so that the operand reads (8 consecutive rows, one unit each, of K; 4
-// rows, 2 units each, of 16-bit V) touch 8 distinct bank groups. fp32 V is read
-// along its rows and needs none.
+// slots. A cycle serves 256 bytes, all 64 banks: 16 lanes of a read of K (16
+// consecutive rows, one unit each) or 32 of a transposing read of 16-bit V (4
+// rows, 4 units each), which the slots spread over the 16 groups of 4 banks. With
+// swizzles for 8 groups every read of 128 elements took twice the cycles. fp32 V
+// is read along its rows and has none.
 template <class T>
-__device__ __forceinline__ uint32_t at_kswz(uint32_t r) { return T::PU >= 8 ? r & 7 : (r >> 1) & 3; }
+__device__ __forceinline__ uint32_t at_kswz(uint32_t r) {
+  return T::PU >= 16 ? r & 15 : T::PU == 8 ? (r >> 1) & 7 : (r >> 2) & 3;
+}
 template <class T>
 __device__ __forceinline__ uint32_t at_vswz(uint32_t r) {
-  return T::F32 ? 0 : T::PU >= 8 ? (r & 3) << 1 : ((r >> 1) & 1) << 1;
+  return T::F32 ? 0 : T::PU >= 16 ? (r & 3) << 2 : T::PU == 8 ? (r & 3) << 1 : 0;
 }
 
 // DMA of instructions i0 .. i0 + NI - 1 of a tile (1 KB, RPI rows each): lane ->
