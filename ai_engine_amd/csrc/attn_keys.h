@@ -142,6 +142,9 @@ __global__ __launch_bounds__(64 * C::WK, C::WPE) void attn_keys_kernel(AttnArgs 
         *reinterpret_cast<u32x4 *>(ql + (((2 * c + lh) ^ at_kswz<T>(l32)) * 16)) = src.unit(a, 2 * c + lh);
       __syncthreads();
     } else {
+      // The compiler waits for these in the loop, in the scores, and with that for
+      // V. A wait of its own in front of the loop makes prompts 3 % and a prefix 2 %
+      // faster and decode steps 2 to 5 % slower (16 x 1024 keys 13.9 -> 14.6 us).
 #pragma unroll
       for (int c = 0; c < T::NC; ++c) q[c] = src.unit(a, 2 * c + lh);
     }
