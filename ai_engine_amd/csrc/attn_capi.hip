@@ -68,7 +68,9 @@ enum class Use { OWN, PREFIX };
 // fp32, 1 stream, 8/2 heads of 64: 384 10.9 | 11.5 us, 512 13.1 | 11.6; a prompt of
 // 1024, 4/4 heads (128 items) 22.7 | 18.8. Few rows are cut at 1024 anyway, since
 // the sequences' lengths may differ a lot. 64 streams behind a prefix of 4096,
-// 32/8 heads of 128: 8 parts 29.2 us, 4 parts 25.1.
+// 32/8 heads of 128: 8 parts 29.2 us, 4 parts 25.1; but 64 of 4 tokens, heads of 64
+// (512 items) 1 part 34.9, 2 parts 26.9: more than 2048 of a prefix's 16-bit keys
+// are too long a chain.
 //
 // A stage of 128 fp32 keys takes 1 us per 32 elements, a chain that shorter parts
 // make the shorter the larger the heads (`heavy`; 1 stream of 271 keys, 16/4 heads of
@@ -93,6 +95,8 @@ Cover cover(int32_t kernel, uint32_t nseq, uint64_t rows, uint32_t len, uint32_t
   const uint32_t least = std::max(7u, (few && use == Use::OWN ? 8 : 9) - heavy);
   c.shift = 31;
   if (len > whole) {
+    if (use == Use::PREFIX && dt != AIH_F32)
+      while (c.shift > 11 && base * parts(c.shift) < 2 * cus) --c.shift;
     if (few && use == Use::OWN) c.shift = len > 2u << (10 - heavy) ? 10 - heavy : 10;
     while (c.shift > least && base * parts(c.shift) < items &&
            (dt != AIH_F32 || use == Use::PREFIX ||
@@ -153,11 +157,16 @@ int check_attn(const aih_attn_desc *d, AttnArgs *a, AttnPlan *p) {
   p->all_parts = p->own.parts;
   if (d->prefix) {
     // The prefix's keys over the wavefronts re-read them for every 32 rows, but
-    // share a launch and leave few partial results: the faster as long as rows x
-    // keys are few. 16 own keys, 32/8 heads of 128, bf16, together | apart: 128
-    // streams behind 4096 keys 34 | 38 us, behind 16384 72 | 68; 256 behind 4096 59 |
-    // 63, behind 16384 146 | 117.
-    p->together = kernel == AIH_ATTN_KEYS && (rows * d->prefix <= 1u << 22 || !rows_fit);
+    // share a launch and leave few partial results: the faster as long as that is not
+    // much to read. 1 to 134 own keys, bf16, together | apart: 64 streams of 4 tokens,
+    // 12/2 heads of 128, behind 4096 keys 24 | 30 us, behind 8000 34 | 39; 128 of 1
+    // token behind 24000 49 | 49; 64 x 4, 8/2 heads of 64, behind 8000 20 | 23, behind
+    // 24000 37 | 35; 64 x 1, 32/8 heads of 128, behind 24000 74 | 58; 16 x 4, 16/4 heads
+    // of 256, behind 24000 86 | 84, behind 60000 147 | 127. fp32 is bound by its
+    // products: 64 x 4, 32/8 heads of 64 behind 1500 to 24000 keys 43 | 55, 89 | 92, 161
+    // | 160, 481 | 526, of 128 76 | 99, 172 | 168, 341 | 296, 996 | 1011.
+    const bool little = rows * d->hkv * d->prefix <= (1ull << 32) / std::max(d->d, 128u);
+    p->together = kernel == AIH_ATTN_KEYS && (little || d->dt == AIH_F32);
     p->pre = cover(p->together ? AIH_ATTN_KEYS : AIH_ATTN_ROWS, 1, rows, d->prefix, d->hkv, d->dt, d->d, Use::PREFIX);
     p->all_parts += p->pre.parts;
   }
