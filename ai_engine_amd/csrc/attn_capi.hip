@@ -79,7 +79,9 @@ enum class Use { OWN, PREFIX };
 // (40 x 600 keys, 4/4 heads of 32, 160 items 11.7 | 18.9; a prompt of 300, 16/4 heads
 // of 256, 152 items 37.7 | 44.3), another one up to a quarter more (8 x 2000, 18/3
 // heads of 256, 8 parts 39.1, 16 parts, 432 items, 49.2; 16 x 4000, 8/2 heads of 64, 4
-// parts 27.9, 8 parts, 288 items, 21.6).
+// parts 27.9, 8 parts, 288 items, 21.6). One of 256 16-bit elements takes 2 us: with
+// few rows shorter parts pay, too (4 x 600 keys, 16/4 heads 14.6 | 11.8; 16 x 600, 72
+// items 15.5 | 18.6).
 Cover cover(int32_t kernel, uint32_t nseq, uint64_t rows, uint32_t len, uint32_t hkv, int32_t dt, uint32_t d, Use use) {
   const uint32_t cus = device_cus();
   Cover c{};
@@ -89,15 +91,15 @@ Cover cover(int32_t kernel, uint32_t nseq, uint64_t rows, uint32_t len, uint32_t
   const uint64_t base = (uint64_t)c.tiles * hkv;
   auto parts = [&](uint32_t x) { return std::max(1u, div_up(len, 1ull << x)); };
   const bool few = rows <= 32ull * nseq;
-  const uint32_t heavy = dt != AIH_F32 ? 0 : d > 128 ? 2 : d > 64 ? 1 : 0;
-  const uint32_t whole = use == Use::PREFIX ? 0 : kernel == AIH_ATTN_ROWS ? len : dt == AIH_F32 ? 384 >> heavy : 768;
+  const uint32_t heavy = dt != AIH_F32 ? d > 128 && 4 * base < cus : d > 128 ? 2 : d > 64 ? 1 : 0;
+  const uint32_t whole = use == Use::PREFIX ? 0 : kernel == AIH_ATTN_ROWS ? len : (dt == AIH_F32 ? 384 : 768) >> heavy;
   const uint32_t items = use == Use::PREFIX || dt == AIH_F32 ? cus : cus / 2;
   const uint32_t least = std::max(7u, (few && use == Use::OWN ? 8 : 9) - heavy);
   c.shift = 31;
   if (len > whole) {
     if (use == Use::PREFIX && dt != AIH_F32)
       while (c.shift > 11 && base * parts(c.shift) < 2 * cus) --c.shift;
-    if (few && use == Use::OWN) c.shift = len > 2u << (10 - heavy) ? 10 - heavy : 10;
+    if (few && use == Use::OWN) c.shift = dt == AIH_F32 && len > 2u << (10 - heavy) ? 10 - heavy : 10;
     while (c.shift > least && base * parts(c.shift) < items &&
            (dt != AIH_F32 || use == Use::PREFIX ||
             base * parts(c.shift - 1) <= (parts(c.shift) > 1 ? cus + cus / 4 : cus)))
