@@ -5,8 +5,9 @@
 // for the rotated pairs. Everything is fp32 between the load and the store,
 // which rounds once.
 //
-// An item is one head of one token; P lanes (a power of two) take it, each two
-// vectors of VW elements. With halves the two are partners (unit j and unit
+// An item is one head of one token; P lanes (a power of two, or the exact number
+// where that would leave more than a quarter of them idle: 30000 tokens of 24 f16
+// heads of 80 61 -> 52 us, of 72 85 -> 60) take it, each two vectors of VW elements. With halves the two are partners (unit j and unit
 // j + rot/2), so a rotation needs no exchange between lanes; the only exchange
 // is the sum of squares over the P lanes. VW is 16 bytes unless the rotated
 // half is no whole number of such units, then 8 or 4 bytes. Items follow the
@@ -26,6 +27,7 @@ namespace aih {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr uint32_t kAnyLanes = 31;  // for pshift: the lanes of an item are no power of two
 
 // VW elements as stored, and as fp32.
 template <int DT, int VW>
@@ -74,8 +76,13 @@ template <int DT, int VW>
 __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(QkRopeArgs a, uint32_t pshift) {
   constexpr int EB = Storage<DT>::bytes;
   const uint32_t lane = threadIdx.x & 63;
-  const uint32_t j = lane & ((1u << pshift) - 1);
-  const uint64_t item = ((uint64_t)blockIdx.x * kThreads + threadIdx.x) >> pshift;
+  uint32_t j = lane & ((1u << pshift) - 1);
+  uint64_t item = ((uint64_t)blockIdx.x * kThreads + threadIdx.x) >> pshift;
+  if (pshift == kAnyLanes) {  // groups of nl lanes; the last ones of a wavefront have none
+    const uint32_t per = 64 / a.nl, g = lane / a.nl;
+    j = lane - g * a.nl;
+    item = g < per ? ((uint64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6)) * per + g : a.items;
+  }
   // a group past the end keeps to the last item, and stores nothing: the lanes
   // of a wavefront stay together for the exchange
   const bool live = item < a.items;
@@ -120,7 +127,15 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(QkRopeArgs a, ui
   float ss = 0.0f;
 #pragma unroll
   for (int i = 0; i < VW; ++i) ss += f0[i] * f0[i] + f1[i] * f1[i];
-  for (uint32_t m = 1; m < (1u << pshift); m <<= 1) ss += __shfl_xor(ss, m);
+  if (pshift == kAnyLanes) {  // to the group's first lane, and from there to all
+    for (uint32_t m = 1; m < a.nl; m <<= 1) {
+      const float up = __shfl(ss, lane + m);
+      if (j % (2 * m) == 0 && j + m < a.nl) ss += up;
+    }
+    ss = __shfl(ss, lane - j);
+  } else {
+    for (uint32_t m = 1; m < (1u << pshift); m <<= 1) ss += __shfl_xor(ss, m);
+  }
 
   if (!is_v) {  // a value head keeps the bits it was loaded with
     const float r = __builtin_amdgcn_rsqf(ss * a.inv_d + a.eps);
@@ -189,10 +204,17 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(QkRopeArgs a, ui
 
 template <int DT, int VW>
 hipError_t launch_vw(const QkRopeArgs &a, hipStream_t st) {
+  // Lanes of an item: a power of two, or, where that left more than a quarter of
+  // them idle, exactly those it needs.
   uint32_t ps = 0;
   while ((1u << ps) < a.nl) ++ps;
-  const uint64_t blocks = ((a.items << ps) + kThreads - 1) / kThreads;
-  if (ps > 6 || blocks > 0x7fffffffu) return hipErrorInvalidValue;
+  uint64_t blocks = ((a.items << ps) + kThreads - 1) / kThreads;
+  if (4 * a.nl < 3u << ps) {
+    const uint32_t per = kThreads / 64 * (64 / a.nl);
+    ps = kAnyLanes;
+    blocks = (a.items + per - 1) / per;
+  }
+  if ((ps > 6 && ps != kAnyLanes) || blocks > 0x7fffffffu) return hipErrorInvalidValue;
   hipLaunchKernelGGL((qk_norm_rope_kernel<DT, VW>), dim3((uint32_t)blocks), dim3(kThreads), 0, st, a, ps);
   return hipGetLastError();
 }
