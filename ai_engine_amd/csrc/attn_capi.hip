@@ -150,10 +150,16 @@ int check_attn(const aih_attn_desc *d, AttnArgs *a, AttnPlan *p) {
   // tokens, 16/4 heads of 96 (512 tiles) 564 | 436 us, 4 x 2048 tokens (1040) 573 |
   // 487, 16 x 720 (1504) 293 | 321; 16 bit, 2880 tokens, 8/2 heads of 64 (180) 41 |
   // 25, 16/4 heads (360) 44.6 | 43.6, of 128 63 | 70; 40 x 100 tokens, 8/2 heads of
-  // 128 (330) 14 | 19: too short to share.
+  // 128 (330) 14 | 19: too short to share. So are fp32 heads above 64 elements, the
+  // longer the more there are: 16/4 heads of 128, 4 x 100 tokens (60 tiles) 21 | 11.5,
+  // 40 x 64 (400) 30 | 41, 8 x 260 (276) 76 | 50, 20 x 300 (792) 125 | 137, 3 x 700
+  // (268) 105 | 80. Above 128 16-bit elements a wavefront's chain is written out: 8/4
+  // heads of 256, 520 tokens (36) 26 | 15, 2 x 900 (120) 38 | 30, 8 x 260 (148) 20 | 28,
+  // 6 x 520 (208) 28 | 42, 3000 (188) 100 | 92, not causal 105 | 149.
   const uint64_t tiles = (uint64_t)d->hkv * (div_up(rows, attn_bm(AIH_ATTN_ROWS, d->dt, d->d)) + d->nseq / 2);
   const uint64_t cus = device_cus();
-  const bool chain = d->dt == AIH_F32 ? tiles < 5 * cus : tiles < cus && len >= 256;
+  const bool chain = d->dt == AIH_F32 ? tiles < 5 * cus && (d->d <= 64 || 180 * tiles < cus * len)
+                                      : tiles < (d->d > 128 ? cus / 2 : cus) && len >= 256;
   const int32_t kernel = rows <= 32ull * d->nseq || !rows_fit || chain ? AIH_ATTN_KEYS : AIH_ATTN_ROWS;
   p->own = cover(kernel, d->nseq, rows, len, d->hkv, d->dt, d->d, Use::OWN);
   p->all_parts = p->own.parts;
