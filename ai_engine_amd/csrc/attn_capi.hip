@@ -77,11 +77,12 @@ enum class Use { OWN, PREFIX };
 // 256: 33.0 | 18.2 us; 5 behind a prefix of 651: 2 parts 47.3, 6 parts 19.8), as
 // long as the parts still run at once: a first cut that does not fit the CUs loses
 // (40 x 600 keys, 4/4 heads of 32, 160 items 11.7 | 18.9; a prompt of 300, 16/4 heads
-// of 256, 152 items 37.7 | 44.3), another one up to a quarter more (8 x 2000, 18/3
-// heads of 256, 8 parts 39.1, 16 parts, 432 items, 49.2; 16 x 4000, 8/2 heads of 64, 4
-// parts 27.9, 8 parts, 288 items, 21.6). One of 256 16-bit elements takes 2 us: with
-// few rows shorter parts pay, too (4 x 600 keys, 16/4 heads 14.6 | 11.8; 16 x 600, 72
-// items 15.5 | 18.6).
+// of 256, 152 items 37.7 | 44.3), another one where it leaves a few over (8 x 2000,
+// 18/3 heads of 256, 8 parts 39.1, 16 parts, 432 items, 49.2). Few rows of at most 128
+// elements run twice a CU: 16 x 2000 keys, 32/8 heads of 64, 2 parts 34.6, 4 parts 33.4, of
+// lengths from 0 to 2000 28.5 | 19.3; in 16 bit that is a tenth slower.
+// One of 256 16-bit elements takes 2 us: with few rows shorter parts pay, too (4 x 600
+// keys, 16/4 heads 14.6 | 11.8; 16 x 600, 72 items 15.5 | 18.6).
 Cover cover(int32_t kernel, uint32_t nseq, uint64_t rows, uint32_t len, uint32_t hkv, int32_t dt, uint32_t d, Use use) {
   const uint32_t cus = device_cus();
   Cover c{};
@@ -93,7 +94,9 @@ Cover cover(int32_t kernel, uint32_t nseq, uint64_t rows, uint32_t len, uint32_t
   const bool few = rows <= 32ull * nseq;
   const uint32_t heavy = dt != AIH_F32 ? d > 128 && 4 * base < cus : d > 128 ? 2 : d > 64 ? 1 : 0;
   const uint32_t whole = use == Use::PREFIX ? 0 : kernel == AIH_ATTN_ROWS ? len : (dt == AIH_F32 ? 384 : 768) >> heavy;
-  const uint32_t items = use == Use::PREFIX || dt == AIH_F32 ? cus : cus / 2;
+  // what the chip runs at once: two workgroups a CU, but one of large or many rows
+  const uint32_t slots = few && use == Use::OWN && heavy < 2 ? 2 * cus : cus;
+  const uint32_t items = dt == AIH_F32 ? slots : use == Use::PREFIX ? cus : cus / 2;
   const uint32_t least = std::max(7u, (few && use == Use::OWN ? 8 : 9) - heavy);
   c.shift = 31;
   if (len > whole) {
@@ -102,7 +105,7 @@ Cover cover(int32_t kernel, uint32_t nseq, uint64_t rows, uint32_t len, uint32_t
     if (few && use == Use::OWN) c.shift = dt == AIH_F32 && len > 2u << (10 - heavy) ? 10 - heavy : 10;
     while (c.shift > least && base * parts(c.shift) < items &&
            (dt != AIH_F32 || use == Use::PREFIX ||
-            base * parts(c.shift - 1) <= (parts(c.shift) > 1 ? cus + cus / 4 : cus)))
+            base * parts(c.shift - 1) <= (parts(c.shift) > 1 ? slots + cus / 4 : cus)))
       --c.shift;
   }
   c.parts = parts(c.shift);
