@@ -45,6 +45,7 @@ struct AttnArgs {
   uint32_t pre_tiles, pre_parts, pre_shift;  // the prefix's
   FastDiv by_g, by_hkv, by_pre_tiles;
   uint32_t all_parts;
+  uint32_t span;  // keys of the longest part, as far as known
 };
 
 // The workspace: O of every part [all_parts][tokens * hq][d] fp32, not yet

@@ -51,7 +51,7 @@ int launched(const char *fn, hipError_t e) {
 // How a launch covers its rows and keys.
 struct Cover {
   int32_t kernel;
-  uint32_t bm, tiles, parts, shift;
+  uint32_t bm, tiles, parts, shift, span;
 };
 
 uint32_t div_up(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
@@ -110,6 +110,7 @@ Cover cover(int32_t kernel, uint32_t nseq, uint64_t rows, uint32_t len, uint32_t
   }
   c.parts = parts(c.shift);
   if (c.parts == 1) c.shift = 31;
+  c.span = (uint32_t)std::min<uint64_t>(len, 1ull << c.shift);
   return c;
 }
 
@@ -269,6 +270,7 @@ extern "C" int aih_attn(const aih_attn_desc *d, const void *q, const void *k, co
     a.by_pre_tiles = make_fastdiv(std::max(1u, p.pre.tiles));
     a.pk = prefix_k, a.pv = prefix_v, a.prefix = d->prefix;
     a.tiles = p.own.tiles, a.parts = p.own.parts, a.shift = p.own.shift, a.part0 = p.pre.parts;
+    a.span = std::max(p.own.span, p.together ? p.pre.span : 0);
     if (d->prefix && !p.together) {
       AttnArgs b = a;
       b.k = prefix_k, b.v = prefix_v, b.ks = a.pks, b.vs = a.pvs, b.k_start = nullptr;

@@ -10,7 +10,7 @@ hipError_t launch_attn_f16(const AttnArgs &a, int kernel, hipStream_t st) {
   if (a.d <= DP) {                                                                        \
     if constexpr (kAtRowsFit<DT_F16, DP>)                                                 \
       if (kernel == AIH_ATTN_ROWS) return at_launch_rows<AtRows<DT_F16, DP>>(a, st);      \
-    return kernel == AIH_ATTN_KEYS ? at_launch_keys<AtKeys<DT_F16, DP>>(a, cus, st) : hipErrorInvalidValue; \
+    return kernel == AIH_ATTN_KEYS ? at_launch_keys<DT_F16, DP>(a, cus, st) : hipErrorInvalidValue; \
   }
   AIH_AT_CASE(32)
   AIH_AT_CASE(64)

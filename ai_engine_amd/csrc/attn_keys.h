@@ -40,10 +40,9 @@ struct AtKeysCfg {
   // then also the queries are in LDS: the registers hold the results
   static constexpr bool QL = ONE;
   static constexpr uint32_t LDS = BUF + (QL ? HALF : 0) > JOIN ? BUF + (QL ? HALF : 0) : JOIN;
-  // workgroups of a CU, and with that wavefronts of a SIMD, that LDS has room for
-  static constexpr int WPE = 2 * LDS <= 160 * 1024 ? 2 : 1;
+  // wavefronts of a SIMD that LDS has room for
+  static constexpr int WPE = WK == 8 || 2 * LDS <= 160 * 1024 ? 2 : 1;
   static_assert(NI >= 1 && NI < 64, "DMA instructions in flight");
-  static_assert(LDS <= 160 * 1024, "LDS");
 };
 
 // Work items: first the prefix's (part, row tile, key head), then sequence by
@@ -281,17 +280,25 @@ hipError_t at_launch_items(const AttnArgs &a, uint64_t items, uint32_t cus, hipS
 
 // Uncut keys: one item a workgroup, handed out as others end. Cut ones: the
 // items are many, and of those that the host counts (the longest length for
-// all) few may exist, so the workgroups that run at once share them.
-template <class C>
+// all) few may exist, so the workgroups that run at once share them. fp32 heads above
+// 64 elements whose items leave every CU at most one take eight wavefronts, if the
+// keys are more than four take at once: long products of two wavefronts a SIMD fill
+// each other's waits (24 x 130 keys, 32/8 heads of 128 17.4 -> 15.7 us, 24 x 750 46 -> 39;
+// others are too short for the larger join: 180 keys, heads of 64 8.9 -> 9.8).
+template <int DT, int DP>
 hipError_t at_launch_keys(const AttnArgs &a, uint32_t cus, hipStream_t st) {
+  using C = AtKeysCfg<DT, DP, 4>;
+  static_assert(C::LDS <= 160 * 1024, "LDS");
   const uint64_t items = (uint64_t)a.hkv * a.parts * a.tiles + (uint64_t)a.hkv * a.pre_parts * a.pre_tiles;
   if (items == 0 || items > 0x7fffffffu) return hipErrorInvalidValue;
   if (a.parts > 1 && items > cus) return at_launch_items<C, true>(a, items, cus, st);
+  if constexpr (C::ONE) {
+    using C8 = AtKeysCfg<DT, DP, 8>;
+    if constexpr (C8::LDS <= 160 * 1024)
+      if (items <= cus && a.span > C::KEYS) return at_launch_items<C8, false>(a, items, cus, st);
+  }
   return at_launch_items<C, false>(a, items, cus, st);
 }
-
-template <int DT, int DP>
-using AtKeys = AtKeysCfg<DT, DP, 4>;
 
 }  // namespace
 }  // namespace aih
