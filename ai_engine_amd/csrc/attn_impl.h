@@ -423,6 +423,19 @@ __device__ __forceinline__ AtSeq at_load_seq(const AttnArgs &a, uint32_t b) {
   }
   return s;
 }
+// The sequences of a wavefront's lanes (a.nseq of them, at most 64) by the number
+// of their keys: the most first, or last.
+__device__ __forceinline__ AtSeq at_sort(const AttnArgs &a, const AtSeq &s, uint32_t lane, bool most_first) {
+  if (!__any(lane < a.nseq && s.len != (uint32_t)__builtin_amdgcn_readfirstlane(s.len))) return s;
+  uint32_t rank = 0;
+  for (uint32_t i = 0; i < a.nseq; ++i) {
+    const uint32_t other = __builtin_amdgcn_readlane(s.len, i);
+    rank += other > s.len || (other == s.len && i < lane);
+  }
+  const int to = 4 * (lane >= a.nseq ? lane : most_first ? rank : a.nseq - 1 - rank);
+  return AtSeq{(uint32_t)__builtin_amdgcn_ds_permute(to, s.q0), (uint32_t)__builtin_amdgcn_ds_permute(to, s.lq),
+               (uint32_t)__builtin_amdgcn_ds_permute(to, s.k0), (uint32_t)__builtin_amdgcn_ds_permute(to, s.len)};
+}
 __device__ __forceinline__ AtSeq at_seq_of(const AtSeq &s, int l) {
   return AtSeq{(uint32_t)__builtin_amdgcn_readlane(s.q0, l), (uint32_t)__builtin_amdgcn_readlane(s.lq, l),
                (uint32_t)__builtin_amdgcn_readlane(s.k0, l), (uint32_t)__builtin_amdgcn_readlane(s.len, l)};

@@ -63,6 +63,7 @@ __global__ __launch_bounds__(64 * C::WK, C::WPE) void attn_keys_kernel(AttnArgs 
   uint32_t b0 = 0, base = pre_items, n = 0, sum = 0, tiles = 0, parts = 0;
   auto count = [&]() {
     mine = at_load_seq(a, b0 + (threadIdx.x & 63));
+    if (a.sort) mine = at_sort(a, mine, threadIdx.x & 63, true);
     tiles = (mine.lq * a.g + 31) / 32;
     const uint32_t x = at_shift(a, mine.len);
     parts = max(1u, (uint32_t)(((uint64_t)mine.len + (1ull << x) - 1) >> x));

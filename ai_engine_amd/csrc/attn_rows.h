@@ -67,6 +67,7 @@ __global__ __launch_bounds__(64 * C::WR, C::WPE) void attn_rows_kernel(AttnArgs 
   uint32_t n = 0, sum = 0, base = 0;
   auto count = [&](uint32_t b0) {
     mine = at_load_seq(a, b0 + lane);
+    if (a.sort) mine = at_sort(a, mine, lane, false);  // the last come first
     n = (mine.lq * a.g + C::BM - 1) / C::BM;  // tokens * hq is below 2^31
     sum = at_scan(n);
   };
