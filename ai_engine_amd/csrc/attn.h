@@ -46,7 +46,7 @@ struct AttnArgs {
   FastDiv by_g, by_hkv, by_pre_tiles;
   uint32_t all_parts;
   uint32_t span;  // keys of the longest part, as far as known
-  uint32_t sort;  // 1: the sequences with the most keys go first 
+  uint32_t sort;  // 1: the sequences with the most keys go first
 };
 
 // The workspace: O of every part [all_parts][tokens * hq][d] fp32, not yet

@@ -4,7 +4,7 @@
 //
 // A single token's g rows fill g of a tile's 32 columns; the products are cheap
 // beside the keys and values that are read once for them, so that serving is bound
-// by memory: 64 sequences of up to 8192 keys, 32/8 bf16 heads of 128, 82 us at 4.3
+// by memory: 64 sequences of up to 8192 keys, 32/8 bf16 heads of 128, 79 us at 4.5
 // TB/s, one of 131071 keys 57.5 us at 4.7 (a large copy reaches 4.76, a large sum
 // 4.0). Short calls are a chain of launch, first keys, softmax and join (180 fp32
 // keys: 8.9 us, 3 of them launch to launch), a short prefix that of its stages, 1 us
