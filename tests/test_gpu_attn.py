@@ -379,6 +379,55 @@ def test_a_cache_beyond_32_bit_offsets(lq):
     c.check(got=out.cpu())
 
 
+# ---------------------------------------------------------------- blocks, orders and cuts
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("d", [32, 64, 96, 128, 256])
+@pytest.mark.parametrize("causal", [True, False])
+def test_keys_that_end_inside_a_stage(dt, d, causal):
+    # ends in the first and the second half of a stage, wavefronts without rows
+    k_lens = [1, 32, 33, 64, 65, 96, 97, 130, 161]
+    Case(dt, 2, 1, d, [70] * len(k_lens), k_lens, causal, seed=d + 1).check()
+
+
+@pytest.mark.parametrize("n", [2, 31, 32, 33])
+@pytest.mark.parametrize("dt", [DType.F16, DType.F32])
+def test_sequences_in_any_order(n, dt):
+    r = np.random.default_rng(n)
+    lens = r.integers(0, 60, n).tolist()
+    lens[0], lens[-1] = 0, 75  # an empty one, the longest last, some equal
+    Case(dt, 4, 2, 64, lens, lens, seed=n).check()
+    Case(dt, 2, 1, 128, [max(1, v // 2) for v in lens], lens, False, seed=n + 1, gap=1).check()
+
+
+def test_the_order_changes_nothing():
+    lens = [40, 7, 130, 0, 64, 130]
+    a = Case(DType.BF16, 4, 2, 64, lens, lens, seed=31)
+    want = a.run()
+    at = starts(lens)
+    for order in ([5, 4, 3, 2, 1, 0], [2, 0, 5, 1, 4, 3]):
+        b = Case(DType.BF16, 4, 2, 64, [lens[i] for i in order], [lens[i] for i in order], seed=32)
+        rows = torch.cat([torch.arange(at[i], at[i + 1]) for i in order])
+        b.q, b.k, b.v = a.q[rows], a.k[rows], a.v[rows]
+        assert torch.equal(b.run(), want[rows])
+
+
+@pytest.mark.parametrize("d", [72, 96, 128, 256])
+@pytest.mark.parametrize("lens", [[129], [300, 131, 0], [1000, 128, 257]])
+def test_fp32_keys_over_more_wavefronts_and_parts(d, lens):
+    Case(DType.F32, 4, 2, d, [1] * len(lens), lens, seed=d).check()
+    Case(DType.F32, 2, 2, d, [20] * len(lens), lens, seed=d + 1).check()
+
+
+@pytest.mark.parametrize("dt, kernel", [(DType.F16, attn.AttnKernel.ROWS), (DType.F32, attn.AttnKernel.KEYS)])
+def test_a_long_prefix_under_many_rows(dt, kernel):
+    # 16 bit: much to read for every 32 rows, so in a launch of its own
+    c = Case(dt, 8, 1, 32, [1] * 512, [5, 0, 9, 2] * 128, prefix=8200, seed=41)
+    p = c.spec().plan()
+    assert (p.kernel, p.prefix_kernel) == (attn.AttnKernel.KEYS, kernel) and p.prefix_parts > 1
+    c.check()
+
+
 # ---------------------------------------------------------------- calls
 
 @pytest.mark.parametrize("kind", ["prompt", "cut", "prefix"])
