@@ -75,6 +75,12 @@ class AttnBlock:
         self.length = 0
         self._len = torch.zeros(self.streams, dtype=torch.int32, device=self.device)
 
+    def _check_rows(self, what, x, wanted, ok):
+        """Refuse what the projection, which takes a bare address, would read as other rows or past their end."""
+        if not ok or x.dtype != self._t or x.device != self.k.device or not x.is_contiguous():
+            raise AihError(f"{what} takes a dense {wanted} {self._t} on {self.k.device}, not {tuple(x.shape)} "
+                           f"{x.dtype} on {x.device}" + ("" if x.is_contiguous() else ", not dense"))
+
     def _project(self, x, n, tokens):
         import torch
 
@@ -89,17 +95,21 @@ class AttnBlock:
                               dt=self.dt, positions=self.cos.shape[0], rows=rows)
 
     def share(self, x):
-        """x [tokens, c]: the context in front of every stream, read once for all by each step."""
+        """x [tokens, c] in the block's type, on the device: the context in front of every stream, read once for
+        all by each step; no tokens: none any more."""
         import torch
 
+        self._check_rows("share", x, f"[tokens, {self.c}]", x.dim() == 2 and x.shape[1] == self.c)
         tokens = x.shape[0]
         if tokens > self.prefix:
             raise AihError(f"{tokens} shared tokens, room for {self.prefix}")
         if self.length:
             raise AihError("share comes before the streams' tokens: their positions start behind it")
-        qkv = self._project(x, 1, tokens)
-        q = torch.empty(tokens, self.hq, self.d, dtype=self._t, device=self.device)
-        self._norm_spec(tokens, tokens).run(qkv, self.wq, self.wk, self.cos, self.sin, None, None, q, self.pk, self.pv)
+        if tokens:
+            qkv = self._project(x, 1, tokens)
+            q = torch.empty(tokens, self.hq, self.d, dtype=self._t, device=self.device)
+            self._norm_spec(tokens, tokens).run(qkv, self.wq, self.wk, self.cos, self.sin, None, None, q, self.pk,
+                                                self.pv)
         self.shared = tokens
         self._plans.clear()
 
@@ -128,10 +138,9 @@ class AttnBlock:
         [streams, tokens, c]."""
         import torch
 
-        streams, tokens, c = x.shape
-        if streams != self.streams or c != self.c or x.dtype != self._t or not x.is_contiguous():
-            raise AihError(f"step takes a dense [{self.streams}, tokens, {self.c}] {self._t}, not "
-                           f"{tuple(x.shape)} {x.dtype}")
+        self._check_rows("step", x, f"[{self.streams}, tokens, {self.c}]",
+                         x.dim() == 3 and x.shape[0] == self.streams and x.shape[2] == self.c)
+        streams, tokens, _ = x.shape
         if tokens == 0:
             return torch.empty_like(x)
         if self.length + tokens > self.capacity:

@@ -1,0 +1,60 @@
+"""CPU tests of the attention block's boundary: what is refused before anything
+runs. Nothing here launches a kernel."""
+import numpy as np
+import pytest
+import torch
+
+from ai_engine_amd.attn_block import AttnBlock
+from ai_engine_amd.conv import AihError, DType
+
+C, HQ, HKV, D = 64, 4, 2, 32
+
+
+def make_weights(**kw):
+    z = lambda *s: np.zeros(s, np.float32)
+    return {**dict(w_qkv=z((HQ + 2 * HKV) * D, C), b_qkv=z((HQ + 2 * HKV) * D), w_out=z(C, HQ * D), b_out=z(C), wq=z(D),
+                   wk=z(D)), **kw}
+
+
+def make_block(dt=DType.F32, **kw):
+    return AttnBlock(C, HQ, HKV, D, streams=2, capacity=8, weights=make_weights(), dt=dt, prefix=4, device="cpu", **kw)
+
+
+# ---------------------------------------------------------------- the rows of share and step
+
+BAD_ROWS = [
+    ("another type", lambda *s: torch.zeros(*s, C, dtype=torch.float16)),
+    ("fewer channels", lambda *s: torch.zeros(*s, C // 2)),
+    ("more channels", lambda *s: torch.zeros(*s, C + 8)),
+    ("transposed", lambda *s: torch.zeros(*s[:-1], C, s[-1]).transpose(-1, -2)),
+    ("a slice", lambda *s: torch.zeros(*s, 2 * C)[..., :C]),
+    ("one dim more", lambda *s: torch.zeros(*s, C, 1)),
+    ("one dim less", lambda *s: torch.zeros(s[-1] * C)),
+    ("another device", lambda *s: torch.zeros(*s, C, device="meta")),
+]
+
+
+@pytest.mark.parametrize("what, make", BAD_ROWS, ids=[w for w, _ in BAD_ROWS])
+def test_share_refuses_other_rows(what, make, monkeypatch):
+    block = make_block()
+    monkeypatch.setattr(block, "_project", lambda *a: pytest.fail("the projection was called"))
+    with pytest.raises(AihError, match="share takes"):
+        block.share(make(3))
+    assert block.shared == 0
+
+
+@pytest.mark.parametrize("what, make", BAD_ROWS, ids=[w for w, _ in BAD_ROWS])
+def test_step_refuses_other_rows(what, make, monkeypatch):
+    block = make_block()
+    monkeypatch.setattr(block, "_project", lambda *a: pytest.fail("the projection was called"))
+    with pytest.raises(AihError, match="step takes"):
+        block.step(make(2, 3))
+    assert block.length == 0
+
+
+def test_sharing_no_tokens_leaves_no_context(monkeypatch):
+    block = make_block()
+    monkeypatch.setattr(block, "_project", lambda *a: pytest.fail("the projection was called"))
+    block.shared = 3
+    block.share(torch.zeros(0, C))
+    assert block.shared == 0
