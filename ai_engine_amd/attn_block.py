@@ -54,11 +54,15 @@ class AttnBlock:
             return a if dt == DType.F32 else a.view(self._t)
 
         heads = hq + 2 * hkv
+        for name, n in (("w_qkv", heads * d * c), ("b_qkv", heads * d), ("w_out", c * hq * d), ("b_out", c), ("wq", d),
+                        ("wk", d)):
+            if np.prod(np.shape(weights[name])) != n:  # what packs and reads them goes by the block's sizes alone
+                raise AihError(f"{name} must hold {n} values, not {tuple(np.shape(weights[name]))}")
         self.w_qkv = put(conv.pack_weights_conv(weights["w_qkv"], heads * d, c, 1, 1, 4, dt)[0])
         self.w_out = put(conv.pack_weights_conv(weights["w_out"], c, hq * d, 1, 1, 4, dt)[0])
         self.b_qkv = put(conv.pack_bias(weights["b_qkv"], heads * d, dt))
         self.b_out = put(conv.pack_bias(weights["b_out"], c, dt))
-        self.wq, self.wk = (torch.as_tensor(weights[n]).to(device, self._t) for n in ("wq", "wk"))
+        self.wq, self.wk = (torch.as_tensor(weights[n]).to(device, self._t).contiguous() for n in ("wq", "wk"))
         self.cos, self.sin = rotation_tables(prefix + capacity, max(self.rot, 4), theta, device)
         self.k = torch.zeros(streams * capacity, hkv, d, dtype=self._t, device=device)
         self.v = torch.zeros_like(self.k)

@@ -16,8 +16,9 @@ def make_weights(**kw):
                    wk=z(D)), **kw}
 
 
-def make_block(dt=DType.F32, **kw):
-    return AttnBlock(C, HQ, HKV, D, streams=2, capacity=8, weights=make_weights(), dt=dt, prefix=4, device="cpu", **kw)
+def make_block(dt=DType.F32, weights=None, **kw):
+    return AttnBlock(C, HQ, HKV, D, streams=2, capacity=8, weights=weights or make_weights(), dt=dt, prefix=4,
+                     device="cpu", **kw)
 
 
 # ---------------------------------------------------------------- the rows of share and step
@@ -58,3 +59,21 @@ def test_sharing_no_tokens_leaves_no_context(monkeypatch):
     block.shared = 3
     block.share(torch.zeros(0, C))
     assert block.shared == 0
+
+
+# ---------------------------------------------------------------- weights
+
+@pytest.mark.parametrize("name", ["w_qkv", "b_qkv", "w_out", "b_out", "wq", "wk"])
+@pytest.mark.parametrize("more", [-1, 1])
+def test_weights_of_another_size_are_refused(name, more):
+    w = make_weights()
+    w[name] = np.zeros(w[name].size + more, np.float32)
+    with pytest.raises(AihError, match=f"{name} must hold"):
+        make_block(weights=w)
+
+
+def test_norm_weights_are_stored_dense():
+    w = make_weights(wq=torch.arange(2.0 * D)[::2], wk=torch.arange(4.0 * D)[::4])
+    block = make_block(weights=w)
+    assert block.wq.is_contiguous() and block.wk.is_contiguous()
+    assert torch.equal(block.wq, w["wq"]) and torch.equal(block.wk, w["wk"])
