@@ -9,6 +9,8 @@ the two pointwise convs of an attention block.
 As in `conv`, buffers are device tensors or raw device addresses, every call is
 asynchronous on the given stream (default: torch's current stream), and there
 is no CPU fallback.  The specs are frozen: their C descriptor is built once.
+Index arrays (starts, lengths, positions, slots) are int32 and tables fp32:
+tensors of another type or length, strided ones and ones on the host are refused.
 """
 from __future__ import annotations
 
@@ -74,6 +76,29 @@ def _u32(name, v, lo=0):
     return v
 
 
+_torch = None  # torch's Tensor, int32 and float32
+
+
+def _torch_types():
+    global _torch
+    import torch
+
+    _torch = torch.Tensor, torch.int32, torch.float32
+    return _torch
+
+
+def _arrays(**arrays):
+    """Device addresses of index and table arrays, name = (tensor, values read, type). Refuses tensors that the
+    kernels would read as other values or past their end; None and raw addresses are the caller's, as everywhere.
+    `run` asks the same in line first, at half the time: a call costs as much as its launch."""
+    for name, (t, n, dtype) in arrays.items():
+        if t is not None and not isinstance(t, int) and (
+                t.dtype is not dtype or not t.is_contiguous() or t.numel() < n or not t.is_cuda):
+            raise AihError(f"{name} must be a dense tensor of at least {n} {dtype} on the GPU, not {tuple(t.shape)} "
+                           f"{t.dtype} on {t.device}" + ("" if t.is_contiguous() else ", not dense"))
+    return [conv._ptr(t) for t, _, _ in arrays.values()]
+
+
 def _workspace_on(nbytes, device, stream):
     """Device memory of the stream it is used on: torch gives a freed block to that stream's next allocation only."""
     device = device or "cuda"  # a raw address has none
@@ -110,13 +135,27 @@ class QkNormRopeSpec:
             *(_u32(n, getattr(self, n)) for n in ("tokens", "hq", "hkv", "d", "rot")), int(bool(self.pairs)),
             self.eps, int(self.dt), _u32("positions", self.positions), _u32("rows", rows),
             *(_u32(n, getattr(self, n)) for n in ("x_stride", "q_stride", "k_stride", "v_stride"))))
+        object.__setattr__(self, "_half", self.positions * (self.rot // 2))  # values of a table
 
     def run(self, x, wq, wk, cosines, sines, pos, slots, q, k, v, stream=None):
         """x [tokens, x_stride]; wq, wk [d] or None; cosines, sines [positions, rot/2] fp32; pos, slots int32
         [tokens] or None; q [tokens, hq, d]; k, v [rows, hkv, d] (v None: the values stay in x)."""
-        p = conv._ptr
-        if (_lib or lib()).aih_qk_norm_rope(C.byref(self._desc), p(x), p(wq), p(wk), p(cosines), p(sines), p(pos), p(slots),
-                                            p(q), p(k), p(v), conv._stream(stream)):
+        T, i32, f32 = _torch or _torch_types()
+        p, n, half = conv._ptr, self.tokens, self._half
+        if (pos.__class__ is T and pos.dtype is i32 and pos.is_cuda and pos.is_contiguous() and pos.numel() >= n
+                and (slots is None or slots.__class__ is T and slots.dtype is i32 and slots.is_cuda
+                     and slots.is_contiguous() and slots.numel() >= n)
+                and cosines.__class__ is T and cosines.dtype is f32 and cosines.is_cuda and cosines.is_contiguous()
+                and cosines.numel() >= half and sines.__class__ is T and sines.dtype is f32 and sines.is_cuda
+                and sines.is_contiguous() and sines.numel() >= half):
+            arrays = cosines.data_ptr(), sines.data_ptr(), pos.data_ptr(), p(slots)
+        else:
+            arrays = _arrays(cosines=(cosines, half, f32), sines=(sines, half, f32), pos=(pos, n, i32),
+                             slots=(slots, n, i32))
+        if (_lib or lib()).aih_qk_norm_rope(
+                C.byref(self._desc), x.data_ptr() if x.__class__ is T else p(x), p(wq), p(wk), *arrays,
+                q.data_ptr() if q.__class__ is T else p(q), k.data_ptr() if k.__class__ is T else p(k),
+                v.data_ptr() if v.__class__ is T else p(v), conv._stream(stream)):
             raise AihError(conv.last_error())
         return q, k, v
 
@@ -167,6 +206,15 @@ class AttnSpec:
     def run(self, q, k, v, q_start, k_start, k_len, out, prefix_k=None, prefix_v=None, ws=None, stream=None):
         """q, out [tokens, hq, d]; k, v [rows, hkv, d]; q_start [nseq + 1], k_start, k_len [nseq] int32;
         prefix_k, prefix_v [prefix, hkv, d]; ws: workspace_bytes() of device memory, made here if None."""
+        T, i32, _ = _torch or _torch_types()
+        b = self.nseq
+        if (q_start.__class__ is T and q_start.dtype is i32 and q_start.is_cuda and q_start.is_contiguous()
+                and q_start.numel() > b and k_start.__class__ is T and k_start.dtype is i32 and k_start.is_cuda
+                and k_start.is_contiguous() and k_start.numel() >= b and k_len.__class__ is T and k_len.dtype is i32
+                and k_len.is_cuda and k_len.is_contiguous() and k_len.numel() >= b):
+            arrays = q_start.data_ptr(), k_start.data_ptr(), k_len.data_ptr()
+        else:
+            arrays = _arrays(q_start=(q_start, b + 1, i32), k_start=(k_start, b, i32), k_len=(k_len, b, i32))
         n = self._ws if self._ws is not None else self.workspace_bytes()
         if n:
             if ws is None:
@@ -174,7 +222,10 @@ class AttnSpec:
             if not isinstance(ws, int) and ws.numel() * ws.element_size() < n:
                 raise AihError(f"the workspace needs {n} bytes, not {ws.numel() * ws.element_size()}")
         p = conv._ptr
-        if (_lib or lib()).aih_attn(C.byref(self._desc), p(q), p(k), p(v), p(q_start), p(k_start), p(k_len), p(prefix_k),
-                                    p(prefix_v), p(out), p(ws) if n else None, n, conv._stream(stream)):
+        if (_lib or lib()).aih_attn(
+                C.byref(self._desc), q.data_ptr() if q.__class__ is T else p(q),
+                k.data_ptr() if k.__class__ is T else p(k), v.data_ptr() if v.__class__ is T else p(v), *arrays,
+                p(prefix_k), p(prefix_v), out.data_ptr() if out.__class__ is T else p(out), p(ws) if n else None, n,
+                conv._stream(stream)):
             raise AihError(conv.last_error())
         return out
