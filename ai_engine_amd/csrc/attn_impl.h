@@ -149,25 +149,43 @@ __device__ __forceinline__ void at_dma(const char *base, uint32_t stride, uint32
   const uint32_t lr = lane / T::PU, ls = lane % T::PU;
   const uint32_t lu = ls ^ (V ? at_vswz<T>(lr) : at_kswz<T>(lr));
   const uint32_t to = (uint32_t)(uintptr_t)(at_lds_void *)dst;
+  constexpr int G = NI < 4 ? NI : 4;  // copies written out together
+  static_assert(NI % G == 0, "DMA instructions");
 #pragma unroll
-  for (int k = 0; k < NI; ++k) {
-    const uint32_t i = i0 + k;
-    // rows i RPI and lr share no bit, so the XORs add up
-    const uint32_t u = lu ^ (T::PU < 8 ? 0 : V ? at_vswz<T>(i * T::RPI) : at_kswz<T>(i * T::RPI));
-    const uint32_t off = u < du ? u * 16 + (i * T::RPI + lr) * stride : kAtOob;
-    const uint32_t m0 = __builtin_amdgcn_readfirstlane(to + i * 1024);
-    // one wait state after m0; five after a vector instruction that may have
-    // written the descriptor
-    if (k == 0)
-      __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+  for (int k = 0; k < NI; k += G) {
+    uint32_t off[G];
+#pragma unroll
+    for (int e = 0; e < G; ++e) {
+      const uint32_t i = i0 + k + e;
+      // rows i RPI and lr share no bit, so the XORs add up
+      const uint32_t u = lu ^ (T::PU < 8 ? 0 : V ? at_vswz<T>(i * T::RPI) : at_kswz<T>(i * T::RPI));
+      off[e] = u < du ? u * 16 + (i * T::RPI + lr) * stride : kAtOob;
+    }
+    const uint32_t m0 = __builtin_amdgcn_readfirstlane(to + (i0 + k) * 1024);
+    // One wait state after m0; five after a vector instruction that may have
+    // written the descriptor, which any piece of text has to hold for itself:
+    // scalar registers that the compiler spills come back through v_readlane, and
+    // it does not know what the text reads.
+#define AIH_AT_COPY(OFF) "buffer_load_dwordx4 " OFF ", %1, 0 offen lds\n\t"
+#define AIH_AT_NEXT(AT) "s_add_u32 m0, %0, " AT "\n\ts_nop 0\n\t"
+    if constexpr (G == 1)
+      __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\t" AIH_AT_COPY("%2")
                        :
-                       : "s"(m0), "v"(off), "s"(rs)
+                       : "s"(m0), "s"(rs), "v"(off[0])
                        : "memory", "m0");
+    else if constexpr (G == 2)
+      __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\t" AIH_AT_COPY("%2") AIH_AT_NEXT("0x400") AIH_AT_COPY("%3")
+                       :
+                       : "s"(m0), "s"(rs), "v"(off[0]), "v"(off[1])
+                       : "memory", "m0", "scc");
     else
-      __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+      __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\t" AIH_AT_COPY("%2") AIH_AT_NEXT("0x400") AIH_AT_COPY("%3")
+                           AIH_AT_NEXT("0x800") AIH_AT_COPY("%4") AIH_AT_NEXT("0xc00") AIH_AT_COPY("%5")
                        :
-                       : "s"(m0), "v"(off), "s"(rs)
-                       : "memory", "m0");
+                       : "s"(m0), "s"(rs), "v"(off[0]), "v"(off[1]), "v"(off[G > 2 ? 2 : 0]), "v"(off[G > 2 ? 3 : 0])
+                       : "memory", "m0", "scc");
+#undef AIH_AT_COPY
+#undef AIH_AT_NEXT
   }
 }
 
