@@ -34,7 +34,11 @@ def rotation_tables(positions: int, rot: int, theta: float = 10000.0, device="cu
 class AttnBlock:
     """weights: w_qkv [(hq + 2 hkv) d, c], b_qkv, w_out [c, hq d], b_out, and the norms' wq, wk [d] (fp32
     arrays); capacity: cache rows of a stream; causal: a token sees the tokens up to its own (else the
-    whole step's); prefix: rows kept for `share`."""
+    whole step's); prefix: rows kept for `share`. Steps follow one another: on one stream, or with a wait in between.
+
+    Besides the cache a block holds the buffers of its longest step: queries, results and the attention's workspace,
+    (d + 2) fp32 values a token and query head for every part of the keys. That is large for whole prompts behind a
+    shared context, whose keys are always in two parts or more (16 x 1024 tokens, 32 heads of 128: 545 MB)."""
 
     def __init__(self, c, hq, hkv, d, streams, capacity, weights, dt=DType.F32, rot=None, causal=True, prefix=0,
                  eps=1e-6, theta=10000.0, device="cuda:0"):
@@ -69,6 +73,9 @@ class AttnBlock:
         self.pk = torch.zeros(max(prefix, 1), hkv, d, dtype=self._t, device=device)
         self.pv = torch.zeros_like(self.pk)
         self._first = torch.arange(streams, dtype=torch.int32, device=device) * capacity
+        self._at = torch.arange(capacity, dtype=torch.int32, device=device)
+        self._rows = torch.empty(2, 0, hq, d, dtype=self._t, device=device)  # queries and results of a step
+        self._ws = torch.empty(0, dtype=torch.float32, device=device)
         self._plans = {}
         self.reset()
 
@@ -117,8 +124,17 @@ class AttnBlock:
         self.shared = tokens
         self._plans.clear()
 
+    def _outgrown(self, buffer):
+        """`buffer` is let go: by the plans, and only after the last step on the current stream."""
+        import torch
+
+        self._plans.clear()
+        if buffer.is_cuda and buffer.numel():
+            buffer.record_stream(torch.cuda.current_stream(buffer.device))
+
     def _plan(self, tokens):
-        """The specs and buffers of a step of `tokens` tokens a stream, made once."""
+        """The specs of a step of `tokens` tokens a stream, made once, and its part of the buffers, which all lengths
+        share: the steps of a block follow one another on a stream."""
         import torch
 
         p = self._plans.get(tokens)
@@ -126,15 +142,19 @@ class AttnBlock:
             n = self.streams * tokens
             spec = AttnSpec(nseq=self.streams, tokens=n, rows=self.streams * self.capacity, hq=self.hq, hkv=self.hkv,
                             d=self.d, causal=self.causal, dt=self.dt, max_len=self.capacity, prefix=self.shared)
-            new = lambda: torch.empty(n, self.hq, self.d, dtype=self._t, device=self.device)
             ws = spec.workspace_bytes()
+            if n > self._rows.shape[1]:
+                self._outgrown(self._rows)
+                self._rows = torch.empty(2, n, self.hq, self.d, dtype=self._t, device=self.device)
+            if ws // 4 > self._ws.shape[0]:
+                self._outgrown(self._ws)
+                self._ws = torch.empty(ws // 4, dtype=torch.float32, device=self.device)
             p = self._plans[tokens] = dict(
-                norm=self._norm_spec(n, self.streams * self.capacity), attn=spec, q=new(), o=new(),
+                norm=self._norm_spec(n, self.streams * self.capacity), attn=spec,
+                q=self._rows[0, :n], o=self._rows[1, :n], ws=self._ws if ws else None, at=self._at[:tokens],
                 out=ConvOp(ih=tokens, iw=1, cin=self.hq * self.d, cout=self.c, residual=True, dt=self.dt,
                            n=self.streams),
-                ws=torch.empty(ws // 4, dtype=torch.float32, device=self.device) if ws else None,
-                q_start=torch.arange(0, n + 1, tokens, dtype=torch.int32, device=self.device),
-                at=torch.arange(tokens, dtype=torch.int32, device=self.device))
+                q_start=torch.arange(0, n + 1, tokens, dtype=torch.int32, device=self.device))
         return p
 
     def step(self, x):

@@ -103,7 +103,9 @@ typedef struct {
   int32_t prefix_kernel; /* the same for the prefix, 0 = no prefix */
   uint32_t prefix_bm, prefix_parts, prefix_chunk;
   uint32_t grid;         /* workgroups of the first launch */
-  size_t ws_bytes;       /* workspace; 0 when no row's keys are cut */
+  size_t ws_bytes;       /* workspace: (d + 2) fp32 values for each of tokens * hq rows and
+                            each part, the prefix's and the own keys' together; 0 when no
+                            row's keys are cut. A prefix always leaves two parts or more */
 } aih_attn_plan_info;
 
 int aih_attn_plan(const aih_attn_desc *d, aih_attn_plan_info *out);

@@ -77,3 +77,30 @@ def test_norm_weights_are_stored_dense():
     block = make_block(weights=w)
     assert block.wq.is_contiguous() and block.wk.is_contiguous()
     assert torch.equal(block.wq, w["wq"]) and torch.equal(block.wk, w["wk"])
+
+
+# ---------------------------------------------------------------- what a block keeps
+
+def held(block):
+    """Bytes of the distinct buffers that a block's steps keep."""
+    tensors = [t for p in block._plans.values() for t in p.values() if isinstance(t, torch.Tensor)]
+    tensors += [t for t in vars(block).values() if isinstance(t, torch.Tensor)]
+    return sum({t.untyped_storage().data_ptr(): t.untyped_storage().nbytes() for t in tensors}.values())
+
+
+@pytest.mark.parametrize("shared", [0, 40])
+def test_steps_of_many_lengths_hold_one_set_of_buffers(shared):
+    make = lambda: AttnBlock(C, HQ, HKV, D, streams=16, capacity=200, weights=make_weights(), prefix=40, device="cpu")
+    one, many = make(), make()
+    one.shared = many.shared = shared
+    one._plan(200)
+    for tokens in [*range(1, 201, 7), 200, *range(200, 0, -7)]:
+        p = many._plan(tokens)
+        assert p["q"].shape == p["o"].shape == (16 * tokens, HQ, D) and p["at"].shape == (tokens,)
+        assert p["q"].data_ptr() != p["o"].data_ptr() and p["q"].is_contiguous() and p["o"].is_contiguous()
+        need = p["attn"].workspace_bytes()
+        assert (p["ws"] is None) == (need == 0) and (need == 0 or 4 * p["ws"].numel() >= need)
+    # the rest is a starts array of each length
+    assert held(many) <= held(one) + 80 * 4 * 17
+    # no length keeps buffers that have been outgrown
+    assert len({p["q"].untyped_storage().data_ptr() for p in many._plans.values()}) == 1
