@@ -240,7 +240,8 @@ extern "C" int aih_attn_plan(const aih_attn_desc *d, aih_attn_plan_info *out) {
     out->chunk = p.own.parts > 1 ? 1u << p.own.shift : 0;
     out->prefix_kernel = p.pre.kernel, out->prefix_bm = p.pre.bm, out->prefix_parts = p.pre.parts;
     out->prefix_chunk = p.pre.parts > 1 ? 1u << p.pre.shift : 0;
-    out->grid = p.own.tiles * d->hkv * p.own.parts;
+    const uint32_t own = p.own.tiles * d->hkv * p.own.parts, pre = p.pre.tiles * d->hkv * p.pre.parts;
+    out->grid = p.pre.parts && !p.together ? pre : own + pre;
     out->ws_bytes = p.ws_floats * 4;
     return AIH_OK;
   });

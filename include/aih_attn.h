@@ -102,7 +102,9 @@ typedef struct {
   uint32_t chunk;        /* keys of a part, unless more parts would be needed */
   int32_t prefix_kernel; /* the same for the prefix, 0 = no prefix */
   uint32_t prefix_bm, prefix_parts, prefix_chunk;
-  uint32_t grid;         /* workgroups of the first launch */
+  uint32_t grid;         /* workgroups of the first launch, which a prefix leads or has to
+                            itself; at most: where keys are cut, no more than run at once
+                            are launched and share the work */
   size_t ws_bytes;       /* workspace: (d + 2) fp32 values for each of tokens * hq rows and
                             each part, the prefix's and the own keys' together; 0 when no
                             row's keys are cut. A prefix always leaves two parts or more */
