@@ -1,4 +1,4 @@
-"""CPU tests of the attention plan's figures.
+"""CPU tests of the attention plan's figures and of where its routes change.
 Nothing here launches a kernel; the plans are those of 256 CUs."""
 import pytest
 
@@ -36,3 +36,48 @@ def test_grid_with_a_prefix_of_its_own_launch():
 
 def test_nothing_to_do_has_no_grid():
     assert plan(nseq=0).grid == 0 and plan(tokens=0, prefix=9).grid == 0
+
+
+# ---------------------------------------------------------------- where routes change: the side that measured faster
+
+H = dict(f32=DType.F32, f16=DType.F16, bf16=DType.BF16)
+
+
+@pytest.mark.parametrize("dt, nseq, keys, hq, hkv, d, parts", [
+    ("f16", 1, 512, 32, 8, 128, 1), ("f16", 1, 1024, 32, 8, 128, None), ("bf16", 1, 4096, 32, 8, 128, None),
+    ("f16", 16, 1024, 32, 8, 128, 1), ("f16", 16, 2048, 32, 8, 128, 2), ("f16", 4, 600, 16, 4, 256, None),
+    ("f16", 16, 600, 16, 4, 256, 1), ("f32", 1, 384, 8, 2, 64, 1), ("f32", 1, 512, 8, 2, 64, None),
+    ("f32", 1, 271, 16, 4, 256, None), ("f32", 40, 600, 4, 4, 32, 1), ("f32", 8, 2000, 18, 3, 256, 8),
+    ("f32", 16, 2000, 32, 8, 64, 4)])
+def test_single_tokens_are_cut_where_it_pays(dt, nseq, keys, hq, hkv, d, parts):
+    p = plan(nseq=nseq, tokens=nseq, rows=nseq * keys, max_len=keys, hq=hq, hkv=hkv, d=d, dt=H[dt])
+    assert p.kernel == KEYS
+    assert p.parts == parts if parts else p.parts > 1
+
+
+@pytest.mark.parametrize("dt, nseq, n, hq, hkv, d, kernel, cut", [
+    ("f16", 1, 1500, 4, 4, 64, KEYS, False), ("f32", 1, 1024, 4, 4, 64, KEYS, True),
+    ("f32", 1, 300, 16, 4, 256, KEYS, False), ("f32", 1, 4096, 16, 4, 96, KEYS, False),
+    ("f32", 4, 2048, 16, 4, 96, KEYS, False), ("f32", 16, 720, 16, 4, 96, ROWS, False),
+    ("f16", 1, 2880, 8, 2, 64, KEYS, False), ("f16", 1, 2880, 16, 4, 128, ROWS, False),
+    ("f16", 40, 100, 8, 2, 128, ROWS, False), ("f32", 4, 100, 16, 4, 128, KEYS, False),
+    ("f32", 40, 64, 16, 4, 128, ROWS, False), ("f32", 8, 260, 16, 4, 128, KEYS, False),
+    ("f32", 20, 300, 16, 4, 128, ROWS, False), ("f32", 3, 700, 16, 4, 128, KEYS, False),
+    ("bf16", 1, 520, 8, 4, 256, KEYS, False), ("bf16", 2, 900, 8, 4, 256, KEYS, False),
+    ("bf16", 8, 260, 8, 4, 256, ROWS, False), ("bf16", 6, 520, 8, 4, 256, ROWS, False),
+    ("bf16", 1, 3000, 8, 4, 256, ROWS, False)])
+def test_prompts_take_the_faster_kernel(dt, nseq, n, hq, hkv, d, kernel, cut):
+    p = plan(nseq=nseq, tokens=nseq * n, rows=nseq * n, max_len=n, hq=hq, hkv=hkv, d=d, dt=H[dt])
+    assert p.kernel == kernel and (p.parts > 1) == cut
+
+
+@pytest.mark.parametrize("dt, nseq, lq, prefix, hq, hkv, d, kernel, parts", [
+    ("bf16", 64, 1, 4096, 32, 8, 128, KEYS, 4), ("bf16", 64, 4, 4096, 12, 2, 128, KEYS, None),
+    ("bf16", 64, 4, 8000, 12, 2, 128, KEYS, None), ("bf16", 64, 4, 8000, 8, 2, 64, KEYS, None),
+    ("bf16", 64, 4, 24000, 8, 2, 64, ROWS, None), ("bf16", 64, 1, 24000, 32, 8, 128, ROWS, None),
+    ("bf16", 16, 4, 24000, 16, 4, 256, ROWS, None), ("bf16", 16, 4, 60000, 16, 4, 256, ROWS, None),
+    ("f32", 5, 1, 651, 16, 4, 256, KEYS, 6), ("f32", 64, 4, 24000, 32, 8, 64, KEYS, None)])
+def test_a_prefix_takes_the_faster_kernel(dt, nseq, lq, prefix, hq, hkv, d, kernel, parts):
+    p = plan(nseq=nseq, tokens=nseq * lq, rows=nseq * 134, max_len=134, hq=hq, hkv=hkv, d=d, dt=H[dt], prefix=prefix)
+    assert p.kernel == KEYS and p.prefix_kernel == kernel
+    assert p.prefix_parts == parts if parts else True
