@@ -124,21 +124,34 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(QkRopeArgs a, ui
 
   float f0[VW], f1[VW];
   v0.get(f0), v1.get(f1);
-  float ss = 0.0f;
+  auto squares = [&]() {  // of the whole head
+    float ss = 0.0f;
 #pragma unroll
-  for (int i = 0; i < VW; ++i) ss += f0[i] * f0[i] + f1[i] * f1[i];
-  if (pshift == kAnyLanes) {  // to the group's first lane, and from there to all
-    for (uint32_t m = 1; m < a.nl; m <<= 1) {
-      const float up = __shfl(ss, lane + m);
-      if (j % (2 * m) == 0 && j + m < a.nl) ss += up;
+    for (int i = 0; i < VW; ++i) ss += f0[i] * f0[i] + f1[i] * f1[i];
+    if (pshift == kAnyLanes) {  // to the group's first lane, and from there to all
+      for (uint32_t m = 1; m < a.nl; m <<= 1) {
+        const float up = __shfl(ss, lane + m);
+        if (j % (2 * m) == 0 && j + m < a.nl) ss += up;
+      }
+      return __shfl(ss, lane - j);
     }
-    ss = __shfl(ss, lane - j);
-  } else {
     for (uint32_t m = 1; m < (1u << pshift); m <<= 1) ss += __shfl_xor(ss, m);
+    return ss;
+  };
+  float mean = squares() * a.inv_d + a.eps;
+  // Squares leave fp32's range, and the root's that of normal numbers, long before
+  // the values do: such heads (below 1e-15 or above 1e15 or so) are taken times a
+  // power of two, which rounds nothing.
+  const bool out = !is_v && !(mean >= 0x1p-100f && mean <= 0x1p100f);
+  if (__any(out)) {
+    const float up = !out ? 1.0f : mean < 0x1p-100f ? 0x1p100f : 0x1p-70f;
+#pragma unroll
+    for (int i = 0; i < VW; ++i) f0[i] *= up, f1[i] *= up;
+    mean = squares() * a.inv_d + a.eps * up * up;
   }
 
   if (!is_v) {  // a value head keeps the bits it was loaded with
-    const float r = __builtin_amdgcn_rsqf(ss * a.inv_d + a.eps);
+    const float r = __builtin_amdgcn_rsqf(mean);
     const char *w = (const char *)(is_q ? a.wq : a.wk);
 #pragma unroll
     for (int i = 0; i < VW; ++i) f0[i] *= r, f1[i] *= r;

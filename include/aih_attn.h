@@ -48,7 +48,7 @@ typedef struct {
   uint32_t d;         /* elements of a head: a multiple of 8, at most 256 */
   uint32_t rot;       /* rotated dims: a multiple of 4, at most d; 0 = none */
   int32_t pairs;      /* 1 = adjacent pairs, 0 = halves */
-  float eps;          /* >= 0, finite */
+  float eps;          /* >= 0, finite; with 0 a head of zeros has no norm (NaN) */
   int32_t dt;         /* enum aih_dtype: x, wq, wk, q, k, v */
   uint32_t positions; /* rows of the tables (used when rot > 0) */
   uint32_t rows;      /* rows of k and v */
