@@ -43,6 +43,12 @@ constexpr float kAtLowest = -3.402823466e38f;
 // alone: what others in the wavefront hold does not change its rounding.
 constexpr float kAtSlack = 8.0f;
 constexpr float kAtMost = 32768.0f;
+// The exponent's argument is one fma: the exact product of score and scale less the
+// maximum, which is rounded. The two are up to half a unit of the maximum's last
+// place apart, a common factor of a row's probabilities while its maximum stays, but
+// from 2^24 on it counts, later it leaves the range. Rows whose maximum is that far
+// out take the product rounded as well (at_far), which fp32 scores are precise to.
+constexpr float kAtFar = 16777216.0f;
 // f16 probabilities are held 2^7 times larger (below 2^15): those of 2^-22 and
 // more keep all their bits, where without it they would be subnormal from 2^-15
 // on. The sum carries the same factor. fp32 and bf16 have the range.
@@ -228,13 +234,12 @@ __device__ __forceinline__ void at_mask(f32x16 &sc, uint32_t to, int lane) {
     if (8 * (r / 4) + r % 4 >= mine) sc[r] = -__builtin_huge_valf();
 }
 
-// Scores -> probabilities 2^(scale s - m + bias) with the running maximum m (in
-// the exponent's units); returns `sum` plus this lane's. Words w0 .. w1 - 1, two
+// Scores -> probabilities 2^(scale s + off), off the bias less the running maximum
+// (in the exponent's units); returns `sum` plus this lane's. Words w0 .. w1 - 1, two
 // keys each.
 template <class T>
-__device__ __forceinline__ float at_probs(const f32x16 &sc, typename T::Probs &p, float m, float scale, int w0 = 0,
+__device__ __forceinline__ float at_probs(const f32x16 &sc, typename T::Probs &p, float off, float scale, int w0 = 0,
                                           int w1 = 8, float sum = 0.0f) {
-  const float off = kAtBias<T::DT> - m;
 #pragma unroll
   for (int w = w0; w < w1; ++w) {
     const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * w], scale, off));
@@ -249,6 +254,26 @@ __device__ __forceinline__ float at_probs(const f32x16 &sc, typename T::Probs &p
     }
   }
   return sum;
+}
+// at_probs' `off` for the maximum m. The scores of rows that are far out become
+// differences to the maximum, whose off is the bias alone.
+template <class T, int N>
+__device__ __forceinline__ float at_far(f32x16 (&sc)[N], float m, float scale) {
+#pragma clang fp contract(off)
+  const bool far = __builtin_fabsf(m) >= kAtFar;
+  float off = kAtBias<T::DT> - m;
+  if (__builtin_expect(__any(far), 0)) {
+    off = far ? kAtBias<T::DT> : off;
+    const float inv = __builtin_amdgcn_rcpf(scale);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float at = sc[i][r] * scale;
+        sc[i][r] = far ? (at - m) * inv : sc[i][r];
+      }
+  }
+  return off;
 }
 // The rows' maximum over N blocks, in the exponent's units.
 template <class T, int N>
@@ -272,31 +297,37 @@ __device__ __forceinline__ void at_raise(float mx, bool row, float &m, float &l,
     for (int r = 0; r < 16; ++r) o[db][r] *= al;
 }
 // `sum` is at_probs' of N blocks: the rows that it is too large for get their
-// maximum found and their probabilities again.
+// maximum found and their probabilities again, and those far out always do.
 template <class T, int N>
-__device__ __forceinline__ void at_settle(const f32x16 (&sc)[N], typename T::Probs (&p)[N], float sum, float &m,
-                                          float &l, f32x16 (&o)[T::DB], float scale) {
-  const bool big = !(sum < kAtMost);
+__device__ __forceinline__ void at_settle(f32x16 (&sc)[N], typename T::Probs (&p)[N], float sum, float &m, float &l,
+                                          f32x16 (&o)[T::DB], float scale) {
+  const bool big = !(sum < kAtMost) || __builtin_fabsf(m) >= kAtFar;
   if (__any(big)) {
     at_raise<T>(at_top<T>(sc, scale), at_pair_max(big ? 1.0f : 0.0f) != 0.0f, m, l, o);
+    const float off = at_far<T>(sc, m, scale);
     sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) sum = at_probs<T>(sc[i], p[i], m, scale, 0, 8, sum);
+    for (int i = 0; i < N; ++i) sum = at_probs<T>(sc[i], p[i], off, scale, 0, 8, sum);
   }
   l += sum;
 }
-// The softmax of N blocks: p, the maximum m and this lane's share of the sum l.
+// The softmax of N blocks: p, the maximum m and this lane's share of the sum l. The
+// scores are used up.
 template <class T, int N>
-__device__ __forceinline__ void at_softmax(const f32x16 (&sc)[N], typename T::Probs (&p)[N], float &m, float &l,
+__device__ __forceinline__ void at_softmax(f32x16 (&sc)[N], typename T::Probs (&p)[N], float &m, float &l,
                                            f32x16 (&o)[T::DB], float scale) {
+  float off = kAtBias<T::DT> - m;
   if constexpr (!T::LAZY) {
     const float mx = at_top<T>(sc, scale);
     const bool row = mx > m + kAtSlack;
-    if (__any(row)) at_raise<T>(mx, row, m, l, o);
+    if (__any(row || __builtin_fabsf(m) >= kAtFar)) {
+      at_raise<T>(mx, row, m, l, o);
+      off = at_far<T>(sc, m, scale);
+    }
   }
   float sum = 0.0f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) sum = at_probs<T>(sc[i], p[i], m, scale, 0, 8, sum);
+  for (int i = 0; i < N; ++i) sum = at_probs<T>(sc[i], p[i], off, scale, 0, 8, sum);
   if constexpr (T::LAZY) at_settle<T>(sc, p, sum, m, l, o, scale);
   else l += sum;
 }
@@ -361,6 +392,7 @@ __device__ __forceinline__ void at_step(const char *kt, const char *vt, Q q, f32
   };
   f32x16 next{};
   typename T::Probs pn[1];
+  const float off = kAtBias<T::DT> - m;
   float sum = 0.0f;
 #pragma unroll
   for (int i = 0; i < FIRST; ++i) load(i);
@@ -368,7 +400,7 @@ __device__ __forceinline__ void at_step(const char *kt, const char *vt, Q q, f32
   for (int i = 0; i < N; ++i) {
     __builtin_amdgcn_sched_barrier(0);
     if (i + FIRST < N) load(i + FIRST);
-    sum = at_probs<T>(sc[0], pn[0], m, scale, 8 * i / N, 8 * (i + 1) / N, sum);
+    sum = at_probs<T>(sc[0], pn[0], off, scale, 8 * i / N, 8 * (i + 1) / N, sum);
     next = at_mfma<T>(kk[i], q(i), next);
     o[i % T::DB] = at_mfma<T>(vv[i], p[0].h[i / T::DB], o[i % T::DB]);
   }
