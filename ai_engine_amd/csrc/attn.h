@@ -57,7 +57,7 @@ __host__ __device__ inline uint64_t attn_ws_ml(const AttnArgs &a) {
 }
 
 // Rows of a tile (enum aih_attn_kernel).
-uint32_t attn_bm(int kernel, int dt, uint32_t d);
+uint32_t attn_bm(int kernel);
 
 hipError_t launch_attn(const AttnArgs &a, int kernel, int dt, hipStream_t st);
 hipError_t launch_attn_f32(const AttnArgs &a, int kernel, hipStream_t st);

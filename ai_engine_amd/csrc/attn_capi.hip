@@ -87,7 +87,7 @@ Cover cover(int32_t kernel, uint32_t nseq, uint64_t rows, uint32_t len, uint32_t
   const uint32_t cus = device_cus();
   Cover c{};
   c.kernel = kernel;
-  c.bm = attn_bm(c.kernel, dt, d);
+  c.bm = attn_bm(c.kernel);
   c.tiles = nseq == 1 ? div_up(rows, c.bm) : (uint32_t)(rows / c.bm) + nseq;
   const uint64_t base = (uint64_t)c.tiles * hkv;
   auto parts = [&](uint32_t x) { return std::max(1u, div_up(len, 1ull << x)); };
@@ -160,7 +160,7 @@ int check_attn(const aih_attn_desc *d, AttnArgs *a, AttnPlan *p) {
   // (268) 105 | 80. Above 128 16-bit elements a wavefront's chain is written out: 8/4
   // heads of 256, 520 tokens (36) 26 | 15, 2 x 900 (120) 38 | 30, 8 x 260 (148) 20 | 28,
   // 6 x 520 (208) 28 | 42, 3000 (188) 100 | 92, not causal 105 | 149.
-  const uint64_t tiles = (uint64_t)d->hkv * (div_up(rows, attn_bm(AIH_ATTN_ROWS, d->dt, d->d)) + d->nseq / 2);
+  const uint64_t tiles = (uint64_t)d->hkv * (div_up(rows, attn_bm(AIH_ATTN_ROWS)) + d->nseq / 2);
   const uint64_t cus = device_cus();
   const bool chain = d->dt == AIH_F32 ? tiles < 5 * cus && (d->d <= 64 || 180 * tiles < cus * len)
                                       : tiles < (d->d > 128 ? cus / 2 : cus) && len >= 256;

@@ -117,7 +117,7 @@ hipError_t launch_attn_join(const AttnArgs &a, int dt, hipStream_t st) {
                       : dt == DT_F16 ? join_dt<DT_F16>(a, ldim, st) : join_dt<DT_BF16>(a, ldim, st);
 }
 
-uint32_t attn_bm(int kernel, int, uint32_t) { return kernel == AIH_ATTN_ROWS ? 128 : 32; }
+uint32_t attn_bm(int kernel) { return kernel == AIH_ATTN_ROWS ? 128 : 32; }
 
 hipError_t launch_attn(const AttnArgs &a, int kernel, int dt, hipStream_t st) {
   return dt == DT_F32 ? launch_attn_f32(a, kernel, st)
