@@ -4,14 +4,14 @@
 //
 // A single token's g rows fill g of a tile's 32 columns; the products are cheap
 // beside the keys and values that are read once for them, so that serving is bound
-// by memory: 64 sequences of up to 8192 keys, 32/8 bf16 heads of 128, 79 us at 4.5
-// TB/s, one of 131071 keys 57.5 us at 4.7 (a large copy reaches 4.76, a large sum
+// by memory: 64 sequences of up to 8192 keys, 32/8 bf16 heads of 128, 82 us at 4.3
+// TB/s, one of 131071 keys 58 us at 4.6 (a large copy reaches 4.76, a large sum
 // 4.0). Short calls are a chain of launch, first keys, softmax and join (180 fp32
-// keys: 8.9 us, 3 of them launch to launch), a short prefix that of its stages, 64 KB
+// keys: 8.8 us, 3 of them launch to launch), a short prefix that of its stages, 64 KB
 // that a CU takes 1 us to bring from L2 into LDS, by one workgroup or two (64 tokens
-// behind 4096 keys, 32/8 heads of 128: 23 us). fp32 prompts run at 82
+// behind 4096 keys, 32/8 heads of 128: 22.4 us). fp32 prompts run at 80
 // TFLOP/s where a matrix product reaches 154 (7 of 181 to 1441 tokens, 8/4 heads of
-// 96: 114 us; matrix instructions 64 % of the time).
+// 96: 117 us; matrix instructions 62 % of the time).
 #pragma once
 
 #include "attn_impl.h"

@@ -7,7 +7,7 @@
 // instructions (16384 tokens causal, 32/8 heads of 128: 2.0 ms, 1.09 PFLOP/s, where
 // a large matrix product reaches 1.12; the clock is down to 1.8 GHz for the power);
 // heads of 64 those and the exponentials together (64 x 720 tokens, 8/2 heads: 93
-// us, 730 TFLOP/s; vector instructions 65 %, matrix instructions 40 % of the time,
+// us, 730 TFLOP/s; vector instructions 66 %, matrix instructions 40 % of the time,
 // and hardly any of it at once: taking half of either out saves what they cost).
 // fp32 is the matrix instructions (16 x 720 causal, 16/4 heads of 128: 375 us).
 #pragma once

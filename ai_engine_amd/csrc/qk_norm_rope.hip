@@ -16,8 +16,8 @@
 // Bound by memory: each element is read and written once, the table rows come
 // from the caches (all heads of a token use the same one). 46080 tokens of 8 + 2 + 2
 // f16 heads of 64 take 33.1 us, 4.6 TB/s, where a large copy reaches 4.76. Few
-// tokens (8: 3.3 us on the device, 4.8 from launch to launch) are bound by the
-// launch.
+// tokens (8: 3.3 us on the device, 5.7 from call to call) are bound by the
+// host's call.
 #include <hip/hip_runtime.h>
 
 #include "aih_device.h"

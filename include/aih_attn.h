@@ -16,12 +16,15 @@
  * thread's message in aih_last_error(), no exception across the boundary,
  * caller-owned device buffers, asynchronous on the caller's stream, nothing
  * allocated by a call, safe to call on several streams at once (each with a
- * workspace of its own). Statistics and sums are fp32 in every storage type.
+ * workspace of its own). Statistics, sums and partial results are fp32 in every
+ * storage type; probabilities are rounded to it for their product with the
+ * values, and their sum is of the rounded ones.
  *
  * A row of a tensor holds its heads one after another, d elements each; rows
  * are `stride` elements apart (0 = dense), so keys and values may stay inside
  * the projection's rows (a pointer to their first head and the row's stride).
- * Tensors are aligned to 16 bytes and row strides are whole 16-byte units.
+ * Tensors are aligned to 16 bytes and row strides are whole 16-byte units of at
+ * most 2^22 elements.
  */
 #ifndef AIH_ATTN_H
 #define AIH_ATTN_H
