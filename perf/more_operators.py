@@ -223,6 +223,11 @@ def _padded(k):
     return -(-k // 128) * 128
 
 
+def _scale_bytes(k):
+    """A row's scales, in whole 16s."""
+    return -(-k // 512) * 16
+
+
 def _prepare_linear(case, gen):
     m, k, n, dt = (case[i] for i in ("m", "k", "cout", "dt"))
     st = {"x": _uneven(gen, m, k, dt)}
@@ -309,12 +314,12 @@ def _prepare_own(st):
         rows, k, kp = c["rows"], c["k"], _padded(c["k"])
         st["quant"] = mx4.Mx4QuantSpec(rows=rows, k=k, dt=dt)
         st["dequant"] = mx4.Mx4DequantSpec(rows=rows, k=k, dt=dt)
-        st["codes"], st["scales"], st["y"] = empty(rows, kp // 2), empty(rows, kp // 32), empty(rows, k, dtype=t)
+        st["codes"], st["scales"], st["y"] = empty(rows, kp // 2), empty(rows, _scale_bytes(k)), empty(rows, k, dtype=t)
     elif c["kind"] == "linear":
         m, k, n, kp = c["m"], c["k"], c["cout"], _padded(c["k"])
         st["quant"] = mx4.Mx4QuantSpec(rows=m, k=k, dt=dt)
         st["pw"] = mx4.Mx4PwSpec(m=m, k=k, cout=n, act=conv.Activation[c["act"].upper()], residual=c["residual"], dt=dt)
-        st["codes"], st["scales"], st["y"] = empty(m, kp // 2), empty(m, kp // 32), empty(m, n, dtype=t)
+        st["codes"], st["scales"], st["y"] = empty(m, kp // 2), empty(m, _scale_bytes(k)), empty(m, n, dtype=t)
     elif c["kind"] == "append":
         st["append"] = mx4.Kv4AppendSpec(tokens=c["tokens"], hq=c["hq"], hkv=c["hkv"], d=c["d"], rot=c["rot"],
                                          pairs=c["pairs"], norm=False, dt=dt, positions=st["cos"].shape[0],
@@ -360,10 +365,11 @@ def run(state):
 # ---------------------------------------------------------------- the plain forms, fp32
 
 def _plain_quant(x):
-    """codes [rows, kp/2] and scales [rows, kp/32], kp the row's length in whole 128s."""
+    """codes [rows, kp/2] and scales [rows, _scale_bytes(k)], kp the row's length in whole 128s."""
     rows, k = x.shape
     x = torch.nn.functional.pad(x.float(), (0, _padded(k) - k)).view(rows, -1, 32)
-    return _quant_blocks(x)
+    codes, scales = _quant_blocks(x)
+    return codes, torch.nn.functional.pad(scales, (0, _scale_bytes(k) - scales.shape[1]))
 
 
 def _quant_blocks(x):
@@ -380,11 +386,11 @@ def _quant_blocks(x):
 
 
 def _values(codes, scales):
-    """fp32 values [rows, blocks * 32] of codes [rows, bytes] and scales [rows, blocks]."""
+    """fp32 values [rows, blocks * 32] of codes [rows, blocks * 16] and scales [rows, blocks or more]."""
     grid = torch.tensor([0, .5, 1, 1.5, 2, 3, 4, 6, -0., -.5, -1, -1.5, -2, -3, -4, -6], device=codes.device)
     two = torch.stack([grid.repeat(16), grid.repeat_interleave(16)], -1)  # of a byte
     v = two[codes.int()].view(codes.shape[0], -1, 32)
-    s = scales.int()
+    s = scales[:, :codes.shape[1] // 16].int()
     s = torch.where(s == 255, 0x7fc00000, torch.where(s == 0, 0x00400000, s << 23)).view(torch.float32)
     return (v * s[..., None]).view(codes.shape[0], -1)
 
@@ -517,6 +523,7 @@ def _decode(codes, scales):
     e, f = (c >> 1) & 3, (c & 1).double()
     mag = torch.where(e == 0, f / 2, torch.ldexp(1 + f / 2, e - 1))
     v = torch.where(c >= 8, -mag, mag)
+    scales = scales[:, :codes.shape[1] // 16]
     s = torch.ldexp(torch.ones_like(scales, dtype=torch.float64), scales.long() - 127)
     return v * s.repeat_interleave(32, -1)
 
