@@ -1,0 +1,311 @@
+// mx4_pw.hip -- the pointwise conv of microscaled 4-bit rows (aih_mx4_pw).
+//
+// y[i][n] = act(sum_b 2^(sx[i][b] + sw[n][b]) sum_{k in b} x w + bias[n]) + res[i][n].
+// The scaled matrix instructions take the codes and the scale bytes as they are
+// stored: a lane holds one row's block of 32 codes (16 bytes) and its scale.
+// Weights are the A operand and pixels the B operand, so that a lane ends up with
+// one pixel's channels.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "aih_device.h"
+#include "mx4.h"
+
+namespace aih {
+namespace {
+
+typedef __attribute__((address_space(3))) void mx_lds_void;
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+constexpr uint32_t kOob = 0x80000000u;  // a byte offset past every buffer
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_rsrc(const void *base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, (int)bytes, 0x00020000);
+}
+
+// 16 bytes a lane from rs to LDS, lane after lane
+__device__ __forceinline__ void mx_dma(__amdgpu_buffer_rsrc_t rs, char *to, uint32_t off, uint32_t soff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (mx_lds_void *)to, 16, off, soff, 0, 0);
+}
+
+template <int N>
+__device__ __forceinline__ void mx_wait_vm() {
+  static_assert(N >= 0 && N < 64, "vmcnt");
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0F70);
+}
+// vmcnt(n) for a wavefront-uniform n in [0, MAXN]
+template <int MAXN>
+__device__ __forceinline__ void mx_wait_vm_n(uint32_t n) {
+  if constexpr (MAXN > 0) {
+    if (n >= (uint32_t)MAXN) {
+      mx_wait_vm<MAXN>();
+      return;
+    }
+    mx_wait_vm_n<MAXN - 1>(n);
+  } else {
+    mx_wait_vm<0>();
+  }
+}
+
+// c + A B, both 4-bit; byte T of each lane's scale word is its block's scale.
+template <int T>
+__device__ __forceinline__ f32x16 mx_mfma32(u32x4 a, u32x4 b, f32x16 c, uint32_t sa, uint32_t sb) {
+  const i32x8 a8 = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};
+  const i32x8 b8 = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a8, b8, c, 4, 4, T, (int)sa, T, (int)sb);
+}
+__device__ __forceinline__ f32x4 mx_mfma16(u32x4 a, u32x4 b, f32x4 c, uint32_t sa, uint32_t sb) {
+  const i32x8 a8 = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};
+  const i32x8 b8 = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a8, b8, c, 4, 4, 0, (int)sa, 0, (int)sb);
+}
+
+// act(v + bias) + res of four channels of a pixel
+template <int DT>
+__device__ __forceinline__ void mx_store4(const Mx4PwArgs &a, const Act &act, uint32_t i, uint32_t n, f32x4 v) {
+  if (i >= a.m || n >= a.cout) return;
+  if (a.bias) v += Vec4IO<DT>::load(a.bias, n / 4);
+  v = act4(act, v);
+  const size_t at = (size_t)i * (a.cout / 4) + n / 4;
+  if (a.res) v += Vec4IO<DT>::load(a.res, at);
+  Vec4IO<DT>::store(a.y, at, v);
+}
+
+// ---------------------------------------------------------------- few pixels
+//
+// Up to 64 pixels: bound by the weights' bytes (or, with few of those, by one chain of
+// loads, products and the join). A workgroup owns 16 channels, its W
+// wavefronts take turns at the stages of 128 elements, operands straight into registers
+// (a lane: channel lane % 16, block lane / 16 of the stage, 64 contiguous bytes a row),
+// and the partial sums are joined in LDS in the wavefronts' order.
+template <int DT, int TM, int W>
+__global__ __launch_bounds__(64 * W) void mx4_pw_few_kernel(Mx4PwArgs a) {
+  __shared__ f32x4 part[W][TM][64];
+  const uint32_t lane = threadIdx.x & 63, r = lane & 15, b = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t n0 = blockIdx.x * 16, nw = min(16u, a.cout - n0);
+  const __amdgpu_buffer_rsrc_t rwc = mx_rsrc(a.wc + (uint64_t)n0 * a.cb, nw * a.cb);
+  const __amdgpu_buffer_rsrc_t rws = mx_rsrc(a.ws + (uint64_t)n0 * a.sb, nw * a.sb);
+  const __amdgpu_buffer_rsrc_t rxc = mx_rsrc(a.xc, a.m * a.cb), rxs = mx_rsrc(a.xs, a.m * a.sb);
+  f32x4 acc[TM];
+#pragma unroll
+  for (int t = 0; t < TM; ++t) acc[t] = f32x4{};
+  constexpr int U = 2;  // stages on their way
+  for (uint32_t s0 = wave; s0 < a.nst; s0 += U * W) {
+    u32x4 wc[U], xc[U][TM];
+    uint32_t ws[U], xs[U][TM];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t s = s0 + u * W;
+      const bool on = s < a.nst;
+      wc[u] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rwc, on ? r * a.cb + s * 64 + b * 16 : kOob, 0, 0));
+      ws[u] = __builtin_amdgcn_raw_buffer_load_b8(rws, on ? r * a.sb + s * 4 + b : kOob, 0, 0);
+#pragma unroll
+      for (int t = 0; t < TM; ++t) {
+        xc[u][t] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rxc, on ? (16 * t + r) * a.cb + s * 64 + b * 16 : kOob, 0, 0));
+        xs[u][t] = __builtin_amdgcn_raw_buffer_load_b8(rxs, on ? (16 * t + r) * a.sb + s * 4 + b : kOob, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int t = 0; t < TM; ++t) acc[t] = mx_mfma16(wc[u], xc[u][t], acc[t], ws[u], xs[u][t]);
+  }
+#pragma unroll
+  for (int t = 0; t < TM; ++t) part[wave][t][lane] = acc[t];
+  __syncthreads();
+  const Act act = act_params(a.act);
+  for (uint32_t t = wave; t < TM; t += W) {
+    f32x4 v = part[0][t][lane];
+#pragma unroll
+    for (int w = 1; w < W; ++w) v += part[w][t][lane];
+    mx_store4<DT>(a, act, 16 * t + r, n0 + 4 * b, v);
+  }
+}
+
+// ---------------------------------------------------------------- tiles
+//
+// WM x WN wavefronts of TM x TN blocks of 32 pixels x 32 channels. Stages of 128
+// elements (64 bytes a row) come into LDS by DMA, NST - 1 ahead of the products;
+// the scales of four stages (16 bytes a row) every fourth one. Unit u of tile row r
+// is at slot u ^ ((r >> 2) & 3), which spreads 16 rows' units over the banks.
+template <int WM_, int WN_, int TM_, int TN_, int NST_>
+struct MxTile {
+  static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, NST = NST_;
+  static constexpr int NW = WM * WN, BM = 32 * WM * TM, BN = 32 * WN * TN;
+  static constexpr uint32_t STAGE = (BM + BN) * 64;
+  static constexpr int CI = (BM + BN) / 16;                       // DMA instructions of a stage
+  static constexpr int SX = (BM + 63) / 64, SI = SX + (BN + 63) / 64;  // of four stages' scales
+  static constexpr uint32_t SCALES = SI * 1024;
+  static constexpr uint32_t LDS = NST * STAGE + 2 * SCALES;
+  static_assert(NST >= 2 && NST <= 4 && LDS <= 160 * 1024, "LDS");
+};
+
+// The products of 64 elements: `at` is where the lane's unit is in its rows.
+template <class C, int T>
+__device__ __forceinline__ void mx_step(const char *px, const char *pw, uint32_t at, f32x16 (&acc)[C::TM][C::TN],
+                                        const uint32_t (&sx)[C::TM], const uint32_t (&sn)[C::TN]) {
+  u32x4 x[C::TM], w[C::TN];
+#pragma unroll
+  for (int i = 0; i < C::TM; ++i) x[i] = *reinterpret_cast<const u32x4 *>(px + i * 2048 + at);
+#pragma unroll
+  for (int j = 0; j < C::TN; ++j) w[j] = *reinterpret_cast<const u32x4 *>(pw + j * 2048 + at);
+#pragma unroll
+  for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) acc[i][j] = mx_mfma32<T>(w[j], x[i], acc[i][j], sn[j], sx[i]);
+}
+
+template <int DT, class C>
+__global__ __launch_bounds__(64 * C::NW) void mx4_pw_kernel(Mx4PwArgs a) {
+  constexpr int TM = C::TM, TN = C::TN, NW = C::NW, NST = C::NST;
+  constexpr int CK = (C::CI + NW - 1) / NW, SK = (C::SI + NW - 1) / NW;
+  extern __shared__ __align__(16) char lds[];
+  const int lane = threadIdx.x & 63, l32 = lane & 31, lh = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave % C::WM, wn = wave / C::WM;
+
+  // tiles in groups of 8 rows of them: those that run at once share operands
+  const uint32_t t = xcd_remap(blockIdx.x, gridDim.x, a.nxcd);
+  const uint32_t group = t / (8 * a.ntiles), first = group * 8, rows = min(a.mtiles - first, 8u);
+  const uint32_t rest = t - group * 8 * a.ntiles, nt = rest / rows, mt = first + (rest - nt * rows);
+  const uint32_t m0 = mt * C::BM, n0 = nt * C::BN;
+  const uint32_t mr = min(a.m - m0, (uint32_t)C::BM), nr = min(a.cout - n0, (uint32_t)C::BN);
+
+  const __amdgpu_buffer_rsrc_t rxc = mx_rsrc(a.xc + (uint64_t)m0 * a.cb, mr * a.cb);
+  const __amdgpu_buffer_rsrc_t rwc = mx_rsrc(a.wc + (uint64_t)n0 * a.cb, nr * a.cb);
+  const __amdgpu_buffer_rsrc_t rxs = mx_rsrc(a.xs + (uint64_t)m0 * a.sb, mr * a.sb);
+  const __amdgpu_buffer_rsrc_t rws = mx_rsrc(a.ws + (uint64_t)n0 * a.sb, nr * a.sb);
+
+  // instruction i of a stage: tile rows 16 i + lane / 4 (pixels, then channels)
+  const uint32_t cu = (uint32_t)(lane & 3) ^ ((lane >> 4) & 3);
+  uint32_t coff[CK];
+#pragma unroll
+  for (int k = 0; k < CK; ++k) {
+    const int i = wave + k * NW;
+    const uint32_t r = (i < C::BM / 16 ? 16 * i : 16 * i - C::BM) + lane / 4;
+    coff[k] = r < (i < C::BM / 16 ? mr : nr) ? r * a.cb + cu * 16 : kOob;
+  }
+  uint32_t soff[SK];
+#pragma unroll
+  for (int k = 0; k < SK; ++k) {
+    const int i = wave + k * NW;
+    const uint32_t r = (i < C::SX ? 64 * i : 64 * (i - C::SX)) + lane;
+    soff[k] = r < (i < C::SX ? mr : nr) ? r * a.sb : kOob;
+  }
+  const uint32_t nc = C::CI % NW == 0 ? CK : (C::CI - wave + NW - 1) / NW;  // this wavefront's
+  const uint32_t ns = C::SI % NW == 0 ? SK : C::SI > wave ? (C::SI - wave + NW - 1) / NW : 0;
+
+  // requests stage s; stages are requested in order
+  auto issue = [&](uint32_t s, uint32_t buf) {
+    if (s % 4 == 0) {
+      char *to = lds + NST * C::STAGE + (s / 4 & 1) * C::SCALES;
+#pragma unroll
+      for (int k = 0; k < SK; ++k) {
+        const int i = wave + k * NW;
+        if (C::SI % NW != 0 && i >= C::SI) break;
+        if (i < C::SX) mx_dma(rxs, to + i * 1024, soff[k], s * 4);
+        else mx_dma(rws, to + i * 1024, soff[k], s * 4);
+      }
+    }
+    char *to = lds + buf * C::STAGE;
+#pragma unroll
+    for (int k = 0; k < CK; ++k) {
+      const int i = wave + k * NW;
+      if (C::CI % NW != 0 && i >= C::CI) break;
+      if (i < C::BM / 16) mx_dma(rxc, to + i * 1024, coff[k], s * 64);
+      else mx_dma(rwc, to + i * 1024, coff[k], s * 64);
+    }
+  };
+
+  f32x16 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = f32x16{};
+
+  const uint32_t pr = 32 * TM * wm + l32, cr = 32 * TN * wn + l32;  // the lane's first rows
+  const uint32_t sw = (l32 >> 2) & 3;
+  auto compute = [&](uint32_t s, uint32_t buf) {
+    const char *base = lds + buf * C::STAGE;
+    // half h takes blocks 2h and 2h + 1 of the stage
+    const char *sc = lds + NST * C::STAGE + (s / 4 & 1) * C::SCALES + (s & 3) * 4 + 2 * lh;
+    uint32_t sx[TM], sn[TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) sx[i] = *reinterpret_cast<const uint16_t *>(sc + (pr + 32 * i) * 16);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) sn[j] = *reinterpret_cast<const uint16_t *>(sc + C::SX * 1024 + (cr + 32 * j) * 16);
+    mx_step<C, 0>(base + pr * 64, base + (C::BM + cr) * 64, ((2 * lh) ^ sw) * 16, acc, sx, sn);
+    mx_step<C, 1>(base + pr * 64, base + (C::BM + cr) * 64, ((2 * lh + 1) ^ sw) * 16, acc, sx, sn);
+  };
+
+#pragma unroll
+  for (int s = 0; s < NST - 1; ++s)
+    if ((uint32_t)s < a.nst) issue(s, s);
+  uint32_t bc = 0, bi = NST - 1;  // buffer of the stage computed / requested
+  for (uint32_t s = 0; s < a.nst; ++s) {
+    // stage s has landed once at most the copies of the stages requested after it
+    // are on their way: of one with scales among them, too
+    const uint32_t later = min(a.nst - 1 - s, (uint32_t)(NST - 2));
+    const uint32_t scales = (s + later) / 4 != s / 4 ? ns : 0;
+    mx_wait_vm_n<CK * (NST - 2) + SK>(later * nc + scales);
+    // for every wavefront, and all are done with the buffer that is requested next. A bare
+    // barrier: a workgroup fence would wait for the copies on their way
+    __asm__ volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (s + NST - 1 < a.nst) issue(s + NST - 1, bi);
+    compute(s, bc);
+    bc = bc + 1 == NST ? 0 : bc + 1;
+    bi = bi + 1 == NST ? 0 : bi + 1;
+  }
+
+  const Act act = act_params(a.act);
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4)
+        mx_store4<DT>(a, act, m0 + pr + 32 * i, n0 + 32 * TN * wn + 32 * j + 8 * r4 + 4 * lh,
+                      f32x4{acc[i][j][4 * r4], acc[i][j][4 * r4 + 1], acc[i][j][4 * r4 + 2], acc[i][j][4 * r4 + 3]});
+}
+
+template <int DT, class C>
+hipError_t launch_tile(Mx4PwArgs a, hipStream_t st) {
+  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(mx4_pw_kernel<DT, C>),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
+  if (attr != hipSuccess) return attr;
+  a.mtiles = (a.m + C::BM - 1) / C::BM, a.ntiles = (a.cout + C::BN - 1) / C::BN;
+  if ((uint64_t)a.mtiles * a.ntiles > 0x7fffffffu) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((mx4_pw_kernel<DT, C>), dim3(a.mtiles * a.ntiles), dim3(64 * C::NW), C::LDS, st, a);
+  return hipGetLastError();
+}
+
+template <int DT, int TM>
+hipError_t launch_few(const Mx4PwArgs &a, hipStream_t st) {
+  const dim3 grid((a.cout + 15) / 16);
+  if (a.nst >= 32) hipLaunchKernelGGL((mx4_pw_few_kernel<DT, TM, 16>), grid, dim3(1024), 0, st, a);
+  else hipLaunchKernelGGL((mx4_pw_few_kernel<DT, TM, 4>), grid, dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+template <int DT>
+hipError_t launch_dt(const Mx4PwArgs &a, hipStream_t st) {
+  if (a.m <= 16) return launch_few<DT, 1>(a, st);
+  if (a.m <= 32) return launch_few<DT, 2>(a, st);
+  if (a.m <= 64) return launch_few<DT, 4>(a, st);
+  const uint64_t big = (uint64_t)((a.m + 255) / 256) * ((a.cout + 255) / 256);
+  const uint64_t mid = (uint64_t)((a.m + 127) / 128) * ((a.cout + 127) / 128);
+  const uint32_t cus = device_cus();
+  if (big >= cus) return launch_tile<DT, MxTile<2, 4, 4, 2, 3>>(a, st);
+  if (mid >= cus) return launch_tile<DT, MxTile<2, 2, 2, 2, 3>>(a, st);
+  return launch_tile<DT, MxTile<2, 2, 1, 1, 4>>(a, st);
+}
+
+}  // namespace
+
+hipError_t launch_mx4_pw(const Mx4PwArgs &a, int dt, hipStream_t st) {
+  return dt == DT_F32 ? launch_dt<DT_F32>(a, st) : dt == DT_F16 ? launch_dt<DT_F16>(a, st) : launch_dt<DT_BF16>(a, st);
+}
+
+}  // namespace aih
