@@ -173,7 +173,8 @@ EXPORTS = (
     "aih_ir_block_stem_plan", "aih_ir_block_stem",
     "aih_ir_block_head_plan", "aih_ir_block_head",
     "aih_qk_norm_rope", "aih_attn_plan", "aih_attn",  # bound in attn.py
-    "aih_mx4_quant", "aih_mx4_dequant", "aih_mx4_pw",  # bound in mx4.py
+    "aih_mx4_quant", "aih_mx4_dequant", "aih_mx4_pw", "aih_kv4_append", "aih_kv4_attn_plan",
+    "aih_kv4_attn",  # bound in mx4.py
 )
 
 _lib = None

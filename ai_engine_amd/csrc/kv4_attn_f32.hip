@@ -1,0 +1,8 @@
+// kv4_attn_f32.hip -- the f32 instances of the attention over a 4-bit cache.
+#include "kv4_attn_impl.h"
+
+namespace aih {
+
+hipError_t launch_kv4_attn_f32(const Kv4AttnArgs &a, hipStream_t st) { return kv_launch_dt<DT_F32>(a, st); }
+
+}  // namespace aih

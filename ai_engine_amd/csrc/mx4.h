@@ -8,6 +8,7 @@
 
 #include "../../include/aih_mx4.h"
 #include "aih_device.h"
+#include "attn.h"
 
 namespace aih {
 
@@ -39,6 +40,39 @@ struct Mx4PwArgs {
 };
 
 hipError_t launch_mx4_pw(const Mx4PwArgs &a, int dt, hipStream_t st);
+
+struct Kv4AppendArgs {
+  const void *x, *wq, *wk;
+  const float *cs, *sn;
+  const int32_t *pos, *slots;
+  void *q;
+  uint8_t *kc, *ks, *vc, *vs;
+  uint64_t xs, qs;          // row strides, elements
+  uint32_t hq, hkv;
+  uint32_t d, rot, pairs, norm;
+  uint32_t positions, rows; // rows: pages * page
+  uint32_t pshift;          // log2 of the rows of a page
+  uint32_t items;           // tokens * (hq + 2 hkv)
+  float eps, inv_d;
+  FastDiv by_ht;
+};
+
+hipError_t launch_kv4_append(const Kv4AppendArgs &a, int dt, hipStream_t st);
+
+// The rows, sequences and parts are those of AttnArgs (its key fields are not
+// used), so the parts join as there.
+struct Kv4AttnArgs {
+  AttnArgs at;
+  const uint8_t *kc, *ks, *vc, *vs;
+  const int32_t *table;
+  uint32_t width, pages, pshift;
+};
+
+uint32_t kv4_attn_bm();
+hipError_t launch_kv4_attn(const Kv4AttnArgs &a, int dt, hipStream_t st);
+hipError_t launch_kv4_attn_f32(const Kv4AttnArgs &a, hipStream_t st);
+hipError_t launch_kv4_attn_f16(const Kv4AttnArgs &a, hipStream_t st);
+hipError_t launch_kv4_attn_bf16(const Kv4AttnArgs &a, hipStream_t st);
 
 // A scale byte as the conversion instructions take it: a float of which they read
 // the exponent alone (0 is 2^-127, 255 makes NaN of whatever is converted).

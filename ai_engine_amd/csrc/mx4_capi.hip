@@ -52,7 +52,87 @@ int rows_stride(const char *fn, const char *what, uint64_t given, uint32_t k, ui
   return AIH_OK;
 }
 
+// A row stride in elements of `row`-long rows: whole 16-byte units.
+int heads_stride(const char *fn, const char *what, uint64_t given, uint64_t row, int32_t dt, uint64_t *out) {
+  *out = given ? given : row;
+  if (*out < row || *out * (dt == AIH_F32 ? 4 : 2) % 16 || *out > kMaxStride)
+    return api_fail(std::string(fn) + ": " + what + " must be 0 or whole 16-byte units from " + num(row) + " to " +
+                    num(kMaxStride) + ", not " + num(given));
+  return AIH_OK;
+}
+
+int cache_ok(const char *fn, uint32_t hkv, uint32_t d, uint32_t page, uint32_t pages, int32_t dt) {
+  if (!dt_ok(dt)) return api_fail(std::string(fn) + ": unknown dtype " + std::to_string(dt));
+  if (d == 0 || d % 32 || d > 256) return api_fail(std::string(fn) + ": d must be a multiple of 32, 32 to 256, not " + num(d));
+  if (hkv == 0 || hkv > 4096) return api_fail(std::string(fn) + ": hkv must be 1 to 4096");
+  if (page < 16 || page > 4096 || (page & (page - 1)))
+    return api_fail(std::string(fn) + ": page must be a power of two, 16 to 4096, not " + num(page));
+  if ((uint64_t)pages * page > 0x7fffffffu) return api_fail(std::string(fn) + ": pages * page must be below 2^31");
+  return AIH_OK;
+}
+
+uint32_t log2_of(uint32_t pow2) {
+  uint32_t s = 0;
+  while ((1u << s) < pow2) ++s;
+  return s;
+}
+
+struct Kv4Plan {
+  uint64_t tiles;  // of a key head, at most
+  uint32_t parts, shift;
+  uint64_t ws_floats;
+};
+
+// How the keys are cut. A workgroup's 32 rows against all keys are a chain; cutting
+// them spreads it and costs partial results and a launch that joins them.
+int check_kv4_attn(const aih_kv4_attn_desc *d, AttnArgs *a, Kv4Plan *p) {
+  const char *fn = "aih_kv4_attn";
+  if (!d) return api_fail("aih_kv4_attn: NULL descriptor");
+  if (int rc = cache_ok(fn, d->hkv, d->d, d->page, d->pages, d->dt)) return rc;
+  if (d->hq == 0 || d->hq > 4096 || d->hq % d->hkv) return api_fail("aih_kv4_attn: hq must be a multiple of hkv, at most 4096");
+  if (d->causal != 0 && d->causal != 1) return api_fail("aih_kv4_attn: causal must be 0 or 1");
+  if (d->nseq > 0x7fffffffu || d->tokens > 0x7fffffffu) return api_fail("aih_kv4_attn: counts must be below 2^31");
+  if ((uint64_t)d->tokens * d->hq > 0x7fffffffu) return api_fail("aih_kv4_attn: tokens * hq must be below 2^31");
+  if ((uint64_t)d->table_width * d->page > 0x7fffffffu) return api_fail("aih_kv4_attn: table_width * page must be below 2^31");
+  if (d->scale != 0.0f && !(d->scale >= 1e-20f && d->scale <= 1e20f))
+    return api_fail("aih_kv4_attn: scale must be 0 or 1e-20 to 1e20");
+  *a = AttnArgs{};
+  *p = Kv4Plan{0, 1, 31, 0};
+  a->nseq = d->nseq, a->tokens = d->tokens;
+  a->rows = d->pages ? d->table_width * d->page : 0;  // keys of a sequence at most
+  a->hq = d->hq, a->hkv = d->hkv, a->g = d->hq / d->hkv, a->d = d->d;
+  a->causal = (uint32_t)d->causal;
+  const double scale = d->scale != 0.0f ? (double)d->scale : 1.0 / std::sqrt((double)d->d);
+  a->scale_log2 = (float)(scale * 1.4426950408889634);
+  if (int rc = heads_stride(fn, "q_stride", d->q_stride, (uint64_t)d->hq * d->d, d->dt, &a->qs)) return rc;
+  if (int rc = heads_stride(fn, "o_stride", d->o_stride, (uint64_t)d->hq * d->d, d->dt, &a->os)) return rc;
+  if (d->nseq == 0 || d->tokens == 0) return AIH_OK;
+  const uint64_t rows = (uint64_t)d->tokens * a->g;
+  const uint32_t bm = kv4_attn_bm();
+  p->tiles = d->nseq == 1 ? (rows + bm - 1) / bm : rows / bm + d->nseq;
+  const uint32_t len = d->max_len ? std::min(d->max_len, a->rows) : a->rows;
+  auto parts = [&](uint32_t x) { return (uint32_t)std::max<uint64_t>(1, ((uint64_t)len + (1ull << x) - 1) >> x); };
+  const uint64_t base = p->tiles * d->hkv;
+  const uint32_t cus = device_cus();
+  if (len > 512) {
+    if (rows <= (uint64_t)bm * d->nseq) p->shift = 10;
+    while (p->shift > 8 && base * parts(p->shift) < 2ull * cus) --p->shift;
+  }
+  p->parts = parts(p->shift);
+  if (p->parts == 1) p->shift = 31;
+  if (base * p->parts > 0x7fffffffu) return api_fail("aih_kv4_attn: more than 2^31 - 1 tiles");
+  if (p->parts > 1) p->ws_floats = (uint64_t)p->parts * d->tokens * d->hq * (d->d + 2);
+  return AIH_OK;
+}
+
 }  // namespace
+
+uint32_t kv4_attn_bm() { return 32; }
+
+hipError_t launch_kv4_attn(const Kv4AttnArgs &a, int dt, hipStream_t st) {
+  return dt == DT_F32 ? launch_kv4_attn_f32(a, st) : dt == DT_F16 ? launch_kv4_attn_f16(a, st) : launch_kv4_attn_bf16(a, st);
+}
+
 }  // namespace aih
 
 using namespace aih;
@@ -129,5 +209,90 @@ extern "C" int aih_mx4_pw(const aih_mx4_pw_desc *d, const void *x_codes, const v
     a.cb = AIH_MX4_CODE_BYTES(d->k), a.sb = AIH_MX4_SCALE_BYTES(d->k), a.nst = a.cb / 64;
     a.nxcd = device_xcds();
     return launched(fn, launch_mx4_pw(a, d->dt, stream_of(stream)));
+  });
+}
+
+extern "C" int aih_kv4_append(const aih_kv4_append_desc *d, const void *x, const void *wq, const void *wk,
+                              const float *cosines, const float *sines, const int32_t *pos, const int32_t *slots,
+                              void *q, void *k_codes, void *k_scales, void *v_codes, void *v_scales, aih_stream stream) {
+  return api_guarded([&]() -> int {
+    const char *fn = "aih_kv4_append";
+    if (!d) return api_fail("aih_kv4_append: NULL descriptor");
+    if (int rc = cache_ok(fn, d->hkv, d->d, d->page, d->pages, d->dt)) return rc;
+    if (d->hq > 4096) return api_fail("aih_kv4_append: hq must be at most 4096");
+    if (d->rot % 16 || d->rot > d->d)
+      return api_fail("aih_kv4_append: rot must be a multiple of 16, at most d, not " + num(d->rot));
+    if (d->pairs != 0 && d->pairs != 1) return api_fail("aih_kv4_append: pairs must be 0 or 1");
+    if (d->norm != 0 && d->norm != 1) return api_fail("aih_kv4_append: norm must be 0 or 1");
+    if (!(d->eps >= 0.0f) || !std::isfinite(d->eps)) return api_fail("aih_kv4_append: eps must be >= 0 and finite");
+    if (d->rot && (d->positions == 0 || d->positions > 0x7fffffffu))
+      return api_fail("aih_kv4_append: the tables need 1 to 2^31 - 1 rows");
+    const uint64_t heads = (uint64_t)d->hq + 2 * (uint64_t)d->hkv;
+    if (d->tokens * heads > 0x7fffffffu) return api_fail("aih_kv4_append: tokens * (hq + 2 hkv) must be below 2^31");
+    Kv4AppendArgs a{};
+    if (int rc = heads_stride(fn, "x_stride", d->x_stride, heads * d->d, d->dt, &a.xs)) return rc;
+    if (int rc = heads_stride(fn, "q_stride", d->q_stride, (uint64_t)d->hq * d->d, d->dt, &a.qs)) return rc;
+    if (d->tokens == 0) return AIH_OK;
+    if (!none_null({x, slots, k_codes, k_scales, v_codes, v_scales}) || (d->hq && !q))
+      return api_fail("aih_kv4_append: NULL tensor");
+    if (d->rot && (!cosines || !sines)) return api_fail("aih_kv4_append: rot > 0 needs cosines and sines");
+    if (!aligned16({x, wq, wk, cosines, sines, q, k_codes, k_scales, v_codes, v_scales}))
+      return api_fail("aih_kv4_append: tensors must be aligned to 16 bytes");
+    a.x = x, a.wq = wq, a.wk = wk, a.cs = cosines, a.sn = sines, a.pos = pos, a.slots = slots, a.q = q;
+    a.kc = static_cast<uint8_t *>(k_codes), a.ks = static_cast<uint8_t *>(k_scales);
+    a.vc = static_cast<uint8_t *>(v_codes), a.vs = static_cast<uint8_t *>(v_scales);
+    a.hq = d->hq, a.hkv = d->hkv, a.d = d->d, a.rot = d->rot, a.pairs = (uint32_t)d->pairs, a.norm = (uint32_t)d->norm;
+    a.positions = d->positions, a.rows = d->pages * d->page, a.pshift = log2_of(d->page);
+    a.items = (uint32_t)(d->tokens * heads);
+    a.eps = d->eps, a.inv_d = 1.0f / (float)d->d;
+    a.by_ht = make_fastdiv((uint32_t)heads);
+    return launched(fn, launch_kv4_append(a, d->dt, stream_of(stream)));
+  });
+}
+
+extern "C" int aih_kv4_attn_plan(const aih_kv4_attn_desc *d, aih_kv4_attn_plan_info *out) {
+  return api_guarded([&]() -> int {
+    AttnArgs a;
+    Kv4Plan p;
+    if (int rc = check_kv4_attn(d, &a, &p)) return rc;
+    if (!out) return api_fail("aih_kv4_attn_plan: NULL output");
+    *out = aih_kv4_attn_plan_info{};
+    out->bm = kv4_attn_bm(), out->parts = p.parts, out->chunk = p.parts > 1 ? 1u << p.shift : 0;
+    out->grid = (uint32_t)(p.tiles * d->hkv * p.parts);
+    out->ws_bytes = p.ws_floats * 4;
+    return AIH_OK;
+  });
+}
+
+extern "C" int aih_kv4_attn(const aih_kv4_attn_desc *d, const void *q, const void *k_codes, const void *k_scales,
+                            const void *v_codes, const void *v_scales, const int32_t *q_start, const int32_t *table,
+                            const int32_t *k_len, void *o, void *ws, size_t ws_bytes, aih_stream stream) {
+  return api_guarded([&]() -> int {
+    const char *fn = "aih_kv4_attn";
+    Kv4AttnArgs a{};
+    Kv4Plan p;
+    if (int rc = check_kv4_attn(d, &a.at, &p)) return rc;
+    if (d->nseq == 0 || d->tokens == 0) return AIH_OK;
+    if (!none_null({q, q_start, k_len, o})) return api_fail("aih_kv4_attn: NULL tensor");
+    if (a.at.rows && !none_null({k_codes, k_scales, v_codes, v_scales, table}))
+      return api_fail("aih_kv4_attn: a cache with pages must not be NULL");
+    if (!aligned16({q, k_codes, k_scales, v_codes, v_scales, o, ws}))
+      return api_fail("aih_kv4_attn: tensors must be aligned to 16 bytes");
+    if (p.ws_floats && (!ws || ws_bytes < p.ws_floats * 4))
+      return api_fail("aih_kv4_attn: the workspace needs " + num(p.ws_floats * 4) + " bytes, not " + num(ws ? ws_bytes : 0));
+    AttnArgs &t = a.at;
+    t.q = q, t.o = o, t.ws = p.ws_floats ? static_cast<float *>(ws) : nullptr;
+    t.q_start = q_start, t.k_len = k_len;
+    t.by_g = make_fastdiv(t.g), t.by_hkv = make_fastdiv(t.hkv);
+    t.tiles = (uint32_t)p.tiles, t.parts = p.parts, t.shift = p.shift, t.all_parts = p.parts;
+    // prompts of different lengths start with the longest
+    t.sort = d->nseq > 1 && d->nseq <= 32 && (uint64_t)d->tokens * t.g > 32ull * d->nseq;
+    a.kc = static_cast<const uint8_t *>(k_codes), a.ks = static_cast<const uint8_t *>(k_scales);
+    a.vc = static_cast<const uint8_t *>(v_codes), a.vs = static_cast<const uint8_t *>(v_scales);
+    a.table = table, a.width = d->table_width, a.pages = d->pages, a.pshift = log2_of(d->page);
+    const hipStream_t st = stream_of(stream);
+    if (int rc = launched(fn, launch_kv4_attn(a, d->dt, st))) return rc;
+    if (!t.ws) return AIH_OK;
+    return launched(fn, launch_attn_join(t, d->dt, st));
   });
 }

@@ -3,6 +3,9 @@
 * `Mx4QuantSpec`   -> aih_mx4_quant: rows of a storage type to 4 bits
 * `Mx4DequantSpec` -> aih_mx4_dequant: the values that 4-bit rows stand for
 * `Mx4PwSpec`      -> aih_mx4_pw: the 1x1 conv of 4-bit rows and 4-bit weights
+* `Kv4AppendSpec`  -> aih_kv4_append: rotation of queries and keys, new keys and
+  values into the pages of a 4-bit cache
+* `Kv4AttnSpec`    -> aih_kv4_attn: attention over such a cache
 
 As in `conv`, buffers are device tensors or raw device addresses, every call is
 asynchronous on the given stream (default: torch's current stream), and there is no
@@ -22,7 +25,7 @@ import ctypes as C
 from dataclasses import dataclass
 
 from . import conv
-from .attn import _u32
+from .attn import _u32, _workspace_on
 from .conv import Activation, AihError, DType
 
 
@@ -40,6 +43,25 @@ class _PwDesc(C.Structure):
                 ("residual", C.c_int32), ("dt", C.c_int32)]
 
 
+class _AppendDesc(C.Structure):
+    _fields_ = [("tokens", C.c_uint32), ("hq", C.c_uint32), ("hkv", C.c_uint32), ("d", C.c_uint32),
+                ("rot", C.c_uint32), ("pairs", C.c_int32), ("norm", C.c_int32), ("eps", C.c_float), ("dt", C.c_int32),
+                ("positions", C.c_uint32), ("page", C.c_uint32), ("pages", C.c_uint32), ("x_stride", C.c_uint64),
+                ("q_stride", C.c_uint64)]
+
+
+class _AttnDesc(C.Structure):
+    _fields_ = [("nseq", C.c_uint32), ("tokens", C.c_uint32), ("hq", C.c_uint32), ("hkv", C.c_uint32),
+                ("d", C.c_uint32), ("page", C.c_uint32), ("pages", C.c_uint32), ("table_width", C.c_uint32),
+                ("causal", C.c_int32), ("scale", C.c_float), ("dt", C.c_int32), ("max_len", C.c_uint32),
+                ("q_stride", C.c_uint64), ("o_stride", C.c_uint64)]
+
+
+class Kv4AttnPlan(C.Structure):
+    _fields_ = [("bm", C.c_uint32), ("parts", C.c_uint32), ("chunk", C.c_uint32), ("grid", C.c_uint32),
+                ("ws_bytes", C.c_size_t)]
+
+
 _lib = None
 
 
@@ -52,6 +74,9 @@ def lib() -> C.CDLL:
             "aih_mx4_quant": [C.POINTER(_QuantDesc)] + [P] * 4,
             "aih_mx4_dequant": [C.POINTER(_DequantDesc)] + [P] * 4,
             "aih_mx4_pw": [C.POINTER(_PwDesc)] + [P] * 8,
+            "aih_kv4_append": [C.POINTER(_AppendDesc)] + [P] * 13,
+            "aih_kv4_attn_plan": [C.POINTER(_AttnDesc), C.POINTER(Kv4AttnPlan)],
+            "aih_kv4_attn": [C.POINTER(_AttnDesc)] + [P] * 10 + [C.c_size_t, P],
         }
         for name, args in sigs.items():
             fn = getattr(L, name)
@@ -196,3 +221,123 @@ class Mx4PwSpec:
                 _take("y", y, ny, t, dev), conv._stream(stream)):
             raise AihError(conv.last_error())
         return y
+
+
+def kv4_cache(pages, page, hkv, d, device="cuda:0"):
+    """(k_codes, k_scales, v_codes, v_scales) of an empty 4-bit cache: [pages, hkv, page, d / 2] and [..., d / 32]."""
+    import torch
+
+    return tuple(torch.zeros(pages, hkv, page, n, dtype=torch.uint8, device=device) for n in (d // 2, d // 32) * 2)
+
+
+@dataclass(frozen=True)
+class Kv4AppendSpec:
+    """New tokens into a 4-bit cache; fields of aih_kv4_append_desc (strides in elements, 0 = dense)."""
+
+    tokens: int
+    hq: int
+    hkv: int
+    d: int
+    page: int
+    pages: int
+    rot: int = 0
+    pairs: bool = False
+    norm: bool = False
+    eps: float = 1e-6
+    dt: DType = DType.F32
+    positions: int = 0
+    x_stride: int = 0
+    q_stride: int = 0
+
+    def __post_init__(self):
+        u = {n: _u32(n, getattr(self, n)) for n in ("tokens", "hq", "hkv", "d", "rot", "positions", "page", "pages",
+                                                    "x_stride", "q_stride")}
+        object.__setattr__(self, "_desc", _AppendDesc(
+            u["tokens"], u["hq"], u["hkv"], u["d"], u["rot"], int(bool(self.pairs)), int(bool(self.norm)), self.eps,
+            int(self.dt), u["positions"], u["page"], u["pages"], u["x_stride"], u["q_stride"]))
+        row, rows = (self.hq + 2 * self.hkv) * self.d, self.pages * self.hkv * self.page
+        object.__setattr__(self, "_sizes", (
+            _span(self.tokens, self.x_stride or row, row),
+            _span(self.tokens, self.q_stride or self.hq * self.d, self.hq * self.d) if self.hq else 0,
+            self.positions * (self.rot // 2), rows * (self.d // 2), rows * (self.d // 32)))
+
+    def run(self, x, wq, wk, cosines, sines, pos, slots, q, k_codes, k_scales, v_codes, v_scales, stream=None):
+        """x [tokens, x_stride]; wq, wk [d] or None; cosines, sines [positions, rot/2] fp32; pos int32 [tokens] or None;
+        slots int32 [tokens]; q [tokens, hq, d]; the cache as kv4_cache makes it."""
+        T, device, types, u8, i32 = _torch or _torch_types()
+        dev, t, f32 = device() if x.__class__ is T else None, types.get(self.dt), types[0]
+        nx, nq, nt, nc, ns = self._sizes
+        if (_lib or lib()).aih_kv4_append(
+                C.byref(self._desc), _take("x", x, nx, t, dev), _take("wq", wq, self.d, t, dev),
+                _take("wk", wk, self.d, t, dev), _take("cosines", cosines, nt, f32, dev),
+                _take("sines", sines, nt, f32, dev), _take("pos", pos, self.tokens, i32, dev),
+                _take("slots", slots, self.tokens, i32, dev), _take("q", q, nq, t, dev),
+                _take("k_codes", k_codes, nc, u8, dev), _take("k_scales", k_scales, ns, u8, dev),
+                _take("v_codes", v_codes, nc, u8, dev), _take("v_scales", v_scales, ns, u8, dev), conv._stream(stream)):
+            raise AihError(conv.last_error())
+        return q
+
+
+@dataclass(frozen=True)
+class Kv4AttnSpec:
+    """Attention over a 4-bit cache; fields of aih_kv4_attn_desc (strides in elements, 0 = dense; scale None =
+    1 / sqrt(d))."""
+
+    nseq: int
+    tokens: int
+    hq: int
+    hkv: int
+    d: int
+    page: int
+    pages: int
+    table_width: int
+    causal: bool = True
+    scale: float | None = None
+    dt: DType = DType.F32
+    max_len: int = 0
+    q_stride: int = 0
+    o_stride: int = 0
+
+    def __post_init__(self):
+        if self.scale is not None and not self.scale > 0:
+            raise AihError(f"scale must be positive, not {self.scale!r}")
+        object.__setattr__(self, "_desc", _AttnDesc(
+            *(_u32(n, getattr(self, n)) for n in ("nseq", "tokens", "hq", "hkv", "d", "page", "pages", "table_width")),
+            int(bool(self.causal)), self.scale or 0.0, int(self.dt), _u32("max_len", self.max_len),
+            _u32("q_stride", self.q_stride), _u32("o_stride", self.o_stride)))
+        row, rows = self.hq * self.d, self.pages * self.hkv * self.page
+        object.__setattr__(self, "_sizes", (
+            _span(self.tokens, self.q_stride or row, row), _span(self.tokens, self.o_stride or row, row),
+            rows * (self.d // 2), rows * (self.d // 32), self.nseq * self.table_width))
+        object.__setattr__(self, "_ws", None)
+
+    def plan(self) -> Kv4AttnPlan:
+        p = Kv4AttnPlan()
+        conv._check(lib().aih_kv4_attn_plan(C.byref(self._desc), C.byref(p)))
+        return p
+
+    def workspace_bytes(self) -> int:
+        if self._ws is None:
+            object.__setattr__(self, "_ws", self.plan().ws_bytes)
+        return self._ws
+
+    def run(self, q, k_codes, k_scales, v_codes, v_scales, q_start, table, k_len, out, ws=None, stream=None):
+        """q, out [tokens, hq, d]; the cache as kv4_cache makes it; q_start [nseq + 1], table [nseq, table_width], k_len
+        [nseq] int32; ws: workspace_bytes() of device memory, made here if None."""
+        T, device, types, u8, i32 = _torch or _torch_types()
+        dev, t, b = device() if out.__class__ is T else None, types.get(self.dt), self.nseq
+        nq, no, nc, ns, nt = self._sizes
+        n = self._ws if self._ws is not None else self.workspace_bytes()
+        if n:
+            if ws is None:
+                ws = _workspace_on(n, conv._device_of(out), stream)
+            if not isinstance(ws, int) and ws.numel() * ws.element_size() < n:
+                raise AihError(f"the workspace needs {n} bytes, not {ws.numel() * ws.element_size()}")
+        if (_lib or lib()).aih_kv4_attn(
+                C.byref(self._desc), _take("q", q, nq, t, dev), _take("k_codes", k_codes, nc, u8, dev),
+                _take("k_scales", k_scales, ns, u8, dev), _take("v_codes", v_codes, nc, u8, dev),
+                _take("v_scales", v_scales, ns, u8, dev), _take("q_start", q_start, b + 1, i32, dev),
+                _take("table", table, nt, i32, dev), _take("k_len", k_len, b, i32, dev), _take("out", out, no, t, dev),
+                conv._ptr(ws) if n else None, n, conv._stream(stream)):
+            raise AihError(conv.last_error())
+        return out

@@ -89,6 +89,87 @@ typedef struct {
 int aih_mx4_pw(const aih_mx4_pw_desc *d, const void *x_codes, const void *x_scales, const void *w_codes,
                const void *w_scales, const void *bias, const void *res, void *y, aih_stream stream);
 
+/* A 4-bit cache. It holds rows of `hkv` heads of d elements in pages of `page` rows:
+ * codes [pages][hkv][page][d / 2] and scales [pages][hkv][page][d / 32] bytes, each
+ * for the keys and for the values. Row r of the cache is row r % page of page r / page.
+ *
+ * Row t of x holds hq query, hkv key and hkv value heads. Of each query and key head
+ *   y = x * rsqrt(mean(x^2) + eps) * w   when `norm` (w: wq or wk, d elements; NULL =
+ * 1), else y = x, and, for i < rot / 2 with (a, b) = (y[i], y[i + rot/2]), or (y[2i],
+ * y[2i+1]) when `pairs`, c and s = row pos[t] of the tables,
+ *   a' = a c - b s,  b' = a s + b c
+ * in fp32, every product and sum rounded by itself; dims from `rot` on are not
+ * rotated. Queries are rounded to q; keys and values (as they are in x) become row
+ * slots[t] of the cache. */
+typedef struct {
+  uint32_t tokens;    /* rows of x and q; tokens * (hq + 2 hkv) below 2^31 */
+  uint32_t hq, hkv;   /* heads; hq may be 0, hkv not */
+  uint32_t d;         /* elements of a head: a multiple of 32, at most 256 */
+  uint32_t rot;       /* rotated dims: a multiple of 16, at most d; 0 = none */
+  int32_t pairs;      /* 1 = adjacent pairs, 0 = halves */
+  int32_t norm;       /* 0 or 1 */
+  float eps;          /* >= 0, finite; with 0 a head of zeros has no norm (NaN) */
+  int32_t dt;         /* enum aih_dtype: x, wq, wk, q */
+  uint32_t positions; /* rows of the tables (used when rot > 0) */
+  uint32_t page;      /* rows of a page: a power of two, 16 to 4096 */
+  uint32_t pages;     /* pages of the cache; pages * page below 2^31 */
+  uint64_t x_stride, q_stride; /* elements, whole 16-byte units; 0 = dense */
+} aih_kv4_append_desc;
+
+/* cosines, sines [positions][rot/2] fp32; pos [tokens] int32, NULL = the token's own
+ * index (positions outside the tables use the nearest row); slots [tokens] int32,
+ * outside [0, pages * page) = the key and value are dropped. Two tokens with the same
+ * slot leave, block by block, either's. q may be x's own query heads (same pointer and
+ * row stride). */
+int aih_kv4_append(const aih_kv4_append_desc *d, const void *x, const void *wq, const void *wk, const float *cosines,
+                   const float *sines, const int32_t *pos, const int32_t *slots, void *q, void *k_codes, void *k_scales,
+                   void *v_codes, void *v_scales, aih_stream stream);
+
+/* Attention over a 4-bit cache. Sequence b has the query rows [q_start[b],
+ * q_start[b+1]); its key and value j are row j % page of page table[b][j / page], j <
+ * k_len[b]. Query head h reads key head h / (hq / hkv). With Lq queries and Lk keys,
+ * query i sees the keys j < Lk, of those only j <= i + Lk - Lq when `causal` (the
+ * queries are the last Lq positions), and none in a page outside [0, pages):
+ *   o_i = sum_j p_ij v_j / sum_j p_ij,   p_ij = exp(scale * q_i . k_j)
+ * A query that sees no key gives 0. What a query does not see never reaches its
+ * output. Keys and values are exact in the products, statistics and sums fp32; fp32
+ * queries and probabilities enter as three bf16 terms (all their bits), f16 ones as
+ * two (16 bits of a probability), bf16 probabilities are rounded to bf16 and their sum is
+ * of the rounded ones. */
+typedef struct {
+  uint32_t nseq;        /* sequences; 0 is allowed */
+  uint32_t tokens;      /* rows of q and o; tokens * hq below 2^31 */
+  uint32_t hq, hkv;     /* hq a multiple of hkv */
+  uint32_t d;           /* elements of a head: a multiple of 32, at most 256 */
+  uint32_t page, pages; /* as above */
+  uint32_t table_width; /* entries of a sequence in the table; table_width * page below 2^31 */
+  int32_t causal;       /* 0 or 1 */
+  float scale;          /* finite, 1e-20 to 1e20; 0 = 1 / sqrt(d) */
+  int32_t dt;           /* enum aih_dtype: q, o */
+  uint32_t max_len;     /* the longest k_len, as far as known (0: all that a table row holds); steers
+                           how the keys are split, results hold for any lengths */
+  uint64_t q_stride, o_stride; /* elements, whole 16-byte units; 0 = dense */
+} aih_kv4_attn_desc;
+
+typedef struct {
+  uint32_t bm;     /* (query, head of a group) rows of a workgroup's tile */
+  uint32_t parts;  /* most parts a sequence's keys are cut into */
+  uint32_t chunk;  /* keys of a part, unless more parts would be needed; 0 = not cut */
+  uint32_t grid;   /* workgroups, at most */
+  size_t ws_bytes; /* workspace: (d + 2) fp32 values for each of tokens * hq rows and each
+                      part; 0 when no row's keys are cut */
+} aih_kv4_attn_plan_info;
+
+int aih_kv4_attn_plan(const aih_kv4_attn_desc *d, aih_kv4_attn_plan_info *out);
+
+/* q_start [nseq + 1] (not descending), table [nseq][table_width], k_len [nseq]: int32
+ * device arrays; lengths past the table and starts past the tensors are cut there, and a
+ * row of o that no sequence covers is not written. ws: plan.ws_bytes of device
+ * memory (may be NULL when 0). */
+int aih_kv4_attn(const aih_kv4_attn_desc *d, const void *q, const void *k_codes, const void *k_scales,
+                 const void *v_codes, const void *v_scales, const int32_t *q_start, const int32_t *table,
+                 const int32_t *k_len, void *o, void *ws, size_t ws_bytes, aih_stream stream);
+
 #ifdef __cplusplus
 }
 #endif
