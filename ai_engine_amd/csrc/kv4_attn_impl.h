@@ -1,18 +1,26 @@
 // kv4_attn_impl.h -- attention over a 4-bit paged cache (aih_kv4_attn).
 //
-// The products, softmax and order of a tile are attn_impl.h's: S^T = K Q^T with 32
-// keys and 32 (query, head of the group) rows, O^T += V^T P^T. A code times its
-// scale has two significant bits, so it is exact in bf16, and the matrix
-// instructions run in bf16 for every type: fp32 queries and probabilities are
-// taken as three bf16 terms, which hold all their 24 bits, f16 ones as two
-// (all 11 bits of a query, 16 of a probability), whose products are summed in fp32.
+// A code times its scale has two significant bits, so keys and values are exact in
+// bf16, and the matrix instructions run in bf16 for every type: fp32 queries and
+// probabilities are taken as three bf16 terms, which hold all their 24 bits, f16
+// ones as two (all 11 bits of a query, 16 of a probability), whose products are
+// summed in fp32.
 //
-// A lane holds a key's codes as they lie in the cache: 16 bytes are one block,
-// whose elements are the operands of four products after conversion, so K goes
-// from memory to the matrix unit without LDS. V has to be transposed: its blocks
-// are converted into a bf16 tile in LDS that transposing reads take. The keys are
-// spread over the wavefronts, which run without barriers until their results are
-// joined; the next keys' codes are on their way meanwhile.
+// As in attn_impl.h the scores are S^T = K Q^T and the result O^T += V^T P^T, here
+// with 16x16x32 instructions and 16 RB (query, head of the group) rows a
+// workgroup: a single token's g rows fill most of 16, and a lane's share of the
+// softmax, which vector instructions do, is half of a 32-row tile's. A lane of a
+// score block holds keys 4 g + 0..3 (g = lane / 16) of one row, of the two blocks
+// of a step together what the second product takes as its operand.
+//
+// 16 keys are always in one page. Of them lane l holds key l % 16, and its quarter
+// g of every block's codes (or block 4 i + g of four): the order of the elements inside
+// a product is free, and the queries follow it. K goes from memory to the matrix
+// unit without LDS; V is converted into a bf16 tile in LDS that transposing reads
+// take. The keys are spread over the wavefronts, 32 a step, which run without
+// barriers until their results are joined. A step's registers are requested again
+// as soon as they are converted, so the next codes are on their way during the rest
+// of it.
 #pragma once
 
 #include "attn_impl.h"
@@ -22,22 +30,22 @@ namespace aih {
 namespace {
 
 // x as N bf16 terms that add up to it (three hold fp32's 24 bits): each takes the
-// leading bits of what is left.
+// leading bits of what is left. The last one is cut by kv_pack.
 template <int N>
 __device__ __forceinline__ void kv_terms(float x, float (&t)[N]) {
-  float rest = x;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    t[i] = __uint_as_float(__float_as_uint(rest) & 0xffff0000u);
-    rest -= t[i];
+  for (int i = 0; i < N - 1; ++i) {
+    t[i] = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+    x -= t[i];
   }
+  t[N - 1] = x;
 }
-// two bf16 of floats whose low halves do not count
+// two bf16 of floats, cut
 __device__ __forceinline__ uint32_t kv_pack(float lo, float hi) {
   return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
 }
 
-// Four dwords of bf16: eight codes times their scale.
+// Eight codes times their scale.
 __device__ __forceinline__ u32x4 kv_decode8(uint32_t c, float s) {
   return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 0)),
                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 1)),
@@ -45,66 +53,200 @@ __device__ __forceinline__ u32x4 kv_decode8(uint32_t c, float s) {
                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 3))};
 }
 
-__device__ __forceinline__ f32x16 kv_mfma(u32x4 a, u32x4 b, f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+__device__ __forceinline__ f32x4 kv_mfma(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-template <int DT_, int DP_, int WK_>
+// over the four lanes that hold a row (l % 16)
+__device__ __forceinline__ float kv_row_max(float x) {
+  x = at_pair_max(x);
+  const uint32_t u = __float_as_uint(x);
+  const auto s = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float kv_row_sum(float x) {
+  x = at_pair_sum(x);
+  const uint32_t u = __float_as_uint(x);
+  const auto s = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+
+// Heads of at most 32 NB elements, 16 RB rows, WK wavefronts.
+template <int DT_, int NB_, int RB_, int WK_>
 struct KvCfg {
-  static constexpr int DT = DT_, DP = DP_, WK = WK_;
+  static constexpr int DT = DT_, NB = NB_, RB = RB_, WK = WK_;
   static constexpr int NT = DT == DT_F32 ? 3 : DT == DT_F16 ? 2 : 1;  // terms
-  using TQ = AtTile<DT, DP>;                                          // of the queries as stored
-  using TV = AtTile<DT_BF16, DP>;                                     // of V in LDS
-  using TS = AtTile<NT == 1 ? DT_BF16 : DT_F32, DP>;                  // of the softmax
-  static constexpr int NB = DP / 32, DB = DP / 32;                    // blocks of a head
-  static constexpr int NP = NB / 2;                                   // whole blocks of a lane (half h: 2 p + h)
-  static constexpr bool ODD = NB % 2;                                 // the last one shared by the halves
-  static constexpr int NS = 2 * NB;                                   // products of 16 elements
+  static constexpr int DP = 32 * NB, TR = 16 * RB;
+  static constexpr bool EXACT = NB <= 4;                              // d is 32 NB, else it may be less
+  static constexpr int SETS = NB / 4, REST = NB % 4;                  // blocks in fours, and the others
   static constexpr int KEYS = 32 * WK;
-  static constexpr uint32_t VT = 32 * TV::RB;                         // V of a wavefront
-  // queries that the registers do not hold go to LDS
-  static constexpr bool QL = NT * DP > 384;
-  static constexpr uint32_t QB = QL ? NT * NS * 1024 : 0;
+  static constexpr int PU = NB == 1 ? 4 : NB == 2 ? 8 : NB <= 4 ? 16 : 32;  // 16-byte units of an LDS row
+  static constexpr uint32_t VT = 32 * PU * 16;                        // V of a wavefront
   static constexpr int JD = DP < 64 ? DP : 64, JP = JD + 4;           // dims of a pass of the join
-  static constexpr uint32_t JOIN = WK * 32u * JP * 4;
-  static constexpr uint32_t ML = WK * 64u * 4;
+  static constexpr uint32_t JOIN = WK * TR * JP * 4u;
+  static constexpr uint32_t ML = WK * 2u * TR * 4u;
+  // queries that the registers do not hold go to LDS
+  static constexpr bool QL = NT * NB * RB > 24;
+  static constexpr uint32_t QB = QL ? NT * NB * RB * 1024u : 0;
   static constexpr uint32_t BUF = WK * VT + QB > JOIN ? WK * VT + QB : JOIN;
   static constexpr uint32_t LDS = BUF + ML;
-  static constexpr int WPE = DP <= 128 && NT < 3 ? 2 : 1;             // wavefronts of a SIMD
   static_assert(LDS <= 160 * 1024, "LDS");
+  // registers that a wavefront cannot do without: queries, results, scores, codes
+  static constexpr int NEED = (QL ? 0 : 4 * NT * NB * RB) + 8 * NB * RB + 8 * RB + 5 * NB;
+  static constexpr int WPE = NEED <= 80 && 4 * LDS <= 160 * 1024 ? 4 : NEED <= 180 && 2 * LDS <= 160 * 1024 ? 2 : 1;
 };
 
-// The unit of 8 elements of a row that a lane half takes in product s.
+// Product s of a head's: where a lane group's eight elements are. Sets of four
+// blocks: block 4 i + g, dword s % 4 of it; of two blocks left over, block g / 2;
+// of one, dword g.
 template <class C>
-__device__ __forceinline__ uint32_t kv_unit(int s, uint32_t lh) {
-  return C::ODD && s >= 4 * C::NP ? 4 * (C::NB - 1) + 2 * lh + (s - 4 * C::NP) : 4 * (2 * (s / 4) + lh) + s % 4;
-}
-
-// The codes and scales of 32 keys on their way: of K a lane's part of key
-// lane % 32, of V block i % NB of a key for every i = lane + 64 n.
-template <class C>
-struct KvLoad {
-  static constexpr int NV = (32 * C::NB + 63) / 64;  // V blocks of a lane
-  u32x4 k[C::NP > 0 ? C::NP : 1], v[NV];
-  u32x2 ko;
-  uint32_t ks[C::NP + 1], vs[NV];
-  uint32_t seen;  // bit j: key j is there
+struct KvPlace {
+  // 16-byte unit of the values (8 elements)
+  static __device__ __forceinline__ uint32_t unit(int s, uint32_t g) {
+    if (s < 4 * C::SETS) return 4 * (4 * (s / 4) + g) + s % 4;
+    const int r = s - 4 * C::SETS;
+    if (C::REST >= 2 && r < 2) return 4 * (4 * C::SETS + (g >> 1)) + 2 * (g & 1) + r;
+    return 4 * (C::NB - 1) + g;
+  }
 };
 
-// The key and block of V that lane's n-th load is, and the LDS row and first unit
-// they go to. The lanes of a group of 16, whose stores share a cycle, take rows
-// whose swizzles differ (for 4 blocks a row).
+// The codes and scales of 16 keys, as a lane holds them.
 template <class C>
-__device__ __forceinline__ void kv_v_place(int n, uint32_t lane, uint32_t &key, uint32_t &block) {
-  const uint32_t i = lane + 64 * n;
-  block = i % C::NB;
-  key = i / C::NB;
-}
-// LDS slot of unit u of row r; as at_vswz in its high bits, which the transposing
-// reads need
+struct KvCodes {
+  u32x4 w[C::SETS > 0 ? C::SETS : 1];
+  u32x2 two;
+  uint32_t one;
+  uint32_t sw[C::SETS > 0 ? C::SETS : 1], s2, s1;
+  // codes: the first of the 16 keys' rows of d / 2 bytes, scales theirs of nb bytes
+  __device__ __forceinline__ void load(const uint8_t *codes, const uint8_t *scales, uint32_t row, uint32_t g, uint32_t nb) {
+    const uint32_t cb = C::EXACT ? C::NB * 16 : nb * 16, sb = C::EXACT ? C::NB : nb;
+    const uint32_t co = row * cb, so = row * sb;
+    auto at = [&](uint32_t b) { return C::EXACT || b < nb ? b : 0u; };  // blocks past the head: read something
+#pragma unroll
+    for (int i = 0; i < C::SETS; ++i) {
+      const uint32_t b = at(4 * i + g);
+      w[i] = *reinterpret_cast<const u32x4 *>(codes + (co + b * 16));
+      sw[i] = scales[so + b];
+    }
+    if constexpr (C::REST >= 2) {
+      const uint32_t b = at(4 * C::SETS + (g >> 1));
+      two = *reinterpret_cast<const u32x2 *>(codes + (co + b * 16 + (g & 1) * 8));
+      s2 = scales[so + b];
+    }
+    if constexpr (C::REST & 1) {
+      one = *reinterpret_cast<const uint32_t *>(codes + (co + (C::NB - 1) * 16 + g * 4));
+      s1 = scales[so + C::NB - 1];
+    }
+  }
+  // the eight codes of product s
+  __device__ __forceinline__ uint32_t code(int s) const {
+    if (s < 4 * C::SETS) return w[s / 4][s % 4];
+    const int r = s - 4 * C::SETS;
+    if (C::REST >= 2 && r < 2) return two[r];
+    return one;
+  }
+  __device__ __forceinline__ uint32_t scale(int s) const {
+    if (s < 4 * C::SETS) return sw[s / 4];
+    return C::REST >= 2 && s - 4 * C::SETS < 2 ? s2 : s1;
+  }
+  // the block of product s
+  static __device__ __forceinline__ uint32_t block(int s, uint32_t g) { return KvPlace<C>::unit(s, g) / 4; }
+  // nothing, where the key is not to count or the head has no such block
+  __device__ __forceinline__ void clear(bool all, uint32_t g, uint32_t nb) {
+#pragma unroll
+    for (int i = 0; i < C::SETS; ++i)
+      if (all || (!C::EXACT && 4 * i + g >= nb)) w[i] = u32x4{}, sw[i] = 127;
+    if constexpr (C::REST >= 2)
+      if (all || (!C::EXACT && 4 * C::SETS + (g >> 1) >= nb)) two = u32x2{}, s2 = 127;
+    if constexpr (C::REST & 1)
+      if (all) one = 0, s1 = 127;
+  }
+  __device__ __forceinline__ void clear_nan() {
+#pragma unroll
+    for (int i = 0; i < C::SETS; ++i)
+      if (sw[i] > 252) w[i] = u32x4{}, sw[i] = 127;
+    if constexpr (C::REST >= 2)
+      if (s2 > 252) two = u32x2{}, s2 = 127;
+    if constexpr (C::REST & 1)
+      if (s1 > 252) one = 0, s1 = 127;
+  }
+  // whether one of the blocks is NaN
+  __device__ __forceinline__ bool nan() const {
+    bool x = false;
+#pragma unroll
+    for (int i = 0; i < C::SETS; ++i) x |= sw[i] > 252;
+    if constexpr (C::REST >= 2) x |= s2 > 252;
+    if constexpr (C::REST & 1) x |= s1 > 252;
+    return x;
+  }
+};
+
+// LDS slot of unit u of row r: u ^ kv_swz(r). A cycle serves 256 bytes. 16 lanes store one unit of
+// 16 rows each, which land in 16 different groups of 4 banks; 32 lanes of a
+// transposing read take two units of 8 rows (r / 4 even and odd).
 template <class C>
 __device__ __forceinline__ uint32_t kv_swz(uint32_t r) {
-  return at_vswz<typename C::TV>(r);
+  if constexpr (C::PU >= 16) return (r & 3) << 2 | (r >> 1 & 2) | (r >> 3 & 1);
+  else if constexpr (C::PU == 8) return (r >> 1 & 3) << 1 | (r >> 3 & 1);
+  else return (r >> 1 & 2) | (r >> 3 & 1);
+}
+
+// Scores of 8 keys -> probabilities as the product's operands; returns their sum.
+template <int NT>
+__device__ __forceinline__ float kv_probs(const float (&s)[8], u32x4 (&pt)[NT], float off, float scale) {
+  float sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * w], scale, off));
+    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * w + 1], scale, off));
+    if constexpr (NT == 1) {
+      const uint32_t x = pack2<DT_BF16>(p0, p1);
+      pt[0][w] = x;
+      sum = at_dot_ones<DT_BF16>(x, sum);
+    } else {
+      float t0[NT], t1[NT];
+      kv_terms(p0, t0), kv_terms(p1, t1);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) pt[t][w] = kv_pack(t0[t], t1[t]);
+      sum += p0 + p1;
+    }
+  }
+  return sum;
+}
+
+// The softmax of a step: as at_settle, the maximum of a row is left as it is until
+// its probabilities add up to more than 2^15, and found then.
+template <class C>
+__device__ __forceinline__ void kv_softmax(float (&s)[8], u32x4 (&pt)[C::NT], float &m, float &l, f32x4 (&o)[2 * C::NB],
+                                           float scale) {
+#pragma clang fp contract(off)
+  float sum = kv_probs<C::NT>(s, pt, -m, scale);
+  const bool far0 = __builtin_fabsf(m) >= kAtFar, big = !(sum < kAtMost) || far0;
+  if (__any(big)) {
+    const bool row = kv_row_max(big ? 1.0f : 0.0f) != 0.0f;
+    float mx = s[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[i]);
+    mx = kv_row_max(mx) * scale;
+    const float mn = row ? fmaxf(m, mx) : m, al = __builtin_amdgcn_exp2f(m - mn);
+    m = mn;
+    l *= al;
+#pragma unroll
+    for (int i = 0; i < 2 * C::NB; ++i) o[i] *= al;
+    float off = -m;
+    const bool far = __builtin_fabsf(m) >= kAtFar;  // see at_far
+    if (__any(far)) {
+      off = far ? 0.0f : off;
+      const float inv = __builtin_amdgcn_rcpf(scale);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float at = s[i] * scale;
+        s[i] = far ? (at - m) * inv : s[i];
+      }
+    }
+    sum = kv_probs<C::NT>(s, pt, off, scale);
+  }
+  l += sum;
 }
 
 // Sequence b's rows and keys, cut to the tensors and the table.
@@ -120,13 +262,49 @@ __device__ __forceinline__ AtSeq kv_load_seq(const Kv4AttnArgs &a, uint32_t b) {
   return s;
 }
 
-template <class C, bool MANY>
+// 8 elements of a query row, unit u, as the terms of an operand.
+template <class C>
+__device__ __forceinline__ void kv_query(const AttnArgs &a, const AtQuery<AtTile<C::DT, 32>> &src, uint32_t u, u32x4 (&out)[C::NT]) {
+  constexpr int NT = C::NT;
+  if constexpr (NT == 1) {
+    out[0] = src.unit(a, u);
+  } else {
+    float f[8];
+    if constexpr (C::DT == DT_F32) {
+      const u32x4 x0 = src.unit(a, 2 * u), x1 = src.unit(a, 2 * u + 1);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(e < 4 ? x0[e] : x1[e % 4]);
+    } else {
+      const u32x4 x0 = src.unit(a, u);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = f16_to_f32((x0[e / 2] >> (16 * (e & 1))) & 0xffffu);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      float t[2][NT];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float x = f[e + i];
+        kv_terms(x, t[i]);
+        // of infinity and NaN the first term is the value and the others nothing
+        if (!(__builtin_fabsf(x) < __builtin_huge_valf())) {
+          t[i][0] = x == x ? x : __uint_as_float(0x7fc00000u);
+#pragma unroll
+          for (int k = 1; k < NT; ++k) t[i][k] = 0.0f;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < NT; ++k) out[k][e / 2] = kv_pack(t[0][k], t[1][k]);
+    }
+  }
+}
+
+// Work items: sequence by sequence (part, row tile, key head). A workgroup takes
+// every gridDim.x-th.
+template <class C>
 __global__ __launch_bounds__(64 * C::WK, C::WPE) void kv4_attn_kernel(Kv4AttnArgs ka) {
-  using TV = typename C::TV;
-  using TS = typename C::TS;
-  using TQ = typename C::TQ;
-  constexpr int WK = C::WK, DB = C::DB, NB = C::NB, NP = C::NP, NS = C::NS, NT = C::NT, DP = C::DP, EB = TQ::EB;
-  constexpr int NV = KvLoad<C>::NV;
+  constexpr int WK = C::WK, NB = C::NB, NT = C::NT, RB = C::RB, DP = C::DP, TR = C::TR;
+  constexpr uint32_t RW = C::PU * 16;  // bytes of an LDS row
   const AttnArgs &a = ka.at;
   extern __shared__ __align__(16) char lds[];
 
@@ -140,7 +318,7 @@ __global__ __launch_bounds__(64 * C::WK, C::WPE) void kv4_attn_kernel(Kv4AttnArg
   auto count = [&]() {
     mine = kv_load_seq(ka, b0 + (threadIdx.x & 63));
     if (a.sort) mine = at_sort(a, mine, threadIdx.x & 63, true);
-    tiles = (mine.lq * a.g + 31) / 32;
+    tiles = (mine.lq * a.g + TR - 1) / TR;
     const uint32_t x = at_shift(a, mine.len);
     parts = max(1u, (uint32_t)(((uint64_t)mine.len + (1ull << x) - 1) >> x));
     n = tiles * parts * a.hkv;
@@ -150,8 +328,8 @@ __global__ __launch_bounds__(64 * C::WK, C::WPE) void kv4_attn_kernel(Kv4AttnArg
 
   for (uint32_t item = blockIdx.x;; item += gridDim.x) {
     int tid = threadIdx.x;
-    if constexpr (MANY) __asm__ volatile("" : "+v"(tid));  // offsets are worked out again for every item
-    const int lane = tid & 63, l32 = lane & 31, lh = lane >> 5;
+    __asm__ volatile("" : "+v"(tid));  // offsets are worked out again for every item: they would fill the registers
+    const int lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     for (;;) {
       const uint32_t here = __builtin_amdgcn_readlane(sum, 63);
       if (item < base + here) break;
@@ -164,229 +342,203 @@ __global__ __launch_bounds__(64 * C::WK, C::WPE) void kv4_attn_kernel(Kv4AttnArg
     const AtSeq s = at_seq_of(mine, sl);
     const uint32_t nt = __builtin_amdgcn_readlane(tiles, sl), nparts = __builtin_amdgcn_readlane(parts, sl);
     const uint32_t at = item - base - (__builtin_amdgcn_readlane(sum, sl) - __builtin_amdgcn_readlane(n, sl));
-    const uint32_t rest = fdiv(at, a.by_hkv), hk = at - rest * a.hkv;
+    const uint32_t rest = __builtin_amdgcn_readfirstlane(fdiv(at, a.by_hkv)), hk = at - rest * a.hkv;
     const uint32_t part = nt == 1 ? rest : rest / nt;
     const uint32_t tile = nt - 1 - (rest - part * nt);  // the last rows see the most keys: they go first
     const uint32_t shift = at_shift(a, s.len);
-    const uint32_t nrows = s.lq * a.g, row0 = tile * 32;
+    const uint32_t nrows = s.lq * a.g, row0 = tile * TR;
     const uint32_t kbeg = part << shift;  // below len, or 0
-    const uint32_t smax = at_limit(a, a.causal, s, min(row0 + 32, nrows) - 1);
-    const uint32_t kend = (uint32_t)min((uint64_t)smax, (uint64_t)kbeg + (1ull << shift));
+    const uint32_t smax = at_limit(a, a.causal, s, min(row0 + TR, nrows) - 1);
+    const uint32_t kend = __builtin_amdgcn_readfirstlane((uint32_t)min((uint64_t)smax, (uint64_t)kbeg + (1ull << shift)));
 
     const uint32_t nb = a.d / 32, pmask = (1u << ka.pshift) - 1;
     const int32_t *table = ka.table + (uint64_t)s.k0 * ka.width;
-    // the page of the lane's key; -1: no such key
-    auto page_of = [&](uint32_t key) {
-      const uint32_t kk = key + l32;
-      const uint32_t p = (uint32_t)table[min(kk, max(kend, 1u) - 1) >> ka.pshift];
-      return kk < kend && p < ka.pages ? (int32_t)p : -1;
+    // the pages of keys key .. key + 15 and the next 16, in lanes 0 and 1
+    auto pages_of = [&](uint32_t key) { return (uint32_t)table[min(key + 16 * (lane & 1), kend - 1) >> ka.pshift]; };
+    // Which of a step's keys are there: bit j for key j.
+    auto there = [&](uint32_t key, uint32_t p0, uint32_t p1) {
+      const uint32_t left = key < kend ? min(kend - key, 32u) : 0;
+      uint32_t x = left == 32 ? 0xffffffffu : (1u << left) - 1;
+      if (p0 >= ka.pages) x &= 0xffff0000u;
+      if (p1 >= ka.pages) x &= 0x0000ffffu;
+      return x;
     };
-    // every lane loads, those without a key from the cache's first row
-    auto load = [&](KvLoad<C> &x, uint32_t key, int32_t page) {
-      x.seen = (uint32_t)__ballot(page >= 0);
-      const uint64_t row = page < 0 ? 0 : (((uint64_t)(uint32_t)page * a.hkv + hk) << ka.pshift) | ((key + l32) & pmask);
-      const uint8_t *c = ka.kc + row * (a.d / 2), *sc = ka.ks + row * nb;
-#pragma unroll
-      for (int p = 0; p < NP; ++p) {
-        const uint32_t b = 2 * p + lh, bb = DP > 128 && b >= nb ? 0 : b;
-        x.k[p] = *reinterpret_cast<const u32x4 *>(c + bb * 16);
-        x.ks[p] = sc[bb];
-      }
-      if constexpr (C::ODD) {
-        x.ko = *reinterpret_cast<const u32x2 *>(c + (NB - 1) * 16 + lh * 8);
-        x.ks[NP] = sc[NB - 1];
-      }
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        uint32_t j, b;
-        kv_v_place<C>(i, lane, j, b);
-        const bool on = (NB % 2 == 0 || j < 32) && (DP <= 128 || b < nb);
-        const int32_t vp = __shfl(page, j & 31);
-        const uint64_t vrow = vp < 0 || !on ? 0 : (((uint64_t)(uint32_t)vp * a.hkv + hk) << ka.pshift) | ((key + j) & pmask);
-        const uint32_t vb = on ? b : 0;
-        x.v[i] = *reinterpret_cast<const u32x4 *>(ka.vc + vrow * (a.d / 2) + vb * 16);
-        x.vs[i] = ka.vs[vrow * nb + vb];
-      }
+    // the first of 16 keys' rows in the cache; where there are none, the cache's own first
+    auto row_of = [&](uint32_t key, uint32_t page) -> uint64_t {
+      if (key >= kend || page >= ka.pages) return 0;
+      return (((uint64_t)page * a.hkv + hk) << ka.pshift) + (key & pmask);
+    };
+    KvCodes<C> kx[2], vx[2];
+    auto load = [&](KvCodes<C> &x, const uint8_t *codes, const uint8_t *scales, uint64_t row) {
+      x.load(codes + row * (C::EXACT ? NB * 16 : nb * 16), scales + row * (C::EXACT ? NB : nb), l16, g, nb);
     };
 
-    uint32_t key = kbeg + wave * 32;
-    KvLoad<C> cur, nxt;
-    int32_t page1 = -1;
+    uint32_t key = kbeg + wave * 32, p0 = 0xffffffffu, p1 = 0xffffffffu, pn = 0;
     if (kend > 0) {  // else there may be no cache
-      const int32_t page = page_of(key);
-      page1 = page_of(key + C::KEYS);
-      load(cur, key, page);
+      const uint32_t pv = pages_of(key);
+      pn = pages_of(key + C::KEYS);
+      p0 = __builtin_amdgcn_readlane(pv, 0), p1 = __builtin_amdgcn_readlane(pv, 1);
+      const uint64_t r0 = row_of(key, p0), r1 = row_of(key + 16, p1);
+      load(kx[0], ka.kc, ka.ks, r0), load(kx[1], ka.kc, ka.ks, r1);
+      load(vx[0], ka.vc, ka.vs, r0), load(vx[1], ka.vc, ka.vs, r1);
     }
 
-    // the queries as bf16 terms
-    u32x4 q[C::QL ? 1 : NT][C::QL ? 1 : NS];
-    const AtQuery<TQ> src(a, s, hk, row0, l32);
+    // the queries
+    u32x4 q[C::QL ? 1 : RB][C::QL ? 1 : NB][C::QL ? 1 : NT];
+    uint32_t lim[RB];
 #pragma unroll
-    for (int st = 0; st < NS; ++st) {
-      if (C::QL && st % WK != wave) continue;
-      const uint32_t u = kv_unit<C>(st, lh);
-      u32x4 out[NT];
-      if constexpr (NT == 1) {
-        out[0] = src.unit(a, u);
-      } else {
-        float f[8];
-        if constexpr (TQ::F32) {
-          const u32x4 x0 = src.unit(a, 2 * u), x1 = src.unit(a, 2 * u + 1);
+    for (int rb = 0; rb < RB; ++rb) {
+      const AtQuery<AtTile<C::DT, 32>> src(a, s, hk, row0, 16 * rb + l16);
+      lim[rb] = at_limit(a, a.causal, s, row0 + 16 * rb + l16);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(e < 4 ? x0[e] : x1[e % 4]);
-        } else {
-          const u32x4 x0 = src.unit(a, u);
+      for (int st = 0; st < NB; ++st) {
+        if (C::QL && (rb * NB + st) % WK != wave) continue;
+        u32x4 out[NT];
+        kv_query<C>(a, src, KvPlace<C>::unit(st, g), out);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] = f16_to_f32((x0[e / 2] >> (16 * (e & 1))) & 0xffffu);
+        for (int t = 0; t < NT; ++t) {
+          if constexpr (C::QL) *reinterpret_cast<u32x4 *>(ql + ((rb * NB + st) * NT + t) * 1024 + lane * 16) = out[t];
+          else q[rb][st][t] = out[t];
         }
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          float t0[NT], t1[NT];
-          kv_terms(f[e], t0), kv_terms(f[e + 1], t1);
-          // of infinity and NaN the first term is the value and the others nothing
-          const bool n0 = !(__builtin_fabsf(f[e]) < __builtin_huge_valf()), n1 = !(__builtin_fabsf(f[e + 1]) < __builtin_huge_valf());
-          if (n0) t0[0] = f[e] == f[e] ? f[e] : __uint_as_float(0x7fc00000u);
-          if (n1) t1[0] = f[e + 1] == f[e + 1] ? f[e + 1] : __uint_as_float(0x7fc00000u);
-#pragma unroll
-          for (int t = 0; t < NT; ++t) out[t][e / 2] = kv_pack(t > 0 && n0 ? 0.0f : t0[t], t > 0 && n1 ? 0.0f : t1[t]);
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        if constexpr (C::QL) *reinterpret_cast<u32x4 *>(ql + (t * NS + st) * 1024 + lane * 16) = out[t];
-        else q[t][st] = out[t];
       }
     }
     if constexpr (C::QL) __syncthreads();
-    const uint32_t lim = at_limit(a, a.causal, s, row0 + l32);
 
-    f32x16 o[DB];
-    float m = kAtLowest, l = 0.0f;
+    f32x4 o[RB][2 * NB];
+    float m[RB], l[RB];
 #pragma unroll
-    for (int db = 0; db < DB; ++db) o[db] = f32x16{};
+    for (int rb = 0; rb < RB; ++rb) {
+      m[rb] = kAtLowest, l[rb] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 2 * NB; ++i) o[rb][i] = f32x4{};
+    }
 
     for (; key < kend; key += C::KEYS) {
-      const int32_t page2 = page_of(key + 2 * C::KEYS);
-      load(nxt, key + C::KEYS, page1);
+      const uint32_t seen = there(key, p0, p1);
+      const uint32_t n0 = __builtin_amdgcn_readlane(pn, 0), n1 = __builtin_amdgcn_readlane(pn, 1);
+      const uint64_t r0 = row_of(key + C::KEYS, n0), r1 = row_of(key + C::KEYS + 16, n1);
+      pn = pages_of(key + 2 * C::KEYS);
 
       // scores
-      f32x16 sc[1];
-      sc[0] = f32x16{};
-      auto product = [&](int st, uint32_t codes, float scale) __attribute__((always_inline)) {
-        const u32x4 k = kv_decode8(codes, scale);
+      f32x4 sc[RB][2];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          u32x4 qt;
-          if constexpr (C::QL) qt = *reinterpret_cast<const u32x4 *>(ql + (t * NS + st) * 1024 + lane * 16);
-          else qt = q[t][st];
-          sc[0] = kv_mfma(k, qt, sc[0]);
+      for (int rb = 0; rb < RB; ++rb) sc[rb][0] = sc[rb][1] = f32x4{};
+      if constexpr (!C::EXACT) kx[0].clear(false, g, nb), kx[1].clear(false, g, nb);
+#pragma unroll
+      for (int st = 0; st < NB; ++st)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const u32x4 k = kv_decode8(kx[h].code(st), mx4_scale(kx[h].scale(st)));
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              u32x4 qt;
+              if constexpr (C::QL) qt = *reinterpret_cast<const u32x4 *>(ql + ((rb * NB + st) * NT + t) * 1024 + lane * 16);
+              else qt = q[rb][st][t];
+              sc[rb][h] = kv_mfma(k, qt, sc[rb][h]);
+            }
         }
-      };
+      load(kx[0], ka.kc, ka.ks, r0), load(kx[1], ka.kc, ka.ks, r1);
+
+      // the keys that this lane's rows see
+      uint32_t vis[RB];
 #pragma unroll
-      for (int p = 0; p < NP; ++p) {
-        const bool on = DP <= 128 || 2 * p + lh < nb;
-        const float scale = mx4_scale(on ? cur.ks[p] : 127u);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) product(4 * p + e, on ? cur.k[p][e] : 0u, scale);
-      }
-      if constexpr (C::ODD) {
-        const float scale = mx4_scale(cur.ks[NP]);
-        product(4 * NP, cur.ko.x, scale), product(4 * NP + 1, cur.ko.y, scale);
+      for (int rb = 0; rb < RB; ++rb) {
+        const uint32_t to = max(min(kend, lim[rb]), key) - key;
+        vis[rb] = seen & (to >= 32 ? 0xffffffffu : (1u << to) - 1);
       }
 
-      // V into LDS; blocks that are NaN as zeros, to be added to the rows that see them
-      uint64_t bad[NV];
-      bool any_bad = false;
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        uint32_t j, b;
-        kv_v_place<C>(i, lane, j, b);
-        const bool in = NB % 2 == 0 || j < 32;
-        const bool there = in && (DP <= 128 || b < nb) && (cur.seen >> (j & 31) & 1);
-        const bool nan = there && cur.vs[i] > 252;
-        bad[i] = __ballot(nan);
-        any_bad |= bad[i] != 0;
-        const bool on = there && !nan;
-        const float scale = mx4_scale(on ? cur.vs[i] : 127u);
-        if (in) {
-          char *to = vt + j * TV::RB;
-          const uint32_t sw = kv_swz<C>(j);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            *reinterpret_cast<u32x4 *>(to + ((4 * b + e) ^ sw) * 16) = kv_decode8(on ? cur.v[i][e] : 0u, scale);
-        }
-      }
-
-      // the keys that this lane's row sees
-      const uint32_t to = max(min(kend, lim), key) - key;
-      const uint32_t vis = cur.seen & (to >= 32 ? 0xffffffffu : (1u << to) - 1);
-      if (__any(vis != 0xffffffffu)) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (!(vis >> (8 * (r / 4) + r % 4 + 4 * lh) & 1)) sc[0][r] = -__builtin_huge_valf();
-      }
-      typename TS::Probs p[1];
-      at_softmax<TS>(sc, p, m, l, o, a.scale_log2);
-
-      if (any_bad) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-          for (uint64_t left = bad[i]; left; left &= left - 1) {
-            uint32_t j, b;
-            kv_v_place<C>(i, __builtin_ctzll(left), j, b);
-            const float x = vis >> j & 1 ? __uint_as_float(0x7fc00000u) : 0.0f;
-#pragma unroll
-            for (int db = 0; db < DB; ++db)
-              if (db == (int)b) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[db][r] += x;
-              }
-          }
-      }
-
-      // probabilities as bf16 terms of 16 keys each
-      u32x4 pt[NT][2];
-      if constexpr (NT == 1) {
-        pt[0][0] = p[0].h[0], pt[0][1] = p[0].h[1];
-      } else {
-#pragma unroll
-        for (int w = 0; w < 8; ++w) {
-          float t0[NT], t1[NT];
-          kv_terms(p[0][2 * w], t0), kv_terms(p[0][2 * w + 1], t1);
-#pragma unroll
-          for (int t = 0; t < NT; ++t) pt[t][w / 4][w % 4] = kv_pack(t0[t], t1[t]);
-        }
-      }
-      // O^T += V^T P^T: a transposing read has 16 lanes read 4 rows x 16 columns, 8 bytes each
-      // (row lane / 4, columns 4 (lane % 4) ..), and lane i gets column i
-      const uint32_t vr = 4 * lh + ((lane & 15) >> 2), vsw = kv_swz<C>(vr);
+      // V into LDS. Keys that are not there as zeros, and so are blocks that are NaN, which are
+      // added to the rows that see them here
 #pragma unroll
       for (int h = 0; h < 2; ++h)
+        if (!C::EXACT || seen != 0xffffffffu) vx[h].clear(!(seen >> (16 * h + l16) & 1), g, nb);
+      if (__any(vx[0].nan() || vx[1].nan())) {
 #pragma unroll
-        for (int db = 0; db < DB; ++db) {
-          const uint32_t unit = (4 * db + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ vsw;
-          const char *pv = vt + (16 * h + vr) * TV::RB + unit * 16 + (lane & 1) * 8;
-          const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_lds_s16x4 *)pv);
-          const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_lds_s16x4 *)(pv + 8 * TV::RB));
-          const u32x4 v = __builtin_bit_cast(u32x4, s16x8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]});
+        for (int h = 0; h < 2; ++h) {
+          for (uint64_t left = __ballot(vx[h].nan()); left; left &= left - 1) {
+            const int from = __builtin_ctzll(left);
+            const uint32_t kb = 1u << (16 * h + (from & 15));
 #pragma unroll
-          for (int t = 0; t < NT; ++t) o[db] = kv_mfma(v, pt[t][h], o[db]);
+            for (int st = 0; st < NB; ++st) {
+              if ((uint32_t)__builtin_amdgcn_readlane(vx[h].scale(st), from) <= 252) continue;
+              const int blk = KvCodes<C>::block(st, from >> 4);
+#pragma unroll
+              for (int b = 0; b < NB; ++b)
+                if (b == blk) {
+#pragma unroll
+                  for (int rb = 0; rb < RB; ++rb) {
+                    const float x = vis[rb] & kb ? __uint_as_float(0x7fc00000u) : 0.0f;
+                    o[rb][2 * b] += x, o[rb][2 * b + 1] += x;
+                  }
+                }
+            }
+          }
+          vx[h].clear_nan();
         }
-      cur = nxt;
-      page1 = page2;
+      }
+      const uint32_t vsw = kv_swz<C>(l16);
+#pragma unroll
+      for (int st = 0; st < NB; ++st)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          *reinterpret_cast<u32x4 *>(vt + (16 * h + l16) * RW + ((KvPlace<C>::unit(st, g) ^ vsw) * 16)) =
+              kv_decode8(vx[h].code(st), mx4_scale(vx[h].scale(st)));
+      load(vx[0], ka.vc, ka.vs, r0), load(vx[1], ka.vc, ka.vs, r1);
+
+      // the softmax; of block h this lane has keys 16 h + 4 g + 0..3
+      u32x4 pt[RB][NT];
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = sc[rb][i / 4][i % 4];
+        if (__any(vis[rb] != 0xffffffffu)) {
+          const uint32_t mine_of = vis[rb] >> (4 * g);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (!(mine_of >> (16 * (i / 4) + i % 4) & 1)) x[i] = -__builtin_huge_valf();
+        }
+        kv_softmax<C>(x, pt[rb], m[rb], l[rb], o[rb], a.scale_log2);
+      }
+
+      // O^T += V^T P^T: in a transposing read 16 lanes read 4 rows x 16 columns, 8 bytes each
+      // (row lane / 4, columns 4 (lane % 4) ..), and lane i gets column i
+      const uint32_t vr = 4 * g + (l16 >> 2), rsw = kv_swz<C>(vr);
+#pragma unroll
+      for (int i = 0; i < 2 * NB; ++i) {
+        const uint32_t unit = (2 * i + ((lane & 3) >> 1)) ^ rsw;
+        const char *pv = vt + vr * RW + unit * 16 + (lane & 1) * 8;
+        const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_lds_s16x4 *)pv);
+        const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_lds_s16x4 *)(pv + 16 * RW));
+        const u32x4 v = __builtin_bit_cast(u32x4, s16x8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]});
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+          for (int t = 0; t < NT; ++t) o[rb][i] = kv_mfma(v, pt[rb][t], o[rb][i]);
+      }
+      p0 = n0, p1 = n1;
     }
-    l = at_pair_sum(l);
 
     // join the wavefronts' keys: a common maximum, scaled sums through LDS, JD dims at a time
-    if (lh == 0) {
-      jml[wave * 64 + l32] = m;
-      jml[wave * 64 + 32 + l32] = l;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      l[rb] = kv_row_sum(l[rb]);
+      if (g == 0) {
+        jml[(2 * wave) * TR + 16 * rb + l16] = m[rb];
+        jml[(2 * wave + 1) * TR + 16 * rb + l16] = l[rb];
+      }
     }
     __syncthreads();  // and all are done with V and the queries
-    float mm = jml[l32];
+    float f[RB];
 #pragma unroll
-    for (int w = 1; w < WK; ++w) mm = fmaxf(mm, jml[w * 64 + l32]);
-    const float f = __builtin_amdgcn_exp2f(m - mm);
+    for (int rb = 0; rb < RB; ++rb) {
+      float mm = jml[16 * rb + l16];
+#pragma unroll
+      for (int w = 1; w < WK; ++w) mm = fmaxf(mm, jml[2 * w * TR + 16 * rb + l16]);
+      f[rb] = __builtin_amdgcn_exp2f(m[rb] - mm);
+    }
     float *jo = reinterpret_cast<float *>(lds);
     const uint64_t rows_all = (uint64_t)a.tokens * a.hq, ml0 = attn_ws_ml(a);
     const bool direct = !a.ws || nparts == 1;
@@ -394,26 +546,25 @@ __global__ __launch_bounds__(64 * C::WK, C::WPE) void kv4_attn_kernel(Kv4AttnArg
     for (int d0 = 0; d0 < DP; d0 += C::JD) {
       if (d0) __syncthreads();
 #pragma unroll
-      for (int db = d0 / 32; db < (d0 + C::JD) / 32 && db < DB; ++db)
+      for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4)
-          *reinterpret_cast<f32x4 *>(jo + (wave * 32 + l32) * C::JP + 32 * db - d0 + 8 * r4 + 4 * lh) =
-              f32x4{o[db][4 * r4], o[db][4 * r4 + 1], o[db][4 * r4 + 2], o[db][4 * r4 + 3]} * f;
+        for (int i = d0 / 16; i < (d0 + C::JD) / 16 && i < 2 * NB; ++i)
+          *reinterpret_cast<f32x4 *>(jo + (wave * TR + 16 * rb + l16) * C::JP + 16 * i - d0 + 4 * g) = o[rb][i] * f[rb];
       __syncthreads();
       constexpr int UR = C::JD / 8;
-      for (uint32_t i = tid; i < 32 * UR; i += 64 * WK) {
+      for (uint32_t i = tid; i < TR * UR; i += 64 * WK) {
         const uint32_t rr = i / UR, dj = (i - rr * UR) * 8, dim = d0 + dj, row = row0 + rr;
         if (row >= nrows || dim >= a.d) continue;
         f32x4 x0{}, x1{};
         float mr = jml[rr], lr = 0.0f;
 #pragma unroll
-        for (int w = 1; w < WK; ++w) mr = fmaxf(mr, jml[w * 64 + rr]);
+        for (int w = 1; w < WK; ++w) mr = fmaxf(mr, jml[2 * w * TR + rr]);
 #pragma unroll
         for (int w = 0; w < WK; ++w) {
-          const float *jp = jo + (w * 32 + rr) * C::JP + dj;
+          const float *jp = jo + (w * TR + rr) * C::JP + dj;
           x0 += *reinterpret_cast<const f32x4 *>(jp);
           x1 += *reinterpret_cast<const f32x4 *>(jp + 4);
-          lr += jml[w * 64 + 32 + rr] * __builtin_amdgcn_exp2f(jml[w * 64 + rr] - mr);
+          lr += jml[(2 * w + 1) * TR + rr] * __builtin_amdgcn_exp2f(jml[2 * w * TR + rr] - mr);
         }
         const uint32_t tok = fdiv(row, a.by_g), hd = hk * a.g + (row - tok * a.g);
         const uint64_t r0 = (uint64_t)(s.q0 + tok) * a.hq + hd;
@@ -435,61 +586,57 @@ __global__ __launch_bounds__(64 * C::WK, C::WPE) void kv4_attn_kernel(Kv4AttnArg
           const float inv = lr == 0.0f ? 0.0f : 1.0f / lr;
           x0 *= inv, x1 *= inv;
           const uint64_t e = (uint64_t)(s.q0 + tok) * a.os + (uint64_t)hd * a.d + dim;
-          if constexpr (TQ::F32) {
+          if constexpr (C::DT == DT_F32) {
             *reinterpret_cast<f32x4 *>((float *)a.o + e) = x0;
             *reinterpret_cast<f32x4 *>((float *)a.o + e + 4) = x1;
           } else {
-            const u32x2 p0 = pack4<C::DT>(x0), p1 = pack4<C::DT>(x1);
-            *reinterpret_cast<u32x4 *>((uint16_t *)a.o + e) = u32x4{p0.x, p0.y, p1.x, p1.y};
+            const u32x2 y0 = pack4<C::DT>(x0), y1 = pack4<C::DT>(x1);
+            *reinterpret_cast<u32x4 *>((uint16_t *)a.o + e) = u32x4{y0.x, y0.y, y1.x, y1.y};
           }
         }
       }
     }
-    if constexpr (!MANY) return;
     __syncthreads();  // the next item's tiles go where the results were read
   }
 }
 
-template <class C, bool MANY>
-hipError_t kv_launch_items(const Kv4AttnArgs &a, uint64_t items, uint32_t cus, hipStream_t st) {
-  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(kv4_attn_kernel<C, MANY>),
+// Items beyond the workgroups that run at once are shared by those: where keys are
+// cut, of the items that the host counts (the longest length for all) few may exist.
+template <class C>
+hipError_t kv_launch_items(const Kv4AttnArgs &a, hipStream_t st) {
+  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(kv4_attn_kernel<C>),
                                                      hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
   if (attr != hipSuccess) return attr;
-  if constexpr (MANY) {
-    // workgroups of a CU that run at once
-    static const int occ = [] {
-      int v = 0;
-      if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&v, reinterpret_cast<const void *>(kv4_attn_kernel<C, MANY>),
-                                                       64 * C::WK, C::LDS) != hipSuccess || v < 1)
-        v = 1;
-      return v;
-    }();
-    if (items > (uint64_t)cus * occ) items = (uint64_t)cus * occ;
-  }
-  hipLaunchKernelGGL((kv4_attn_kernel<C, MANY>), dim3((uint32_t)items), dim3(64 * C::WK), C::LDS, st, a);
+  static const int occ = [] {
+    int v = 0;
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&v, reinterpret_cast<const void *>(kv4_attn_kernel<C>), 64 * C::WK,
+                                                     C::LDS) != hipSuccess || v < 1)
+      v = 1;
+    return v;
+  }();
+  uint64_t items = (uint64_t)a.at.hkv * a.at.parts * a.at.tiles;
+  if (items == 0 || items > 0x7fffffffu) return hipErrorInvalidValue;
+  if (a.at.parts > 1) items = items < (uint64_t)device_cus() * occ ? items : (uint64_t)device_cus() * occ;
+  hipLaunchKernelGGL((kv4_attn_kernel<C>), dim3((uint32_t)items), dim3(64 * C::WK), C::LDS, st, a);
   return hipGetLastError();
 }
 
-// Uncut keys: one item a workgroup, handed out as others end. Cut ones: of the items
-// that the host counts (the longest length for all) few may exist, so the
-// workgroups that run at once share them.
-template <int DT, int DP>
-hipError_t kv_launch(const Kv4AttnArgs &a, hipStream_t st) {
-  using C = KvCfg<DT, DP, 4>;
-  const uint32_t cus = device_cus();
-  const uint64_t items = (uint64_t)a.at.hkv * a.at.parts * a.at.tiles;
-  if (items == 0 || items > 0x7fffffffu) return hipErrorInvalidValue;
-  if (a.at.parts > 1 && items > cus) return kv_launch_items<C, true>(a, items, cus, st);
-  return kv_launch_items<C, false>(a, items, cus, st);
+template <int DT, int RB>
+hipError_t kv_launch_rows(const Kv4AttnArgs &a, hipStream_t st) {
+  switch (a.at.d / 32) {
+    case 1: return kv_launch_items<KvCfg<DT, 1, RB, 4>>(a, st);
+    case 2: return kv_launch_items<KvCfg<DT, 2, RB, 4>>(a, st);
+    case 3: return kv_launch_items<KvCfg<DT, 3, RB, 4>>(a, st);
+    case 4: return kv_launch_items<KvCfg<DT, 4, RB, 4>>(a, st);
+    case 5:
+    case 6: return kv_launch_items<KvCfg<DT, 6, RB, 4>>(a, st);
+    default: return kv_launch_items<KvCfg<DT, 8, RB, 4>>(a, st);
+  }
 }
 
 template <int DT>
 hipError_t kv_launch_dt(const Kv4AttnArgs &a, hipStream_t st) {
-  if (a.at.d == 32) return kv_launch<DT, 32>(a, st);
-  if (a.at.d == 64) return kv_launch<DT, 64>(a, st);
-  if (a.at.d == 96) return kv_launch<DT, 96>(a, st);
-  if (a.at.d == 128) return kv_launch<DT, 128>(a, st);
-  return kv_launch<DT, 256>(a, st);
+  return a.rb == 1 ? kv_launch_rows<DT, 1>(a, st) : kv_launch_rows<DT, 2>(a, st);
 }
 
 }  // namespace

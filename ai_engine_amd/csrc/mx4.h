@@ -66,9 +66,9 @@ struct Kv4AttnArgs {
   const uint8_t *kc, *ks, *vc, *vs;
   const int32_t *table;
   uint32_t width, pages, pshift;
+  uint32_t rb;  // a tile's rows: 16 rb
 };
 
-uint32_t kv4_attn_bm();
 hipError_t launch_kv4_attn(const Kv4AttnArgs &a, int dt, hipStream_t st);
 hipError_t launch_kv4_attn_f32(const Kv4AttnArgs &a, hipStream_t st);
 hipError_t launch_kv4_attn_f16(const Kv4AttnArgs &a, hipStream_t st);

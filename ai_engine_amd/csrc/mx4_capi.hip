@@ -78,6 +78,7 @@ uint32_t log2_of(uint32_t pow2) {
 }
 
 struct Kv4Plan {
+  uint32_t rb;     // a tile's rows: 16 rb
   uint64_t tiles;  // of a key head, at most
   uint32_t parts, shift;
   uint64_t ws_floats;
@@ -97,7 +98,7 @@ int check_kv4_attn(const aih_kv4_attn_desc *d, AttnArgs *a, Kv4Plan *p) {
   if (d->scale != 0.0f && !(d->scale >= 1e-20f && d->scale <= 1e20f))
     return api_fail("aih_kv4_attn: scale must be 0 or 1e-20 to 1e20");
   *a = AttnArgs{};
-  *p = Kv4Plan{0, 1, 31, 0};
+  *p = Kv4Plan{1, 0, 1, 31, 0};
   a->nseq = d->nseq, a->tokens = d->tokens;
   a->rows = d->pages ? d->table_width * d->page : 0;  // keys of a sequence at most
   a->hq = d->hq, a->hkv = d->hkv, a->g = d->hq / d->hkv, a->d = d->d;
@@ -108,7 +109,8 @@ int check_kv4_attn(const aih_kv4_attn_desc *d, AttnArgs *a, Kv4Plan *p) {
   if (int rc = heads_stride(fn, "o_stride", d->o_stride, (uint64_t)d->hq * d->d, d->dt, &a->os)) return rc;
   if (d->nseq == 0 || d->tokens == 0) return AIH_OK;
   const uint64_t rows = (uint64_t)d->tokens * a->g;
-  const uint32_t bm = kv4_attn_bm();
+  p->rb = rows <= 16ull * d->nseq ? 1 : 2;
+  const uint32_t bm = 16 * p->rb;
   p->tiles = d->nseq == 1 ? (rows + bm - 1) / bm : rows / bm + d->nseq;
   const uint32_t len = d->max_len ? std::min(d->max_len, a->rows) : a->rows;
   auto parts = [&](uint32_t x) { return (uint32_t)std::max<uint64_t>(1, ((uint64_t)len + (1ull << x) - 1) >> x); };
@@ -126,8 +128,6 @@ int check_kv4_attn(const aih_kv4_attn_desc *d, AttnArgs *a, Kv4Plan *p) {
 }
 
 }  // namespace
-
-uint32_t kv4_attn_bm() { return 32; }
 
 hipError_t launch_kv4_attn(const Kv4AttnArgs &a, int dt, hipStream_t st) {
   return dt == DT_F32 ? launch_kv4_attn_f32(a, st) : dt == DT_F16 ? launch_kv4_attn_f16(a, st) : launch_kv4_attn_bf16(a, st);
@@ -257,7 +257,7 @@ extern "C" int aih_kv4_attn_plan(const aih_kv4_attn_desc *d, aih_kv4_attn_plan_i
     if (int rc = check_kv4_attn(d, &a, &p)) return rc;
     if (!out) return api_fail("aih_kv4_attn_plan: NULL output");
     *out = aih_kv4_attn_plan_info{};
-    out->bm = kv4_attn_bm(), out->parts = p.parts, out->chunk = p.parts > 1 ? 1u << p.shift : 0;
+    out->bm = 16 * p.rb, out->parts = p.parts, out->chunk = p.parts > 1 ? 1u << p.shift : 0;
     out->grid = (uint32_t)(p.tiles * d->hkv * p.parts);
     out->ws_bytes = p.ws_floats * 4;
     return AIH_OK;
@@ -286,9 +286,10 @@ extern "C" int aih_kv4_attn(const aih_kv4_attn_desc *d, const void *q, const voi
     t.by_g = make_fastdiv(t.g), t.by_hkv = make_fastdiv(t.hkv);
     t.tiles = (uint32_t)p.tiles, t.parts = p.parts, t.shift = p.shift, t.all_parts = p.parts;
     // prompts of different lengths start with the longest
-    t.sort = d->nseq > 1 && d->nseq <= 32 && (uint64_t)d->tokens * t.g > 32ull * d->nseq;
+    t.sort = d->nseq > 1 && d->nseq <= 32 && (uint64_t)d->tokens * t.g > 16ull * p.rb * d->nseq;
     a.kc = static_cast<const uint8_t *>(k_codes), a.ks = static_cast<const uint8_t *>(k_scales);
     a.vc = static_cast<const uint8_t *>(v_codes), a.vs = static_cast<const uint8_t *>(v_scales);
+    a.rb = p.rb;
     a.table = table, a.width = d->table_width, a.pages = d->pages, a.pshift = log2_of(d->page);
     const hipStream_t st = stream_of(stream);
     if (int rc = launched(fn, launch_kv4_attn(a, d->dt, st))) return rc;

@@ -94,7 +94,7 @@ def test_nothing_to_do():
 
 def test_plan():
     p = attn().plan()  # 128 keys at most
-    assert (p.bm, p.parts, p.chunk, p.ws_bytes) == (32, 1, 0, 0)
+    assert (p.bm, p.parts, p.chunk, p.ws_bytes) == (32, 1, 0, 0) and attn(tokens=2).plan().bm == 16
     p = attn(nseq=1, tokens=1, pages=4096, table_width=4096, page=64, hq=16, hkv=4, d=128).plan()
     assert p.parts > 1 and p.parts * p.chunk >= 4096 * 64 and p.ws_bytes == p.parts * 16 * 130 * 4
     assert p.grid == 4 * p.parts
