@@ -82,18 +82,18 @@ struct KvCfg {
   static constexpr int KEYS = 32 * WK;
   static constexpr int PU = NB == 1 ? 4 : NB == 2 ? 8 : NB <= 4 ? 16 : 32;  // 16-byte units of an LDS row
   static constexpr uint32_t VT = 32 * PU * 16;                        // V of a wavefront
-  static constexpr int JD = DP < 64 ? DP : 64, JP = JD + 4;           // dims of a pass of the join
+  static constexpr int JD = DP < 64 || RB > 2 ? 32 : 64, JP = JD + 4;  // dims of a pass of the join
   static constexpr uint32_t JOIN = WK * TR * JP * 4u;
   static constexpr uint32_t ML = WK * 2u * TR * 4u;
   // queries that the registers do not hold go to LDS
-  static constexpr bool QL = NT * NB * RB > 24;
+  static constexpr bool QL = NT * NB * RB > (RB > 2 ? 8 : 24);
   static constexpr uint32_t QB = QL ? NT * NB * RB * 1024u : 0;
   static constexpr uint32_t BUF = WK * VT + QB > JOIN ? WK * VT + QB : JOIN;
   static constexpr uint32_t LDS = BUF + ML;
   static_assert(LDS <= 160 * 1024, "LDS");
   // registers that a wavefront cannot do without: queries, results, scores, codes
   static constexpr int NEED = (QL ? 0 : 4 * NT * NB * RB) + 8 * NB * RB + 8 * RB + 5 * NB;
-  static constexpr int WPE = NEED <= 80 && 4 * LDS <= 160 * 1024 ? 4 : NEED <= 180 && 2 * LDS <= 160 * 1024 ? 2 : 1;
+  static constexpr int WPE = NEED <= 80 && 4 * LDS <= 160 * 1024 ? 4 : NEED <= 190 && 2 * LDS <= 160 * 1024 ? 2 : 1;
 };
 
 // Product s of a head's: where a lane group's eight elements are. Sets of four
@@ -636,7 +636,15 @@ hipError_t kv_launch_rows(const Kv4AttnArgs &a, hipStream_t st) {
 
 template <int DT>
 hipError_t kv_launch_dt(const Kv4AttnArgs &a, hipStream_t st) {
-  return a.rb == 1 ? kv_launch_rows<DT, 1>(a, st) : kv_launch_rows<DT, 2>(a, st);
+  if (a.rb == 1) return kv_launch_rows<DT, 1>(a, st);
+  if (a.rb == 2) return kv_launch_rows<DT, 2>(a, st);
+  switch (a.at.d / 32) {
+    case 1: return kv_launch_items<KvCfg<DT, 1, 4, 4>>(a, st);
+    case 2: return kv_launch_items<KvCfg<DT, 2, 4, 4>>(a, st);
+    case 3: return kv_launch_items<KvCfg<DT, 3, 4, 4>>(a, st);
+    case 4: return kv_launch_items<KvCfg<DT, 4, 4, 4>>(a, st);
+    default: return hipErrorInvalidValue;
+  }
 }
 
 }  // namespace

@@ -84,8 +84,14 @@ struct Kv4Plan {
   uint64_t ws_floats;
 };
 
-// How the keys are cut. A workgroup's 32 rows against all keys are a chain; cutting
-// them spreads it and costs partial results and a launch that joins them.
+// How the keys are cut. A workgroup's rows against all keys are a chain, about 0.8 us
+// for each 128; cutting it costs partial results and a launch that joins them, 4 us.
+// Measured, whole | cut to 256, 512, 1024, 2048 (32/8 heads of 128 bf16): 32 x 700 keys,
+// 8/2 heads of 64 9.0 | 11.7, 11.7 us; 1 x 4000 33 | 11.7, 12.4, 15.4, 22; 16 x 2000 22 |
+// 16.7, 15.6, 17.4; 64 of 0 to 8192 82 | 46, 38, 31.4, 37.7; 1 x 131071, 16/4 heads f16
+// 902 | 40, 28.5, 23.3, 25.2. Prompts are cut where their tiles leave CUs without one: 1024
+// tokens, 8/2 heads of 64 (256) 11.1 | 19, 16.3; 2000 tokens, 8/4 heads of 128 f16 (500) 31 to
+// 1024 45; 2 x 300 behind 4000 keys, 8/2 heads (154) 43 | 51, 43, 35.2, 35.8.
 int check_kv4_attn(const aih_kv4_attn_desc *d, AttnArgs *a, Kv4Plan *p) {
   const char *fn = "aih_kv4_attn";
   if (!d) return api_fail("aih_kv4_attn: NULL descriptor");
@@ -109,16 +115,24 @@ int check_kv4_attn(const aih_kv4_attn_desc *d, AttnArgs *a, Kv4Plan *p) {
   if (int rc = heads_stride(fn, "o_stride", d->o_stride, (uint64_t)d->hq * d->d, d->dt, &a->os)) return rc;
   if (d->nseq == 0 || d->tokens == 0) return AIH_OK;
   const uint64_t rows = (uint64_t)d->tokens * a->g;
-  p->rb = rows <= 16ull * d->nseq ? 1 : 2;
+  const uint32_t cus = device_cus();
+  // 64 rows convert the keys half as often as 32, once there are two such tiles a CU.
+  // 32 | 64, bf16: four prompts of 100 to 1024 behind 2000 keys, 32/8 heads of 128
+  // (1112 tiles of 64) 148 | 137 us, 4096 tokens (2048) 218 | 177, 4 x 500 behind 100, 16/4
+  // heads of 96 (516) 24.5 | 21.8; f16, 8 x 720, 8/2 heads of 64 (368) 31.8 | 33.9
+  const bool wide = d->d <= 128 && (rows / 64 + d->nseq / 2) * d->hkv >= 2ull * cus;
+  p->rb = rows <= 16ull * d->nseq ? 1 : wide ? 4 : 2;
   const uint32_t bm = 16 * p->rb;
   p->tiles = d->nseq == 1 ? (rows + bm - 1) / bm : rows / bm + d->nseq;
   const uint32_t len = d->max_len ? std::min(d->max_len, a->rows) : a->rows;
   auto parts = [&](uint32_t x) { return (uint32_t)std::max<uint64_t>(1, ((uint64_t)len + (1ull << x) - 1) >> x); };
   const uint64_t base = p->tiles * d->hkv;
-  const uint32_t cus = device_cus();
-  if (len > 512) {
-    if (rows <= (uint64_t)bm * d->nseq) p->shift = 10;
+  const bool few = rows <= 32ull * d->nseq;
+  if (few && len > (d->d > 128 ? 512u : 1024u)) {
+    p->shift = 10;
     while (p->shift > 8 && base * parts(p->shift) < 2ull * cus) --p->shift;
+  } else if (!few && base < cus) {
+    while (p->shift > 10 && base * parts(p->shift) < 2ull * cus) --p->shift;
   }
   p->parts = parts(p->shift);
   if (p->parts == 1) p->shift = 31;
