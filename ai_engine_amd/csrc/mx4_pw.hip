@@ -127,9 +127,13 @@ __global__ __launch_bounds__(64 * W) void mx4_pw_few_kernel(Mx4PwArgs a) {
 // ---------------------------------------------------------------- tiles
 //
 // WM x WN wavefronts of TM x TN blocks of 32 pixels x 32 channels. Stages of 128
-// elements (64 bytes a row) come into LDS by DMA, NST - 1 ahead of the products;
-// the scales of four stages (16 bytes a row) every fourth one. Unit u of tile row r
+// elements (64 bytes a row) come into LDS by DMA, up to NST of them ahead; the
+// scales of four stages (16 bytes a row) every fourth one. Unit u of tile row r
 // is at slot u ^ ((r >> 2) & 3), which spreads 16 rows' units over the banks.
+//
+// A stage is two products of 64 elements. The operands of the second are read while
+// the first runs, those of the next stage's first while the second does, so that the
+// matrix unit has a product's work in registers when the wavefronts meet.
 template <int WM_, int WN_, int TM_, int TN_, int NST_>
 struct MxTile {
   static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, NST = NST_;
@@ -138,23 +142,50 @@ struct MxTile {
   static constexpr int CI = (BM + BN) / 16;                       // DMA instructions of a stage
   static constexpr int SX = (BM + 63) / 64, SI = SX + (BN + 63) / 64;  // of four stages' scales
   static constexpr uint32_t SCALES = SI * 1024;
-  static constexpr uint32_t LDS = NST * STAGE + 2 * SCALES;
+  static constexpr int CW = TN % 2 == 0 ? 64 : 32, PITCH = CW + 4;  // channels of a staged pixel, its floats
+  static constexpr uint32_t OUT = NW * 32u * PITCH * 4u, IN = NST * STAGE + 2 * SCALES;
+  static constexpr uint32_t LDS = IN > OUT ? IN : OUT;
   static_assert(NST >= 2 && NST <= 4 && LDS <= 160 * 1024, "LDS");
 };
 
-// The products of 64 elements: `at` is where the lane's unit is in its rows.
-template <class C, int T>
-__device__ __forceinline__ void mx_step(const char *px, const char *pw, uint32_t at, f32x16 (&acc)[C::TM][C::TN],
-                                        const uint32_t (&sx)[C::TM], const uint32_t (&sn)[C::TN]) {
+// The operands of 64 elements.
+template <class C>
+struct MxOperands {
   u32x4 x[C::TM], w[C::TN];
+  // `at`: where the lane's unit is in its rows
+  __device__ __forceinline__ void read(const char *px, const char *pw, uint32_t at) {
 #pragma unroll
-  for (int i = 0; i < C::TM; ++i) x[i] = *reinterpret_cast<const u32x4 *>(px + i * 2048 + at);
+    for (int j = 0; j < C::TN; ++j) w[j] = *reinterpret_cast<const u32x4 *>(pw + j * 2048 + at);
 #pragma unroll
-  for (int j = 0; j < C::TN; ++j) w[j] = *reinterpret_cast<const u32x4 *>(pw + j * 2048 + at);
+    for (int i = 0; i < C::TM; ++i) x[i] = *reinterpret_cast<const u32x4 *>(px + i * 2048 + at);
+  }
+};
+// The scales of a stage: bytes 0 and 1 of a word are those of the two products.
+template <class C>
+struct MxScales {
+  uint32_t x[C::TM], w[C::TN];
+  __device__ __forceinline__ void read(const char *px, const char *pw) {
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) w[j] = *reinterpret_cast<const uint16_t *>(pw + j * 512);
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i) x[i] = *reinterpret_cast<const uint16_t *>(px + i * 512);
+  }
+};
+template <class C, int T>
+__device__ __forceinline__ void mx_product(const MxOperands<C> &p, const MxScales<C> &s, f32x16 (&acc)[C::TM][C::TN]) {
 #pragma unroll
   for (int i = 0; i < C::TM; ++i)
 #pragma unroll
-    for (int j = 0; j < C::TN; ++j) acc[i][j] = mx_mfma32<T>(w[j], x[i], acc[i][j], sn[j], sx[i]);
+    for (int j = 0; j < C::TN; ++j) acc[i][j] = mx_mfma32<T>(p.w[j], p.x[i], acc[i][j], s.w[j], s.x[i]);
+}
+// The scheduler's order for a product and N LDS reads: a read after each matrix instruction.
+template <class C, int N>
+__device__ __forceinline__ void mx_interleave() {
+#pragma unroll
+  for (int i = 0; i < C::TM * C::TN; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+    if (i < N) __builtin_amdgcn_sched_group_barrier(0x100, (N + C::TM * C::TN - 1) / (C::TM * C::TN), 0);
+  }
 }
 
 template <int DT, class C>
@@ -218,6 +249,12 @@ __global__ __launch_bounds__(64 * C::NW) void mx4_pw_kernel(Mx4PwArgs a) {
       else mx_dma(rwc, to + i * 1024, coff[k], s * 64);
     }
   };
+  // waits for stage s, of the stages up to `last` that are requested
+  auto arrived = [&](uint32_t s, uint32_t last) {
+    const uint32_t later = last > s ? last - s : 0;
+    const uint32_t scales = later && last / 4 != s / 4 ? ns : 0;
+    mx_wait_vm_n<CK * (NST - 1) + SK>(later * nc + scales);
+  };
 
   f32x16 acc[TM][TN];
 #pragma unroll
@@ -226,48 +263,100 @@ __global__ __launch_bounds__(64 * C::NW) void mx4_pw_kernel(Mx4PwArgs a) {
     for (int j = 0; j < TN; ++j) acc[i][j] = f32x16{};
 
   const uint32_t pr = 32 * TM * wm + l32, cr = 32 * TN * wn + l32;  // the lane's first rows
-  const uint32_t sw = (l32 >> 2) & 3;
-  auto compute = [&](uint32_t s, uint32_t buf) {
-    const char *base = lds + buf * C::STAGE;
-    // half h takes blocks 2h and 2h + 1 of the stage
-    const char *sc = lds + NST * C::STAGE + (s / 4 & 1) * C::SCALES + (s & 3) * 4 + 2 * lh;
-    uint32_t sx[TM], sn[TN];
-#pragma unroll
-    for (int i = 0; i < TM; ++i) sx[i] = *reinterpret_cast<const uint16_t *>(sc + (pr + 32 * i) * 16);
-#pragma unroll
-    for (int j = 0; j < TN; ++j) sn[j] = *reinterpret_cast<const uint16_t *>(sc + C::SX * 1024 + (cr + 32 * j) * 16);
-    mx_step<C, 0>(base + pr * 64, base + (C::BM + cr) * 64, ((2 * lh) ^ sw) * 16, acc, sx, sn);
-    mx_step<C, 1>(base + pr * 64, base + (C::BM + cr) * 64, ((2 * lh + 1) ^ sw) * 16, acc, sx, sn);
-  };
+  // half h takes blocks 2h and 2h + 1 of a stage
+  const uint32_t at0 = ((2 * lh) ^ ((l32 >> 2) & 3)) * 16, at1 = at0 ^ 16;
+  const char *px = lds + pr * 64, *pw = lds + (C::BM + cr) * 64;
+  const char *sx = lds + NST * C::STAGE + pr * 16 + 2 * lh, *sn = lds + NST * C::STAGE + C::SX * 1024 + cr * 16 + 2 * lh;
+  auto scale_at = [&](uint32_t s) { return (s / 4 & 1) * C::SCALES + (s & 3) * 4; };
 
 #pragma unroll
-  for (int s = 0; s < NST - 1; ++s)
+  for (int s = 0; s < NST; ++s)
     if ((uint32_t)s < a.nst) issue(s, s);
-  uint32_t bc = 0, bi = NST - 1;  // buffer of the stage computed / requested
+  arrived(0, min(a.nst, (uint32_t)NST) - 1);
+  // A bare barrier: a workgroup fence would wait for the copies on their way.
+  __asm__ volatile("s_barrier" ::: "memory");
+  MxOperands<C> p0, p1;
+  MxScales<C> sc, sc_next;
+  sc.read(sx, sn);
+  p0.read(px, pw, at0);
+  uint32_t buf = 0;  // stage s's
   for (uint32_t s = 0; s < a.nst; ++s) {
-    // stage s has landed once at most the copies of the stages requested after it
-    // are on their way: of one with scales among them, too
-    const uint32_t later = min(a.nst - 1 - s, (uint32_t)(NST - 2));
-    const uint32_t scales = (s + later) / 4 != s / 4 ? ns : 0;
-    mx_wait_vm_n<CK * (NST - 2) + SK>(later * nc + scales);
-    // for every wavefront, and all are done with the buffer that is requested next. A bare
-    // barrier: a workgroup fence would wait for the copies on their way
+    const uint32_t cur = buf * C::STAGE, next_buf = buf + 1 == NST ? 0 : buf + 1, next = next_buf * C::STAGE;
+    p1.read(px + cur, pw + cur, at1);
+    mx_product<C, 0>(p0, sc, acc);
+    mx_interleave<C, TM + TN>();
+    // the next stage is there for every wavefront, and all have read this one
+    arrived(s + 1, min(a.nst - 1, s + NST - 1));
     __asm__ volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (s + NST - 1 < a.nst) issue(s + NST - 1, bi);
-    compute(s, bc);
-    bc = bc + 1 == NST ? 0 : bc + 1;
-    bi = bi + 1 == NST ? 0 : bi + 1;
+    if (s + NST < a.nst) issue(s + NST, buf);
+    sc_next.read(sx + scale_at(s + 1), sn + scale_at(s + 1));  // behind the last stage: something, and not used
+    p0.read(px + next, pw + next, at0);
+    mx_product<C, 1>(p1, sc, acc);
+    mx_interleave<C, 2 * (TM + TN)>();
+    sc = sc_next;
+    buf = next_buf;
   }
+  __syncthreads();  // the buffers become the wavefronts' staging rows
 
+  // act(acc + bias) + res, whole runs of a pixel's channels
   const Act act = act_params(a.act);
+  constexpr bool F32 = DT == DT_F32;
+  constexpr int CW = C::CW, PITCH = C::PITCH, CB = CW / 32;
+  constexpr int CPL = F32 ? 4 : 8, LPR = CW / CPL, PPI = 64 / LPR;  // channels of a lane, lanes of a pixel, pixels at once
+  float *st = reinterpret_cast<float *>(lds) + wave * 32 * PITCH;
+  const bool row16 = F32 || a.cout % 8 == 0;  // 16-byte runs stay aligned from pixel to pixel
+  const uint32_t rl = lane / LPR, cl = (lane % LPR) * CPL;
 #pragma unroll
-  for (int i = 0; i < TM; ++i)
+  for (int j0 = 0; j0 < TN; j0 += CB) {
+    const uint32_t n = n0 + 32 * (TN * wn + j0) + cl;
+    const bool n_ok = n < a.cout, two = !F32 && n + 8 <= a.cout;
+    const f32x4 b0 = a.bias && n_ok ? Vec4IO<DT>::load(a.bias, n / 4) : f32x4{};
+    const f32x4 b1 = a.bias && two ? Vec4IO<DT>::load(a.bias, n / 4 + 1) : f32x4{};
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
+    for (int i = 0; i < TM; ++i) {
 #pragma unroll
-      for (int r4 = 0; r4 < 4; ++r4)
-        mx_store4<DT>(a, act, m0 + pr + 32 * i, n0 + 32 * TN * wn + 32 * j + 8 * r4 + 4 * lh,
-                      f32x4{acc[i][j][4 * r4], acc[i][j][4 * r4 + 1], acc[i][j][4 * r4 + 2], acc[i][j][4 * r4 + 3]});
+      for (int j = 0; j < CB; ++j)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4)
+          *reinterpret_cast<f32x4 *>(st + l32 * PITCH + 32 * j + 8 * r4 + 4 * lh) =
+              f32x4{acc[i][j0 + j][4 * r4], acc[i][j0 + j][4 * r4 + 1], acc[i][j0 + j][4 * r4 + 2], acc[i][j0 + j][4 * r4 + 3]};
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll 2
+      for (int g = 0; g < 32 / PPI; ++g) {
+        const uint32_t r = g * PPI + rl, m = m0 + 32 * (TM * wm + i) + r;
+        if (m >= a.m || !n_ok) continue;
+        const size_t vi = (size_t)m * (a.cout / 4) + n / 4;
+        f32x4 v0 = *reinterpret_cast<const f32x4 *>(st + r * PITCH + cl) + b0;
+        if constexpr (F32) {
+          v0 = act4(act, v0);
+          if (a.res) v0 += reinterpret_cast<const f32x4 *>(a.res)[vi];
+          reinterpret_cast<f32x4 *>(a.y)[vi] = v0;
+        } else {
+          f32x4 v1 = *reinterpret_cast<const f32x4 *>(st + r * PITCH + cl + 4) + b1;
+          float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+          act_array<8>(act, v);
+          v0 = f32x4{v[0], v[1], v[2], v[3]}, v1 = f32x4{v[4], v[5], v[6], v[7]};
+          if (a.res) {
+            if (row16) {
+              const u32x4 x = reinterpret_cast<const u32x4 *>(a.res)[vi / 2];
+              v0 += unpack4<DT>(u32x2{x.x, x.y}), v1 += unpack4<DT>(u32x2{x.z, x.w});
+            } else {
+              v0 += Vec4IO<DT>::load(a.res, vi);
+              if (two) v1 += Vec4IO<DT>::load(a.res, vi + 1);
+            }
+          }
+          const u32x2 lo = pack4<DT>(v0), hi = pack4<DT>(v1);
+          if (row16) {
+            reinterpret_cast<u32x4 *>(a.y)[vi / 2] = u32x4{lo.x, lo.y, hi.x, hi.y};
+          } else {
+            reinterpret_cast<u32x2 *>(a.y)[vi] = lo;
+            if (two) reinterpret_cast<u32x2 *>(a.y)[vi + 1] = hi;
+          }
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
 }
 
 template <int DT, class C>
@@ -294,6 +383,23 @@ hipError_t launch_dt(const Mx4PwArgs &a, hipStream_t st) {
   if (a.m <= 16) return launch_few<DT, 1>(a, st);
   if (a.m <= 32) return launch_few<DT, 2>(a, st);
   if (a.m <= 64) return launch_few<DT, 4>(a, st);
+#ifdef MX_ENV
+  if (const char *e = getenv("MX_TILE")) switch (atoi(e)) {
+    case 0: return launch_tile<DT, MxTile<2, 4, 4, 2, 3>>(a, st);
+    case 1: return launch_tile<DT, MxTile<2, 2, 2, 2, 3>>(a, st);
+    case 2: return launch_tile<DT, MxTile<2, 2, 1, 1, 4>>(a, st);
+    case 3: return launch_tile<DT, MxTile<4, 1, 1, 5, 3>>(a, st);
+    case 4: return launch_tile<DT, MxTile<2, 1, 1, 5, 3>>(a, st);
+    case 5: return launch_tile<DT, MxTile<2, 2, 4, 4, 3>>(a, st);
+    case 6: return launch_tile<DT, MxTile<2, 4, 4, 2, 4>>(a, st);
+    case 7: return launch_tile<DT, MxTile<2, 2, 4, 2, 3>>(a, st);
+    case 8: return launch_tile<DT, MxTile<4, 2, 1, 2, 3>>(a, st);
+    case 9: return launch_tile<DT, MxTile<2, 2, 1, 2, 3>>(a, st);
+    case 10: return launch_tile<DT, MxTile<4, 1, 1, 1, 4>>(a, st);
+    case 11: return launch_tile<DT, MxTile<2, 2, 2, 2, 2>>(a, st);
+    case 12: return launch_tile<DT, MxTile<2, 4, 4, 2, 2>>(a, st);
+  }
+#endif
   const uint64_t big = (uint64_t)((a.m + 255) / 256) * ((a.cout + 255) / 256);
   const uint64_t mid = (uint64_t)((a.m + 127) / 128) * ((a.cout + 127) / 128);
   const uint32_t cus = device_cus();
