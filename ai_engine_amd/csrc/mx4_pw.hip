@@ -8,6 +8,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "aih_device.h"
 #include "mx4.h"
@@ -74,8 +75,8 @@ __device__ __forceinline__ void mx_store4(const Mx4PwArgs &a, const Act &act, ui
 
 // ---------------------------------------------------------------- few pixels
 //
-// Up to 64 pixels: bound by the weights' bytes (or, with few of those, by one chain of
-// loads, products and the join). A workgroup owns 16 channels, its W
+// Up to 32 pixels: bound by the weights' bytes (16 x 8192 x 8192 17 us, 2.1 TB/s) or, with
+// few of those, by one chain of loads, products and the join (8 x 4096 x 4096 5.6 us). A workgroup owns 16 channels, its W
 // wavefronts take turns at the stages of 128 elements, operands straight into registers
 // (a lane: channel lane % 16, block lane / 16 of the stage, 64 contiguous bytes a row),
 // and the partial sums are joined in LDS in the wavefronts' order.
@@ -126,27 +127,38 @@ __global__ __launch_bounds__(64 * W) void mx4_pw_few_kernel(Mx4PwArgs a) {
 
 // ---------------------------------------------------------------- tiles
 //
-// WM x WN wavefronts of TM x TN blocks of 32 pixels x 32 channels. Stages of 128
-// elements (64 bytes a row) come into LDS by DMA, up to NST of them ahead; the
-// scales of four stages (16 bytes a row) every fourth one. Unit u of tile row r
-// is at slot u ^ ((r >> 2) & 3), which spreads 16 rows' units over the banks.
+// WM x WN wavefronts of TM x TN blocks of 32 pixels x 32 channels. Stages of U
+// blocks of 32 elements (16 U bytes a row; 8 are a whole cache line) come into LDS by
+// DMA, up to NST of them ahead; the scales of 16 blocks a row with every 16 / U-th
+// one. Unit u of tile row r is at slot u ^ mx_swz(r), which spreads 16 rows' units over
+// the banks.
 //
-// A stage is two products of 64 elements. The operands of the second are read while
-// the first runs, those of the next stage's first while the second does, so that the
-// matrix unit has a product's work in registers when the wavefronts meet.
-template <int WM_, int WN_, int TM_, int TN_, int NST_>
+// A stage is U / 2 products of 64 elements. The operands of each are read while the
+// one before it runs, those of the next stage's first too, so that the matrix unit has a
+// product's work in registers when the wavefronts meet. 8192 cubed takes 285 us, 3.85
+// PFLOP/s, where the matrix unit alone reaches 7.1; without the copies it took 230, without
+// the products 236: both pipes are busy most of the time. With the products of a stage
+// behind its barrier, and half a cache line a row, it took 353.
+template <int WM_, int WN_, int TM_, int TN_, int NST_, int U_>
 struct MxTile {
-  static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, NST = NST_;
+  static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, NST = NST_, U = U_;
   static constexpr int NW = WM * WN, BM = 32 * WM * TM, BN = 32 * WN * TN;
-  static constexpr uint32_t STAGE = (BM + BN) * 64;
-  static constexpr int CI = (BM + BN) / 16;                       // DMA instructions of a stage
-  static constexpr int SX = (BM + 63) / 64, SI = SX + (BN + 63) / 64;  // of four stages' scales
+  static constexpr int RB = 16 * U, RPI = 64 / U;                 // bytes of a row, rows of a DMA instruction
+  static constexpr uint32_t STAGE = (BM + BN) * RB;
+  static constexpr int CX = BM / RPI, CI = CX + BN / RPI;         // DMA instructions of a stage
+  static constexpr int G = 16 / U;                                // stages of a group of scales
+  static constexpr int SX = (BM + 63) / 64, SI = SX + (BN + 63) / 64;
   static constexpr uint32_t SCALES = SI * 1024;
   static constexpr int CW = TN % 2 == 0 ? 64 : 32, PITCH = CW + 4;  // channels of a staged pixel, its floats
   static constexpr uint32_t OUT = NW * 32u * PITCH * 4u, IN = NST * STAGE + 2 * SCALES;
   static constexpr uint32_t LDS = IN > OUT ? IN : OUT;
-  static_assert(NST >= 2 && NST <= 4 && LDS <= 160 * 1024, "LDS");
+  // two groups of scales at a time
+  static_assert((U == 4 || U == 8) && NST >= 2 && NST <= G && LDS <= 160 * 1024, "LDS");
 };
+template <class C>
+__device__ __forceinline__ uint32_t mx_swz(uint32_t r) {
+  return C::U == 4 ? (r >> 2) & 3 : (r >> 1) & 7;
+}
 
 // The operands of 64 elements.
 template <class C>
@@ -155,20 +167,27 @@ struct MxOperands {
   // `at`: where the lane's unit is in its rows
   __device__ __forceinline__ void read(const char *px, const char *pw, uint32_t at) {
 #pragma unroll
-    for (int j = 0; j < C::TN; ++j) w[j] = *reinterpret_cast<const u32x4 *>(pw + j * 2048 + at);
+    for (int j = 0; j < C::TN; ++j) w[j] = *reinterpret_cast<const u32x4 *>(pw + j * 32 * C::RB + at);
 #pragma unroll
-    for (int i = 0; i < C::TM; ++i) x[i] = *reinterpret_cast<const u32x4 *>(px + i * 2048 + at);
+    for (int i = 0; i < C::TM; ++i) x[i] = *reinterpret_cast<const u32x4 *>(px + i * 32 * C::RB + at);
   }
 };
-// The scales of a stage: bytes 0 and 1 of a word are those of the two products.
+// The scales of a stage: byte T of a word is that of product T.
 template <class C>
 struct MxScales {
   uint32_t x[C::TM], w[C::TN];
+  using Word = std::conditional_t<C::U == 4, uint16_t, uint32_t>;
   __device__ __forceinline__ void read(const char *px, const char *pw) {
 #pragma unroll
-    for (int j = 0; j < C::TN; ++j) w[j] = *reinterpret_cast<const uint16_t *>(pw + j * 512);
+    for (int j = 0; j < C::TN; ++j) w[j] = *reinterpret_cast<const Word *>(pw + j * 512);
 #pragma unroll
-    for (int i = 0; i < C::TM; ++i) x[i] = *reinterpret_cast<const uint16_t *>(px + i * 512);
+    for (int i = 0; i < C::TM; ++i) x[i] = *reinterpret_cast<const Word *>(px + i * 512);
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) w[j] = 0;
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i) x[i] = 0;
   }
 };
 template <class C, int T>
@@ -178,18 +197,18 @@ __device__ __forceinline__ void mx_product(const MxOperands<C> &p, const MxScale
 #pragma unroll
     for (int j = 0; j < C::TN; ++j) acc[i][j] = mx_mfma32<T>(p.w[j], p.x[i], acc[i][j], s.w[j], s.x[i]);
 }
-// The scheduler's order for a product and N LDS reads: a read after each matrix instruction.
-template <class C, int N>
-__device__ __forceinline__ void mx_interleave() {
+// Products are no memory accesses, and the compiler moves them down, past the barrier
+// and the next reads; an empty text that takes the sums keeps them here.
+template <class C>
+__device__ __forceinline__ void mx_pin(f32x16 (&acc)[C::TM][C::TN]) {
 #pragma unroll
-  for (int i = 0; i < C::TM * C::TN; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-    if (i < N) __builtin_amdgcn_sched_group_barrier(0x100, (N + C::TM * C::TN - 1) / (C::TM * C::TN), 0);
-  }
+  for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) __asm__ volatile("" : "+v"(acc[i][j])::"memory");
 }
 
 template <int DT, class C>
-__global__ __launch_bounds__(64 * C::NW) void mx4_pw_kernel(Mx4PwArgs a) {
+__global__ __launch_bounds__(64 * C::NW, 2) void mx4_pw_kernel(Mx4PwArgs a) {
   constexpr int TM = C::TM, TN = C::TN, NW = C::NW, NST = C::NST;
   constexpr int CK = (C::CI + NW - 1) / NW, SK = (C::SI + NW - 1) / NW;
   extern __shared__ __align__(16) char lds[];
@@ -209,15 +228,20 @@ __global__ __launch_bounds__(64 * C::NW) void mx4_pw_kernel(Mx4PwArgs a) {
   const __amdgpu_buffer_rsrc_t rxs = mx_rsrc(a.xs + (uint64_t)m0 * a.sb, mr * a.sb);
   const __amdgpu_buffer_rsrc_t rws = mx_rsrc(a.ws + (uint64_t)n0 * a.sb, nr * a.sb);
 
-  // instruction i of a stage: tile rows 16 i + lane / 4 (pixels, then channels)
-  const uint32_t cu = (uint32_t)(lane & 3) ^ ((lane >> 4) & 3);
+  // Instruction i of a stage: tile rows RPI i + lane / U (pixels, then channels).
+  // The last stage may be half a one.
   uint32_t coff[CK];
+  bool past[CK];  // the unit is in the second half
 #pragma unroll
   for (int k = 0; k < CK; ++k) {
     const int i = wave + k * NW;
-    const uint32_t r = (i < C::BM / 16 ? 16 * i : 16 * i - C::BM) + lane / 4;
-    coff[k] = r < (i < C::BM / 16 ? mr : nr) ? r * a.cb + cu * 16 : kOob;
+    const uint32_t r = (i < C::CX ? C::RPI * i : C::RPI * (i - C::CX)) + lane / C::U;
+    const uint32_t u = (uint32_t)(lane % C::U) ^ mx_swz<C>(r);
+    coff[k] = r < (i < C::CX ? mr : nr) ? r * a.cb + u * 16 : kOob;
+    past[k] = u >= 4;
   }
+  const uint32_t nst = C::U == 4 ? a.nst : (a.nst + 1) / 2;
+  const bool odd = C::U == 8 && (a.nst & 1);
   uint32_t soff[SK];
 #pragma unroll
   for (int k = 0; k < SK; ++k) {
@@ -230,14 +254,14 @@ __global__ __launch_bounds__(64 * C::NW) void mx4_pw_kernel(Mx4PwArgs a) {
 
   // requests stage s; stages are requested in order
   auto issue = [&](uint32_t s, uint32_t buf) {
-    if (s % 4 == 0) {
-      char *to = lds + NST * C::STAGE + (s / 4 & 1) * C::SCALES;
+    if (s % C::G == 0) {
+      char *to = lds + NST * C::STAGE + (s / C::G & 1) * C::SCALES;
 #pragma unroll
       for (int k = 0; k < SK; ++k) {
         const int i = wave + k * NW;
         if (C::SI % NW != 0 && i >= C::SI) break;
-        if (i < C::SX) mx_dma(rxs, to + i * 1024, soff[k], s * 4);
-        else mx_dma(rws, to + i * 1024, soff[k], s * 4);
+        if (i < C::SX) mx_dma(rxs, to + i * 1024, soff[k], s * C::U);
+        else mx_dma(rws, to + i * 1024, soff[k], s * C::U);
       }
     }
     char *to = lds + buf * C::STAGE;
@@ -245,14 +269,15 @@ __global__ __launch_bounds__(64 * C::NW) void mx4_pw_kernel(Mx4PwArgs a) {
     for (int k = 0; k < CK; ++k) {
       const int i = wave + k * NW;
       if (C::CI % NW != 0 && i >= C::CI) break;
-      if (i < C::BM / 16) mx_dma(rxc, to + i * 1024, coff[k], s * 64);
-      else mx_dma(rwc, to + i * 1024, coff[k], s * 64);
+      const uint32_t off = odd && s == nst - 1 && past[k] ? kOob : coff[k];
+      if (i < C::CX) mx_dma(rxc, to + i * 1024, off, s * C::RB);
+      else mx_dma(rwc, to + i * 1024, off, s * C::RB);
     }
   };
   // waits for stage s, of the stages up to `last` that are requested
   auto arrived = [&](uint32_t s, uint32_t last) {
     const uint32_t later = last > s ? last - s : 0;
-    const uint32_t scales = later && last / 4 != s / 4 ? ns : 0;
+    const uint32_t scales = later && last / C::G != s / C::G ? ns : 0;
     mx_wait_vm_n<CK * (NST - 1) + SK>(later * nc + scales);
   };
 
@@ -263,37 +288,51 @@ __global__ __launch_bounds__(64 * C::NW) void mx4_pw_kernel(Mx4PwArgs a) {
     for (int j = 0; j < TN; ++j) acc[i][j] = f32x16{};
 
   const uint32_t pr = 32 * TM * wm + l32, cr = 32 * TN * wn + l32;  // the lane's first rows
-  // half h takes blocks 2h and 2h + 1 of a stage
-  const uint32_t at0 = ((2 * lh) ^ ((l32 >> 2) & 3)) * 16, at1 = at0 ^ 16;
-  const char *px = lds + pr * 64, *pw = lds + (C::BM + cr) * 64;
-  const char *sx = lds + NST * C::STAGE + pr * 16 + 2 * lh, *sn = lds + NST * C::STAGE + C::SX * 1024 + cr * 16 + 2 * lh;
-  auto scale_at = [&](uint32_t s) { return (s / 4 & 1) * C::SCALES + (s & 3) * 4; };
+  // half h takes blocks h U / 2 .. of a stage, one a product
+  constexpr int NP = C::U / 2;
+  uint32_t at[NP];
+#pragma unroll
+  for (int T = 0; T < NP; ++T) at[T] = ((NP * lh + T) ^ mx_swz<C>(l32)) * 16;
+  const char *px = lds + pr * C::RB, *pw = lds + (C::BM + cr) * C::RB;
+  const char *sx = lds + NST * C::STAGE + pr * 16 + NP * lh;
+  const char *sn = lds + NST * C::STAGE + C::SX * 1024 + cr * 16 + NP * lh;
+  auto scale_at = [&](uint32_t s) { return (s / C::G & 1) * C::SCALES + (s % C::G) * C::U; };
 
 #pragma unroll
   for (int s = 0; s < NST; ++s)
-    if ((uint32_t)s < a.nst) issue(s, s);
-  arrived(0, min(a.nst, (uint32_t)NST) - 1);
+    if ((uint32_t)s < nst) issue(s, s);
+  arrived(0, min(nst, (uint32_t)NST) - 1);
   // A bare barrier: a workgroup fence would wait for the copies on their way.
   __asm__ volatile("s_barrier" ::: "memory");
-  MxOperands<C> p0, p1;
+  MxOperands<C> p[2];
   MxScales<C> sc, sc_next;
   sc.read(sx, sn);
-  p0.read(px, pw, at0);
+  if (odd && nst == 1 && lh) sc.clear();  // no scales: whatever is behind the row's
+  p[0].read(px, pw, at[0]);
   uint32_t buf = 0;  // stage s's
-  for (uint32_t s = 0; s < a.nst; ++s) {
+  for (uint32_t s = 0; s < nst; ++s) {
     const uint32_t cur = buf * C::STAGE, next_buf = buf + 1 == NST ? 0 : buf + 1, next = next_buf * C::STAGE;
-    p1.read(px + cur, pw + cur, at1);
-    mx_product<C, 0>(p0, sc, acc);
-    mx_interleave<C, TM + TN>();
+    p[1].read(px + cur, pw + cur, at[1]);
+    mx_product<C, 0>(p[0], sc, acc);
+    mx_pin<C>(acc);
+    if constexpr (C::U == 8) {
+      p[0].read(px + cur, pw + cur, at[NP - 2]);
+      mx_product<C, 1>(p[1], sc, acc);
+      mx_pin<C>(acc);
+      p[1].read(px + cur, pw + cur, at[NP - 1]);
+      mx_product<C, NP - 2>(p[0], sc, acc);
+      mx_pin<C>(acc);
+    }
     // the next stage is there for every wavefront, and all have read this one
-    arrived(s + 1, min(a.nst - 1, s + NST - 1));
+    arrived(s + 1, min(nst - 1, s + NST - 1));
     __asm__ volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (s + NST < a.nst) issue(s + NST, buf);
+    if (s + NST < nst) issue(s + NST, buf);
     sc_next.read(sx + scale_at(s + 1), sn + scale_at(s + 1));  // behind the last stage: something, and not used
-    p0.read(px + next, pw + next, at0);
-    mx_product<C, 1>(p1, sc, acc);
-    mx_interleave<C, 2 * (TM + TN)>();
+    p[0].read(px + next, pw + next, at[0]);
+    mx_product<C, NP - 1>(p[1], sc, acc);
+    mx_pin<C>(acc);
     sc = sc_next;
+    if (odd && s + 2 == nst && lh) sc.clear();
     buf = next_buf;
   }
   __syncthreads();  // the buffers become the wavefronts' staging rows
@@ -378,34 +417,30 @@ hipError_t launch_few(const Mx4PwArgs &a, hipStream_t st) {
   return hipGetLastError();
 }
 
+// Measured, bf16, us: 8192 cubed with tiles of 256 x 256 289, 128 x 128 356, 64 x 128 483;
+// 4096 cubed 40.6 | 48 | 63; 2048 cubed 20 | 12.0 | 11.0, 64 x 64 12.0; 1024 x 4096 x 4096 32 |
+// 17.9 | 17.7 | 20.1; 3000 x 4096 x 4096 34.8 | 39 | 48; 5000 x 8192 x 1000 54 | 39 | 48; 300 x
+// 4096 x 4096 31 | 15.5 | 13.0 | 11.6. A short sum gives little
+// to overlap within a workgroup, so stages are half as long and more workgroups
+// share a CU: 46080 x 960 x 160 with a residual, 128 x 128, long and short stages 23.0
+// | 17.4, 46080 x 192 x 768 28.4 | 21.4, 184320 x 64 x 64, 64 x 64, 12.8 | 9.8. Few pixels,
+// split over wavefronts | tiles of 64 x 64: 8 x 4096 x 4096 6.3 | 7.9, 20 6.5 | 8.2, 48 10.0 | 8.6.
 template <int DT>
 hipError_t launch_dt(const Mx4PwArgs &a, hipStream_t st) {
   if (a.m <= 16) return launch_few<DT, 1>(a, st);
   if (a.m <= 32) return launch_few<DT, 2>(a, st);
-  if (a.m <= 64) return launch_few<DT, 4>(a, st);
-#ifdef MX_ENV
-  if (const char *e = getenv("MX_TILE")) switch (atoi(e)) {
-    case 0: return launch_tile<DT, MxTile<2, 4, 4, 2, 3>>(a, st);
-    case 1: return launch_tile<DT, MxTile<2, 2, 2, 2, 3>>(a, st);
-    case 2: return launch_tile<DT, MxTile<2, 2, 1, 1, 4>>(a, st);
-    case 3: return launch_tile<DT, MxTile<4, 1, 1, 5, 3>>(a, st);
-    case 4: return launch_tile<DT, MxTile<2, 1, 1, 5, 3>>(a, st);
-    case 5: return launch_tile<DT, MxTile<2, 2, 4, 4, 3>>(a, st);
-    case 6: return launch_tile<DT, MxTile<2, 4, 4, 2, 4>>(a, st);
-    case 7: return launch_tile<DT, MxTile<2, 2, 4, 2, 3>>(a, st);
-    case 8: return launch_tile<DT, MxTile<4, 2, 1, 2, 3>>(a, st);
-    case 9: return launch_tile<DT, MxTile<2, 2, 1, 2, 3>>(a, st);
-    case 10: return launch_tile<DT, MxTile<4, 1, 1, 1, 4>>(a, st);
-    case 11: return launch_tile<DT, MxTile<2, 2, 2, 2, 2>>(a, st);
-    case 12: return launch_tile<DT, MxTile<2, 4, 4, 2, 2>>(a, st);
+  auto tiles = [&](uint32_t bm, uint32_t bn) { return (uint64_t)((a.m + bm - 1) / bm) * ((a.cout + bn - 1) / bn); };
+  const uint64_t cus = device_cus(), big = tiles(256, 256), mid = tiles(128, 128);
+  if (a.nst < 16) {
+    if (a.cout > 64 && mid >= cus) return launch_tile<DT, MxTile<2, 2, 2, 2, 2, 4>>(a, st);
+    return launch_tile<DT, MxTile<2, 2, 1, 1, 2, 4>>(a, st);
   }
-#endif
-  const uint64_t big = (uint64_t)((a.m + 255) / 256) * ((a.cout + 255) / 256);
-  const uint64_t mid = (uint64_t)((a.m + 127) / 128) * ((a.cout + 127) / 128);
-  const uint32_t cus = device_cus();
-  if (big >= cus) return launch_tile<DT, MxTile<2, 4, 4, 2, 3>>(a, st);
-  if (mid >= cus) return launch_tile<DT, MxTile<2, 2, 2, 2, 3>>(a, st);
-  return launch_tile<DT, MxTile<2, 2, 1, 1, 4>>(a, st);
+  // rounds of tiles; one of 128 x 128, two a CU, takes 0.6 of one of 256 x 256
+  const uint64_t big_rounds = (big + cus - 1) / cus, mid_rounds = (mid + 2 * cus - 1) / (2 * cus);
+  if (10 * big_rounds <= 6 * mid_rounds) return launch_tile<DT, MxTile<2, 4, 4, 2, 2, 8>>(a, st);
+  if (mid > cus) return launch_tile<DT, MxTile<2, 2, 2, 2, 2, 8>>(a, st);
+  if (tiles(64, 128) >= cus) return launch_tile<DT, MxTile<2, 2, 1, 2, 2, 8>>(a, st);
+  return launch_tile<DT, MxTile<2, 2, 1, 1, 2, 8>>(a, st);
 }
 
 }  // namespace
