@@ -85,26 +85,25 @@ def lib() -> C.CDLL:
     return _lib
 
 
-_torch = None  # torch's Tensor, current device, and the types of DType, codes and index arrays
+_torch = None  # torch's Tensor, current device and its current stream, and the types of DType, codes and index arrays
 
 
 def _torch_types():
     global _torch
     import torch
 
-    _torch = (torch.Tensor, torch.cuda.current_device, {0: torch.float32, 1: torch.float16, 2: torch.bfloat16},
-              torch.uint8, torch.int32)
+    _torch = (torch.Tensor, torch.cuda.current_device, torch._C._cuda_getCurrentRawStream,
+              {0: torch.float32, 1: torch.float16, 2: torch.bfloat16}, torch.uint8, torch.int32)
     return _torch
 
 
-def _take(name, t, n, dtype, device):
+def _take(name, t, n, dtype):
     """The device address of `n` values; refuses a tensor that the kernels would read as other values, past its end
-    or on another device. None and raw addresses are the caller's, as everywhere."""
+    or on another device. None and raw addresses are the caller's, as everywhere. `run` asks the same in line
+    first, at half the time: a call costs as much as its launch."""
     if t is None or t.__class__ is int:
         return t
-    if device is None:  # the call's other tensors are raw addresses
-        device = _torch[1]()
-    if t.dtype is dtype and t.get_device() == device and t.is_contiguous() and t.numel() >= n:
+    if t.dtype is dtype and t.is_cuda and t.get_device() == _torch[1]() and t.is_contiguous() and t.numel() >= n:
         return t.data_ptr()
     raise AihError(f"{name} must be a dense tensor of at least {n} {dtype} on the current device, not {tuple(t.shape)} "
                    f"{t.dtype} on {t.device}" + ("" if t.is_contiguous() else ", not dense"))
@@ -118,6 +117,12 @@ def code_bytes(k: int) -> int:
 def scale_bytes(k: int) -> int:
     """Bytes of a row's scales, as Mx4QuantSpec writes them."""
     return -(-k // 512) * 16
+
+
+def _keep(spec, desc, sizes):
+    """The descriptor, a reference to it for the calls, and how many values each tensor has to hold."""
+    for name, v in (("_desc", desc), ("_ref", C.byref(desc)), ("_sizes", sizes)):
+        object.__setattr__(spec, name, v)
 
 
 def _span(rows, stride, last):
@@ -135,10 +140,9 @@ class Mx4QuantSpec:
     x_stride: int = 0
 
     def __post_init__(self):
-        object.__setattr__(self, "_desc", _QuantDesc(_u32("rows", self.rows), _u32("k", self.k), int(self.dt),
-                                                     _u32("x_stride", self.x_stride)))
-        object.__setattr__(self, "_sizes", (_span(self.rows, self.x_stride or self.k, self.k),
-                                            self.rows * self.code_bytes, self.rows * self.scale_bytes))
+        desc = _QuantDesc(_u32("rows", self.rows), _u32("k", self.k), int(self.dt), _u32("x_stride", self.x_stride))
+        _keep(self, desc, (_span(self.rows, self.x_stride or self.k, self.k), self.rows * self.code_bytes,
+                           self.rows * self.scale_bytes))
 
     @property
     def code_bytes(self) -> int:
@@ -150,11 +154,19 @@ class Mx4QuantSpec:
 
     def run(self, x, codes, scales, stream=None):
         """x [rows, x_stride]; codes [rows, code_bytes], scales [rows, scale_bytes] uint8."""
-        T, device, types, u8, _ = _torch or _torch_types()
-        dev, (nx, nc, ns) = device() if x.__class__ is T else None, self._sizes
-        if (_lib or lib()).aih_mx4_quant(
-                C.byref(self._desc), _take("x", x, nx, types.get(self.dt), dev), _take("codes", codes, nc, u8, dev),
-                _take("scales", scales, ns, u8, dev), conv._stream(stream)):
+        T, device, raw, types, u8, _ = _torch or _torch_types()
+        (nx, nc, ns), t = self._sizes, types.get(self.dt)
+        if (x.__class__ is T and x.is_cuda and x.get_device() == (dev := device()) and x.dtype is t
+                and x.is_contiguous() and x.numel() >= nx
+                and codes.__class__ is T and codes.get_device() == dev and codes.dtype is u8
+                and codes.is_contiguous() and codes.numel() >= nc
+                and scales.__class__ is T and scales.get_device() == dev and scales.dtype is u8
+                and scales.is_contiguous() and scales.numel() >= ns):
+            at = x.data_ptr(), codes.data_ptr(), scales.data_ptr(), raw(dev) if stream is None else conv._stream(stream)
+        else:
+            at = (_take("x", x, nx, t), _take("codes", codes, nc, u8), _take("scales", scales, ns, u8),
+                  conv._stream(stream))
+        if (_lib or lib()).aih_mx4_quant(self._ref, *at):
             raise AihError(conv.last_error())
         return codes, scales
 
@@ -171,22 +183,30 @@ class Mx4DequantSpec:
     y_stride: int = 0
 
     def __post_init__(self):
-        object.__setattr__(self, "_desc", _DequantDesc(
+        desc = _DequantDesc(
             _u32("rows", self.rows), _u32("k", self.k), int(self.dt), _u32("code_stride", self.code_stride),
-            _u32("scale_stride", self.scale_stride), _u32("y_stride", self.y_stride)))
+            _u32("scale_stride", self.scale_stride), _u32("y_stride", self.y_stride))
         blocks = -(-self.k // 32)
-        object.__setattr__(self, "_sizes", (
+        _keep(self, desc, (
             _span(self.rows, self.code_stride or code_bytes(self.k), blocks * 16),
             _span(self.rows, self.scale_stride or scale_bytes(self.k), blocks),
             _span(self.rows, self.y_stride or self.k, self.k)))
 
     def run(self, codes, scales, y, stream=None):
         """codes, scales uint8; y [rows, y_stride]."""
-        T, device, types, u8, _ = _torch or _torch_types()
-        dev, (nc, ns, ny) = device() if y.__class__ is T else None, self._sizes
-        if (_lib or lib()).aih_mx4_dequant(
-                C.byref(self._desc), _take("codes", codes, nc, u8, dev), _take("scales", scales, ns, u8, dev),
-                _take("y", y, ny, types.get(self.dt), dev), conv._stream(stream)):
+        T, device, raw, types, u8, _ = _torch or _torch_types()
+        (nc, ns, ny), t = self._sizes, types.get(self.dt)
+        if (codes.__class__ is T and codes.is_cuda and codes.get_device() == (dev := device()) and codes.dtype is u8
+                and codes.is_contiguous() and codes.numel() >= nc
+                and scales.__class__ is T and scales.get_device() == dev and scales.dtype is u8
+                and scales.is_contiguous() and scales.numel() >= ns
+                and y.__class__ is T and y.get_device() == dev and y.dtype is t and y.is_contiguous()
+                and y.numel() >= ny):
+            at = codes.data_ptr(), scales.data_ptr(), y.data_ptr(), raw(dev) if stream is None else conv._stream(stream)
+        else:
+            at = (_take("codes", codes, nc, u8), _take("scales", scales, ns, u8), _take("y", y, ny, t),
+                  conv._stream(stream))
+        if (_lib or lib()).aih_mx4_dequant(self._ref, *at):
             raise AihError(conv.last_error())
         return y
 
@@ -203,22 +223,40 @@ class Mx4PwSpec:
     dt: DType = DType.F32
 
     def __post_init__(self):
-        object.__setattr__(self, "_desc", _PwDesc(
+        desc = _PwDesc(
             *(_u32(n, getattr(self, n)) for n in ("m", "k", "cout")), int(self.act), int(bool(self.residual)),
-            int(self.dt)))
+            int(self.dt))
         cb, sb = code_bytes(self.k), scale_bytes(self.k)
-        object.__setattr__(self, "_sizes", (self.m * cb, self.m * sb, self.cout * cb, self.cout * sb, self.m * self.cout))
+        _keep(self, desc, (self.m * cb, self.m * sb, self.cout * cb, self.cout * sb, self.m * self.cout))
 
     def run(self, x_codes, x_scales, w_codes, w_scales, bias, res, y, stream=None):
         """Codes and scales as Mx4QuantSpec makes them, of x [m, k] and of the weights [cout, k]; bias [cout] or None;
         res (with `residual`) and y [m, cout]."""
-        T, device, types, u8, _ = _torch or _torch_types()
-        dev, (nxc, nxs, nwc, nws, ny), t = device() if y.__class__ is T else None, self._sizes, types.get(self.dt)
-        if (_lib or lib()).aih_mx4_pw(
-                C.byref(self._desc), _take("x_codes", x_codes, nxc, u8, dev), _take("x_scales", x_scales, nxs, u8, dev),
-                _take("w_codes", w_codes, nwc, u8, dev), _take("w_scales", w_scales, nws, u8, dev),
-                _take("bias", bias, self.cout, t, dev), _take("res", res, ny if self.residual else 0, t, dev),
-                _take("y", y, ny, t, dev), conv._stream(stream)):
+        T, device, raw, types, u8, _ = _torch or _torch_types()
+        (nxc, nxs, nwc, nws, ny), t = self._sizes, types.get(self.dt)
+        if (y.__class__ is T and y.is_cuda and y.get_device() == (dev := device()) and y.dtype is t
+                and y.is_contiguous() and y.numel() >= ny
+                and x_codes.__class__ is T and x_codes.get_device() == dev and x_codes.dtype is u8
+                and x_codes.is_contiguous() and x_codes.numel() >= nxc
+                and x_scales.__class__ is T and x_scales.get_device() == dev and x_scales.dtype is u8
+                and x_scales.is_contiguous() and x_scales.numel() >= nxs
+                and w_codes.__class__ is T and w_codes.get_device() == dev and w_codes.dtype is u8
+                and w_codes.is_contiguous() and w_codes.numel() >= nwc
+                and w_scales.__class__ is T and w_scales.get_device() == dev and w_scales.dtype is u8
+                and w_scales.is_contiguous() and w_scales.numel() >= nws
+                and (bias is None or bias.__class__ is T and bias.get_device() == dev and bias.dtype is t
+                     and bias.is_contiguous() and bias.numel() >= self.cout)
+                and (res is None or res.__class__ is T and res.get_device() == dev and res.dtype is t
+                     and res.is_contiguous() and res.numel() >= (ny if self.residual else 0))):
+            at = (x_codes.data_ptr(), x_scales.data_ptr(), w_codes.data_ptr(), w_scales.data_ptr(),
+                  None if bias is None else bias.data_ptr(), None if res is None else res.data_ptr(), y.data_ptr(),
+                  raw(dev) if stream is None else conv._stream(stream))
+        else:
+            at = (_take("x_codes", x_codes, nxc, u8), _take("x_scales", x_scales, nxs, u8),
+                  _take("w_codes", w_codes, nwc, u8), _take("w_scales", w_scales, nws, u8),
+                  _take("bias", bias, self.cout, t), _take("res", res, ny if self.residual else 0, t),
+                  _take("y", y, ny, t), conv._stream(stream))
+        if (_lib or lib()).aih_mx4_pw(self._ref, *at):
             raise AihError(conv.last_error())
         return y
 
@@ -252,11 +290,11 @@ class Kv4AppendSpec:
     def __post_init__(self):
         u = {n: _u32(n, getattr(self, n)) for n in ("tokens", "hq", "hkv", "d", "rot", "positions", "page", "pages",
                                                     "x_stride", "q_stride")}
-        object.__setattr__(self, "_desc", _AppendDesc(
+        desc = _AppendDesc(
             u["tokens"], u["hq"], u["hkv"], u["d"], u["rot"], int(bool(self.pairs)), int(bool(self.norm)), self.eps,
-            int(self.dt), u["positions"], u["page"], u["pages"], u["x_stride"], u["q_stride"]))
+            int(self.dt), u["positions"], u["page"], u["pages"], u["x_stride"], u["q_stride"])
         row, rows = (self.hq + 2 * self.hkv) * self.d, self.pages * self.hkv * self.page
-        object.__setattr__(self, "_sizes", (
+        _keep(self, desc, (
             _span(self.tokens, self.x_stride or row, row),
             _span(self.tokens, self.q_stride or self.hq * self.d, self.hq * self.d) if self.hq else 0,
             self.positions * (self.rot // 2), rows * (self.d // 2), rows * (self.d // 32)))
@@ -264,16 +302,34 @@ class Kv4AppendSpec:
     def run(self, x, wq, wk, cosines, sines, pos, slots, q, k_codes, k_scales, v_codes, v_scales, stream=None):
         """x [tokens, x_stride]; wq, wk [d] or None; cosines, sines [positions, rot/2] fp32; pos int32 [tokens] or None;
         slots int32 [tokens]; q [tokens, hq, d]; the cache as kv4_cache makes it."""
-        T, device, types, u8, i32 = _torch or _torch_types()
-        dev, t, f32 = device() if x.__class__ is T else None, types.get(self.dt), types[0]
+        T, device, raw, types, u8, i32 = _torch or _torch_types()
+        t, f32, n = types.get(self.dt), types[0], self.tokens
         nx, nq, nt, nc, ns = self._sizes
+        if (x.__class__ is T and x.is_cuda and x.get_device() == (dev := device()) and x.dtype is t
+                and x.is_contiguous() and x.numel() >= nx
+                and slots.__class__ is T and slots.get_device() == dev and slots.dtype is i32
+                and slots.is_contiguous() and slots.numel() >= n
+                and q.__class__ is T and q.get_device() == dev and q.dtype is t and q.is_contiguous()
+                and q.numel() >= nq
+                and k_codes.__class__ is T and k_codes.get_device() == dev and k_codes.dtype is u8
+                and k_codes.is_contiguous() and k_codes.numel() >= nc
+                and k_scales.__class__ is T and k_scales.get_device() == dev and k_scales.dtype is u8
+                and k_scales.is_contiguous() and k_scales.numel() >= ns
+                and v_codes.__class__ is T and v_codes.get_device() == dev and v_codes.dtype is u8
+                and v_codes.is_contiguous() and v_codes.numel() >= nc
+                and v_scales.__class__ is T and v_scales.get_device() == dev and v_scales.dtype is u8
+                and v_scales.is_contiguous() and v_scales.numel() >= ns):
+            end = (q.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
+                   raw(dev) if stream is None else conv._stream(stream))
+            first, to = x.data_ptr(), slots.data_ptr()
+        else:
+            end = (_take("q", q, nq, t), _take("k_codes", k_codes, nc, u8), _take("k_scales", k_scales, ns, u8),
+                   _take("v_codes", v_codes, nc, u8), _take("v_scales", v_scales, ns, u8), conv._stream(stream))
+            first, to = _take("x", x, nx, t), _take("slots", slots, n, i32)
         if (_lib or lib()).aih_kv4_append(
-                C.byref(self._desc), _take("x", x, nx, t, dev), _take("wq", wq, self.d, t, dev),
-                _take("wk", wk, self.d, t, dev), _take("cosines", cosines, nt, f32, dev),
-                _take("sines", sines, nt, f32, dev), _take("pos", pos, self.tokens, i32, dev),
-                _take("slots", slots, self.tokens, i32, dev), _take("q", q, nq, t, dev),
-                _take("k_codes", k_codes, nc, u8, dev), _take("k_scales", k_scales, ns, u8, dev),
-                _take("v_codes", v_codes, nc, u8, dev), _take("v_scales", v_scales, ns, u8, dev), conv._stream(stream)):
+                self._ref, first, wq if wq is None else _take("wq", wq, self.d, t),
+                wk if wk is None else _take("wk", wk, self.d, t), _take("cosines", cosines, nt, f32),
+                _take("sines", sines, nt, f32), pos if pos is None else _take("pos", pos, n, i32), to, *end):
             raise AihError(conv.last_error())
         return q
 
@@ -301,12 +357,12 @@ class Kv4AttnSpec:
     def __post_init__(self):
         if self.scale is not None and not self.scale > 0:
             raise AihError(f"scale must be positive, not {self.scale!r}")
-        object.__setattr__(self, "_desc", _AttnDesc(
+        desc = _AttnDesc(
             *(_u32(n, getattr(self, n)) for n in ("nseq", "tokens", "hq", "hkv", "d", "page", "pages", "table_width")),
             int(bool(self.causal)), self.scale or 0.0, int(self.dt), _u32("max_len", self.max_len),
-            _u32("q_stride", self.q_stride), _u32("o_stride", self.o_stride)))
+            _u32("q_stride", self.q_stride), _u32("o_stride", self.o_stride))
         row, rows = self.hq * self.d, self.pages * self.hkv * self.page
-        object.__setattr__(self, "_sizes", (
+        _keep(self, desc, (
             _span(self.tokens, self.q_stride or row, row), _span(self.tokens, self.o_stride or row, row),
             rows * (self.d // 2), rows * (self.d // 32), self.nseq * self.table_width))
         object.__setattr__(self, "_ws", None)
@@ -324,20 +380,41 @@ class Kv4AttnSpec:
     def run(self, q, k_codes, k_scales, v_codes, v_scales, q_start, table, k_len, out, ws=None, stream=None):
         """q, out [tokens, hq, d]; the cache as kv4_cache makes it; q_start [nseq + 1], table [nseq, table_width], k_len
         [nseq] int32; ws: workspace_bytes() of device memory, made here if None."""
-        T, device, types, u8, i32 = _torch or _torch_types()
-        dev, t, b = device() if out.__class__ is T else None, types.get(self.dt), self.nseq
+        T, device, raw, types, u8, i32 = _torch or _torch_types()
+        t, b = types.get(self.dt), self.nseq
         nq, no, nc, ns, nt = self._sizes
         n = self._ws if self._ws is not None else self.workspace_bytes()
         if n:
             if ws is None:
                 ws = _workspace_on(n, conv._device_of(out), stream)
-            if not isinstance(ws, int) and ws.numel() * ws.element_size() < n:
+            if ws.__class__ is not int and ws.numel() * ws.element_size() < n:
                 raise AihError(f"the workspace needs {n} bytes, not {ws.numel() * ws.element_size()}")
-        if (_lib or lib()).aih_kv4_attn(
-                C.byref(self._desc), _take("q", q, nq, t, dev), _take("k_codes", k_codes, nc, u8, dev),
-                _take("k_scales", k_scales, ns, u8, dev), _take("v_codes", v_codes, nc, u8, dev),
-                _take("v_scales", v_scales, ns, u8, dev), _take("q_start", q_start, b + 1, i32, dev),
-                _take("table", table, nt, i32, dev), _take("k_len", k_len, b, i32, dev), _take("out", out, no, t, dev),
-                conv._ptr(ws) if n else None, n, conv._stream(stream)):
+        if (out.__class__ is T and out.is_cuda and out.get_device() == (dev := device()) and out.dtype is t
+                and out.is_contiguous() and out.numel() >= no
+                and q.__class__ is T and q.get_device() == dev and q.dtype is t and q.is_contiguous()
+                and q.numel() >= nq
+                and k_codes.__class__ is T and k_codes.get_device() == dev and k_codes.dtype is u8
+                and k_codes.is_contiguous() and k_codes.numel() >= nc
+                and k_scales.__class__ is T and k_scales.get_device() == dev and k_scales.dtype is u8
+                and k_scales.is_contiguous() and k_scales.numel() >= ns
+                and v_codes.__class__ is T and v_codes.get_device() == dev and v_codes.dtype is u8
+                and v_codes.is_contiguous() and v_codes.numel() >= nc
+                and v_scales.__class__ is T and v_scales.get_device() == dev and v_scales.dtype is u8
+                and v_scales.is_contiguous() and v_scales.numel() >= ns
+                and q_start.__class__ is T and q_start.get_device() == dev and q_start.dtype is i32
+                and q_start.is_contiguous() and q_start.numel() > b
+                and table.__class__ is T and table.get_device() == dev and table.dtype is i32
+                and table.is_contiguous() and table.numel() >= nt
+                and k_len.__class__ is T and k_len.get_device() == dev and k_len.dtype is i32
+                and k_len.is_contiguous() and k_len.numel() >= b):
+            at = (q.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
+                  q_start.data_ptr(), table.data_ptr(), k_len.data_ptr(), out.data_ptr(), conv._ptr(ws) if n else None, n,
+                  raw(dev) if stream is None else conv._stream(stream))
+        else:
+            at = (_take("q", q, nq, t), _take("k_codes", k_codes, nc, u8), _take("k_scales", k_scales, ns, u8),
+                  _take("v_codes", v_codes, nc, u8), _take("v_scales", v_scales, ns, u8),
+                  _take("q_start", q_start, b + 1, i32), _take("table", table, nt, i32), _take("k_len", k_len, b, i32),
+                  _take("out", out, no, t), conv._ptr(ws) if n else None, n, conv._stream(stream))
+        if (_lib or lib()).aih_kv4_attn(self._ref, *at):
             raise AihError(conv.last_error())
         return out

@@ -118,8 +118,8 @@ typedef struct {
 
 /* cosines, sines [positions][rot/2] fp32; pos [tokens] int32, NULL = the token's own
  * index (positions outside the tables use the nearest row); slots [tokens] int32,
- * outside [0, pages * page) = the key and value are dropped. Two tokens with the same
- * slot leave, block by block, either's. q may be x's own query heads (same pointer and
+ * outside [0, pages * page) = the key and value are dropped; tokens of one call with the
+ * same slot leave a row that mixes theirs. q may be x's own query heads (same pointer and
  * row stride). */
 int aih_kv4_append(const aih_kv4_append_desc *d, const void *x, const void *wq, const void *wk, const float *cosines,
                    const float *sines, const int32_t *pos, const int32_t *slots, void *q, void *k_codes, void *k_scales,
