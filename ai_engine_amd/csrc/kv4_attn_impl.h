@@ -21,6 +21,15 @@
 // barriers until their results are joined. A step's registers are requested again
 // as soon as they are converted, so the next codes are on their way during the rest
 // of it.
+//
+// Single tokens are bound by memory between a start and an end: 64 sequences of 0 to 8192
+// keys, 32/8 bf16 heads of 128, 23.5 us and 4.5 to join their parts (94 MB: 18.4 us at a
+// large copy's 5.1 TB/s), one of 131071 keys, 16/4 f16 heads of 128, 19.3 and 4.8 (71 MB:
+// 14). The first loads (lengths, table, codes) follow each other, 3 us. With 32x32x16
+// products, whose tile a token's rows fill an eighth of, and addresses of each lane's own
+// it was 38 and 28. Prompts are bound by vector instructions (conversions, softmax) and
+// matrix instructions in turn: four behind 2000 keys, 87 GFLOP, 136 us, 640 TFLOP/s,
+// where a large matrix product reaches 1220.
 #pragma once
 
 #include "attn_impl.h"

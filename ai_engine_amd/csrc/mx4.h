@@ -53,8 +53,9 @@ struct Kv4AppendArgs {
   uint32_t positions, rows; // rows: pages * page
   uint32_t pshift;          // log2 of the rows of a page
   uint32_t items;           // tokens * (hq + 2 hkv)
+  uint32_t nl, per;         // lanes of a head, heads of a wavefront
   float eps, inv_d;
-  FastDiv by_ht;
+  FastDiv by_ht, by_nl;
 };
 
 hipError_t launch_kv4_append(const Kv4AppendArgs &a, int dt, hipStream_t st);

@@ -259,7 +259,8 @@ extern "C" int aih_kv4_append(const aih_kv4_append_desc *d, const void *x, const
     a.positions = d->positions, a.rows = d->pages * d->page, a.pshift = log2_of(d->page);
     a.items = (uint32_t)(d->tokens * heads);
     a.eps = d->eps, a.inv_d = 1.0f / (float)d->d;
-    a.by_ht = make_fastdiv((uint32_t)heads);
+    a.nl = d->d / 8, a.per = 64 / a.nl;
+    a.by_ht = make_fastdiv((uint32_t)heads), a.by_nl = make_fastdiv(a.nl);
     return launched(fn, launch_kv4_append(a, d->dt, stream_of(stream)));
   });
 }

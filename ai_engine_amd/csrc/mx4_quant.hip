@@ -5,6 +5,10 @@
 // largest magnitude is one exchange within the four (on the bits, whose order is
 // the magnitudes'), its exponent less 2 the scale byte, and the conversion
 // instructions do the rest. All of it is exact: the scales are powers of two.
+//
+// Bound by memory: 46080 rows of 960 f16 elements to 4 bits 20.6 us (5.4 TB/s of what
+// has to be read and written, where a large copy reaches 5.1) and back 18.2. A few rows are
+// bound by the host's call (9 x 4096: 2.5 us on the device, 4.6 from call to call).
 #include <hip/hip_runtime.h>
 
 #include "aih_device.h"

@@ -309,6 +309,12 @@ class Kv4AppendSpec:
                 and x.is_contiguous() and x.numel() >= nx
                 and slots.__class__ is T and slots.get_device() == dev and slots.dtype is i32
                 and slots.is_contiguous() and slots.numel() >= n
+                and (cosines is None or cosines.__class__ is T and cosines.get_device() == dev and cosines.dtype is f32
+                     and cosines.is_contiguous() and cosines.numel() >= nt)
+                and (sines is None or sines.__class__ is T and sines.get_device() == dev and sines.dtype is f32
+                     and sines.is_contiguous() and sines.numel() >= nt)
+                and (pos is None or pos.__class__ is T and pos.get_device() == dev and pos.dtype is i32
+                     and pos.is_contiguous() and pos.numel() >= n)
                 and q.__class__ is T and q.get_device() == dev and q.dtype is t and q.is_contiguous()
                 and q.numel() >= nq
                 and k_codes.__class__ is T and k_codes.get_device() == dev and k_codes.dtype is u8
@@ -321,15 +327,18 @@ class Kv4AppendSpec:
                 and v_scales.is_contiguous() and v_scales.numel() >= ns):
             end = (q.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
                    raw(dev) if stream is None else conv._stream(stream))
-            first, to = x.data_ptr(), slots.data_ptr()
+            first = x.data_ptr()
+            index = (None if cosines is None else cosines.data_ptr(), None if sines is None else sines.data_ptr(),
+                     None if pos is None else pos.data_ptr(), slots.data_ptr())
         else:
             end = (_take("q", q, nq, t), _take("k_codes", k_codes, nc, u8), _take("k_scales", k_scales, ns, u8),
                    _take("v_codes", v_codes, nc, u8), _take("v_scales", v_scales, ns, u8), conv._stream(stream))
-            first, to = _take("x", x, nx, t), _take("slots", slots, n, i32)
+            first = _take("x", x, nx, t)
+            index = (_take("cosines", cosines, nt, f32), _take("sines", sines, nt, f32), _take("pos", pos, n, i32),
+                     _take("slots", slots, n, i32))
         if (_lib or lib()).aih_kv4_append(
                 self._ref, first, wq if wq is None else _take("wq", wq, self.d, t),
-                wk if wk is None else _take("wk", wk, self.d, t), _take("cosines", cosines, nt, f32),
-                _take("sines", sines, nt, f32), pos if pos is None else _take("pos", pos, n, i32), to, *end):
+                wk if wk is None else _take("wk", wk, self.d, t), *index, *end):
             raise AihError(conv.last_error())
         return q
 

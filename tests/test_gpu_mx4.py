@@ -146,7 +146,8 @@ def check_pw(xq, wq, b, r, m, k, cout, dt, act=Activation.NONE, y=None, stream=N
 @pytest.mark.parametrize("dt", DTS, ids=IDS)
 @pytest.mark.parametrize("m, k, cout", [
     (1, 4, 4), (1, 4096, 20), (16, 128, 16), (17, 132, 36), (33, 2048, 100), (64, 960, 160), (65, 260, 68),
-    (100, 36, 4), (129, 1000, 132), (500, 516, 260), (1007, 1000, 724), (260, 4160, 64)])
+    (100, 36, 4), (129, 1000, 132), (500, 516, 260), (1007, 1000, 724), (260, 4160, 64),
+    (3, 70000, 8), (70, 70020, 8), (300, 2180, 300)])
 def test_product(m, k, cout, dt):
     residual = (m + cout) % 3 == 0
     xq, wq, b, r = make_pw(m * k, m, k, cout, dt, residual)
