@@ -468,3 +468,62 @@ def test_short_strided_and_other_tensors_are_refused():
         for bad in (t.flatten()[:-1], t.double(), t.cpu()):
             with pytest.raises(AihError, match=f"{name} must be a dense tensor"):
                 spec.run(*{**args, name: bad}.values())
+
+
+@pytest.mark.parametrize("norm", [False, True])
+def test_a_captured_step_follows_positions_and_slots(norm):
+    # one token of four streams: into the cache and attention over it, replayed with other rows each time
+    hq, hkv, d, page, dt, n = 8, 2, 64, 16, DType.BF16, 60
+    g = torch.Generator().manual_seed(13)
+    cos, sin = rotation_tables(n, d, device=DEV)
+    table = torch.randperm(16, generator=g).int().view(4, 4).to(DEV)
+    caches = [mx4.kv4_cache(16, page, hkv, d) for _ in range(2)]
+    w = (1 + 0.1 * torch.randn(d, generator=g)).to(TORCH[dt]).to(DEV) if norm else None
+    append = mx4.Kv4AppendSpec(tokens=4, hq=hq, hkv=hkv, d=d, page=page, pages=16, rot=d, positions=n, norm=norm, dt=dt)
+    attn = mx4.Kv4AttnSpec(nseq=4, tokens=4, hq=hq, hkv=hkv, d=d, page=page, pages=16, table_width=4, dt=dt)
+    x = torch.empty(4, hq + 2 * hkv, d, dtype=TORCH[dt], device=DEV)
+    pos, slots, k_len = (torch.zeros(4, dtype=torch.int32, device=DEV) for _ in range(3))
+    q_start = i32([0, 1, 2, 3, 4])
+    q, out = torch.empty(2, 4, hq, d, dtype=TORCH[dt], device=DEV)
+
+    def step(cache):
+        append.run(x, w, w, cos, sin, pos, slots, q, *cache)
+        attn.run(q, *cache, q_start, table, k_len, out)
+
+    slots.fill_(-1)
+    step(caches[0])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(caches[0])
+    for t in range(40):
+        at = torch.tensor([t, t // 2, t, 59 - t])
+        x.copy_(torch.randn(4, hq + 2 * hkv, d, generator=g))
+        pos.copy_(at.int()), k_len.copy_((at + 1).int())
+        slots.copy_(table[torch.arange(4), at.to(DEV) // page] * page + at.to(DEV) % page)
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = out.clone()
+        step(caches[1])
+        assert torch.equal(out, replayed) and torch.isfinite(out).all()
+    for a, b in zip(*caches):
+        assert torch.equal(a, b)
+
+
+def test_appending_on_another_stream_and_into_a_slice_of_a_projection():
+    hq, hkv, d = 2, 1, 96
+    x = torch.randn(90, 2 * hq + 2 * hkv, d, device=DEV)
+    cos, sin = rotation_tables(90, d, device=DEV)
+    slots = torch.arange(90, dtype=torch.int32, device=DEV)
+    spec = dict(tokens=90, hq=hq, hkv=hkv, d=d, rot=d, positions=90, page=32, pages=3)
+    own, other = mx4.kv4_cache(3, 32, hkv, d), mx4.kv4_cache(3, 32, hkv, d)
+    q = torch.empty(2, 90, hq, d, device=DEV)
+    dense = x[:, hq:].contiguous()
+    mx4.Kv4AppendSpec(**spec).run(dense, None, None, cos, sin, None, slots, q[0], *own)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    row = x.shape[1] * d
+    at = x.data_ptr() + hq * d * 4  # the heads from hq on, still in the projection's rows
+    mx4.Kv4AppendSpec(**spec, x_stride=row).run(at, None, None, cos, sin, None, slots, q[1], *other, stream=s)
+    s.synchronize()
+    assert torch.equal(q[0], q[1]) and all(torch.equal(a, b) for a, b in zip(own, other))

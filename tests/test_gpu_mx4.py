@@ -247,3 +247,23 @@ def test_short_strided_and_other_tensors_are_refused():
     for bad in (c[:3], c.to(torch.int8), c.cpu()):
         with pytest.raises(AihError, match="codes must be a dense tensor"):
             spec.run(x, bad, s)
+
+
+@pytest.mark.parametrize("m, k, cout", [
+    (1, 100, 40), (20, 2100, 36), (200, 1000, 64), (300, 2100, 300), (1100, 2100, 2100), (2000, 2100, 2500), (4096, 2176, 4096)])
+def test_scales_of_no_element_do_not_count(m, k, cout):
+    # an odd number of 128s, every size of tile; what is behind a row's scales reads as NaN
+    xq, wq, b, r = make_pw(17, m, k, cout, DType.BF16, False)
+    for q in (xq, wq):
+        q[1][:, -(-k // 128) * 4:] = 255
+    check_pw(xq, wq, b, r, m, k, cout, DType.BF16)
+
+
+def test_a_row_is_its_own():
+    # the same pixels among others, in another place and in another number of them: the same tile, the same bits
+    xq, wq, b, _ = make_pw(19, 700, 1024, 200, DType.F32, False)
+    y = check_pw(xq, wq, b, None, 700, 1024, 200, DType.F32)[:700]
+    at = torch.randperm(700, generator=torch.Generator().manual_seed(1)).to(DEV)
+    other = torch.empty_like(y)
+    mx4.Mx4PwSpec(m=700, k=1024, cout=200).run(xq[0][at].contiguous(), xq[1][at].contiguous(), *wq, b, None, other)
+    assert torch.equal(other, y[at])
