@@ -100,9 +100,11 @@ struct KvCfg {
   static constexpr uint32_t BUF = WK * VT + QB > JOIN ? WK * VT + QB : JOIN;
   static constexpr uint32_t LDS = BUF + ML;
   static_assert(LDS <= 160 * 1024, "LDS");
-  // registers that a wavefront cannot do without: queries, results, scores, codes
-  static constexpr int NEED = (QL ? 0 : 4 * NT * NB * RB) + 8 * NB * RB + 8 * RB + 5 * NB;
-  static constexpr int WPE = NEED <= 80 && 4 * LDS <= 160 * 1024 ? 4 : NEED <= 190 && 2 * LDS <= 160 * 1024 ? 2 : 1;
+  // registers that a wavefront cannot do without: queries, results, scores, probabilities, codes
+  static constexpr int NEED = (QL ? 0 : 4 * NT * NB * RB) + 8 * NB * RB + 8 * RB + 4 * NT * RB + 5 * NB;
+  // wavefronts of a SIMD: a few registers that spill cost less than one of them (4096 tokens, 32/8
+  // fp32 heads of 96, one 405 us, two 271)
+  static constexpr int WPE = NEED <= 80 && 4 * LDS <= 160 * 1024 ? 4 : NEED <= (NT == 3 ? 195 : 215) && 2 * LDS <= 160 * 1024 ? 2 : 1;
 };
 
 // Product s of a head's: where a lane group's eight elements are. Sets of four
@@ -648,7 +650,6 @@ hipError_t kv_launch_dt(const Kv4AttnArgs &a, hipStream_t st) {
   if (a.rb == 1) return kv_launch_rows<DT, 1>(a, st);
   if (a.rb == 2) return kv_launch_rows<DT, 2>(a, st);
   switch (a.at.d / 32) {
-    case 1: return kv_launch_items<KvCfg<DT, 1, 4, 4>>(a, st);
     case 2: return kv_launch_items<KvCfg<DT, 2, 4, 4>>(a, st);
     case 3: return kv_launch_items<KvCfg<DT, 3, 4, 4>>(a, st);
     case 4: return kv_launch_items<KvCfg<DT, 4, 4, 4>>(a, st);
