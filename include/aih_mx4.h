@@ -42,9 +42,10 @@ extern "C" {
 #endif
 
 /* Rows in 4 bits, as aih_mx4_quant writes and aih_mx4_pw reads them, one after
- * another: AIH_MX4_CODE_BYTES(k) bytes of codes, whole 128s of elements with 0 past
- * k, and AIH_MX4_SCALE_BYTES(k) bytes of scales, whole 512s; those of no element
- * are not written and may hold anything. */
+ * another: AIH_MX4_CODE_BYTES(k) bytes of codes, whole 128s of elements, and
+ * AIH_MX4_SCALE_BYTES(k) bytes of scales, room for whole 512s. Codes and scales of a
+ * row's last 128 that are past k are 0; scales behind those are not written and may
+ * hold anything. */
 #define AIH_MX4_CODE_BYTES(k) (((k) + 127) / 128 * 64)
 #define AIH_MX4_SCALE_BYTES(k) (((k) + 511) / 512 * 16)
 

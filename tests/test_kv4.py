@@ -1,6 +1,9 @@
 """CPU tests of the 4-bit cache operators' boundary: what is refused and with which
 message, and what the plan says. Nothing here launches a kernel."""
+import ctypes as C
+
 import pytest
+import torch
 
 from ai_engine_amd import conv, mx4
 from ai_engine_amd.conv import AihError, DType
@@ -105,8 +108,10 @@ def test_workspace():
     n = spec.workspace_bytes()
     with pytest.raises(AihError, match="aligned"):
         run(spec, ws=FAKE + 8)
+    for ws in (torch.empty(n // 4), torch.empty(n // 4 - 1), torch.empty(n // 4, 2)[:, 0]):  # on the host, all of them
+        with pytest.raises(AihError, match="the workspace needs"):
+            run(spec, ws=ws)
     d = spec._desc
-    import ctypes as C
     rc = mx4.lib().aih_kv4_attn(C.byref(d), *[FAKE] * 9, FAKE, n - 4, None)
     assert rc == -1 and "workspace needs" in conv.last_error()
     rc = mx4.lib().aih_kv4_attn(C.byref(d), *[FAKE] * 9, None, n, None)
