@@ -267,3 +267,30 @@ def test_a_row_is_its_own():
     other = torch.empty_like(y)
     mx4.Mx4PwSpec(m=700, k=1024, cout=200).run(xq[0][at].contiguous(), xq[1][at].contiguous(), *wq, b, None, other)
     assert torch.equal(other, y[at])
+
+
+def test_rows_and_results_beyond_4_gib():
+    rows, k, cout, dt = (1 << 21) + 37, 1024, 1024, DType.BF16
+    x = torch.zeros(rows, k, dtype=torch.bfloat16, device=DEV)
+    x[-200:] = some_rows(1, 200, k, dt).to(DEV)
+    assert x.numel() * 2 > 1 << 32
+    codes, scales = row_buffers(rows, k)
+    mx4.Mx4QuantSpec(rows=rows, k=k, dt=dt).run(x, codes, scales)
+    want_c, want_s = quant_rows(x[-200:].cpu())
+    assert torch.equal(codes[-200:].cpu(), want_c) and torch.equal(scales[-200:].cpu()[:, :want_s.shape[1]], want_s)
+    assert not codes[:-200].any()
+    x.fill_(7.0)
+    mx4.Mx4DequantSpec(rows=rows, k=k, dt=dt).run(codes, scales, x)
+    assert torch.equal(x[-200:].cpu(), values(codes[-200:], scales[-200:]).bfloat16()) and not x[:-200].any()
+    # the product of the same rows: the last ones among all are the same as alone
+    w = some_rows(2, cout, k, dt).to(DEV)
+    wq = row_buffers(cout, k)
+    mx4.Mx4QuantSpec(rows=cout, k=k, dt=dt).run(w, *wq)
+    x.fill_(7.0)
+    mx4.Mx4PwSpec(m=rows, k=k, cout=cout, dt=dt).run(codes, scales, *wq, None, None, x)
+    assert not x[:-200].any()
+    check_pw((codes[-200:].contiguous(), scales[-200:].contiguous()), wq, None, None, 200, k, cout, dt)
+    alone = torch.empty(200, cout, dtype=torch.bfloat16, device=DEV)
+    mx4.Mx4PwSpec(m=200, k=k, cout=cout, dt=dt).run(codes[-200:].contiguous(), scales[-200:].contiguous(), *wq, None, None, alone)
+    # sums of the same blocks in another order: a few roundings of fp32 each, and one of the store
+    assert ((x[-200:].float() - alone.float()).abs() <= 2.0 ** -7 * alone.float().abs() + 1e-3 * alone.float().abs().max()).all()
