@@ -172,14 +172,25 @@ struct KvCodes {
     if constexpr (C::REST & 1)
       if (all) one = 0, s1 = 127;
   }
-  __device__ __forceinline__ void clear_nan() {
+  // scale bytes that the product does not take: of NaN, and those below `less`
+  static __device__ __forceinline__ bool odd(uint32_t byte, uint32_t less) { return byte - less > 252 - less; }
+  __device__ __forceinline__ void clear_odd(uint32_t less) {
 #pragma unroll
     for (int i = 0; i < C::SETS; ++i)
-      if (sw[i] > 252) w[i] = u32x4{}, sw[i] = 127;
+      if (odd(sw[i], less)) w[i] = u32x4{}, sw[i] = 127;
     if constexpr (C::REST >= 2)
-      if (s2 > 252) two = u32x2{}, s2 = 127;
+      if (odd(s2, less)) two = u32x2{}, s2 = 127;
     if constexpr (C::REST & 1)
-      if (s1 > 252) one = 0, s1 = 127;
+      if (odd(s1, less)) one = 0, s1 = 127;
+  }
+  // whether one of the blocks has such a scale
+  __device__ __forceinline__ bool odd(uint32_t less) const {
+    bool x = false;
+#pragma unroll
+    for (int i = 0; i < C::SETS; ++i) x |= odd(sw[i], less);
+    if constexpr (C::REST >= 2) x |= odd(s2, less);
+    if constexpr (C::REST & 1) x |= odd(s1, less);
+    return x;
   }
   // whether one of the blocks is NaN
   __device__ __forceinline__ bool nan() const {
@@ -225,14 +236,25 @@ __device__ __forceinline__ float kv_probs(const float (&s)[8], u32x4 (&pt)[NT], 
   return sum;
 }
 
+// The probabilities of a lane and step, 8 keys, from which a row's maximum is found anew.
+constexpr float kKvMost = 256.0f;
+
+// Values reach 6 * 2^125, a third below fp32's largest number, and sums of them times
+// probabilities must not leave its range where the mean does not. A row's probabilities add
+// up to at most kKvMost / 8 for each key (in whole steps of 32): values are taken 2^-kv_less
+// times as large, which costs nothing (their scales are made with one add), and the sum of the
+// probabilities too, at the end. What becomes less than the format's smallest scale is read as
+// zero: values below 6 * 2^(kv_less - 127), 2^-102 with 131072 keys.
+__device__ __forceinline__ uint32_t kv_less(uint32_t keys) { return 32 - __builtin_clz(max(keys, 32u) - 1) + 5; }
+
 // The softmax of a step: as at_settle, the maximum of a row is left as it is until
-// its probabilities add up to more than 2^15, and found then.
+// its probabilities add up to kKvMost, and found then.
 template <class C>
 __device__ __forceinline__ void kv_softmax(float (&s)[8], u32x4 (&pt)[C::NT], float &m, float &l, f32x4 (&o)[2 * C::NB],
                                            float scale) {
 #pragma clang fp contract(off)
   float sum = kv_probs<C::NT>(s, pt, -m, scale);
-  const bool far0 = __builtin_fabsf(m) >= kAtFar, big = !(sum < kAtMost) || far0;
+  const bool far0 = __builtin_fabsf(m) >= kAtFar, big = !(sum < kKvMost) || far0;
   if (__any(big)) {
     const bool row = kv_row_max(big ? 1.0f : 0.0f) != 0.0f;
     float mx = s[0];
@@ -362,6 +384,7 @@ __global__ __launch_bounds__(64 * C::WK, C::WPE) void kv4_attn_kernel(Kv4AttnArg
     const uint32_t smax = at_limit(a, a.causal, s, min(row0 + TR, nrows) - 1);
     const uint32_t kend = __builtin_amdgcn_readfirstlane((uint32_t)min((uint64_t)smax, (uint64_t)kbeg + (1ull << shift)));
 
+    const uint32_t less = kv_less(s.len);
     const uint32_t nb = a.d / 32, pmask = (1u << ka.pshift) - 1;
     const int32_t *table = ka.table + (uint64_t)s.k0 * ka.width;
     // the pages of keys key .. key + 15 and the next 16, in lanes 0 and 1
@@ -460,12 +483,12 @@ __global__ __launch_bounds__(64 * C::WK, C::WPE) void kv4_attn_kernel(Kv4AttnArg
         vis[rb] = seen & (to >= 32 ? 0xffffffffu : (1u << to) - 1);
       }
 
-      // V into LDS. Keys that are not there as zeros, and so are blocks that are NaN, which are
-      // added to the rows that see them here
+      // V into LDS. Keys that are not there as zeros, and so are blocks of scales that are too small
+      // (see kv_less) and blocks that are NaN, which are added to the rows that see them here
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         if (!C::EXACT || seen != 0xffffffffu) vx[h].clear(!(seen >> (16 * h + l16) & 1), g, nb);
-      if (__any(vx[0].nan() || vx[1].nan())) {
+      if (__any(vx[0].odd(less) || vx[1].odd(less))) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           for (uint64_t left = __ballot(vx[h].nan()); left; left &= left - 1) {
@@ -486,7 +509,7 @@ __global__ __launch_bounds__(64 * C::WK, C::WPE) void kv4_attn_kernel(Kv4AttnArg
                 }
             }
           }
-          vx[h].clear_nan();
+          vx[h].clear_odd(less);
         }
       }
       const uint32_t vsw = kv_swz<C>(l16);
@@ -495,7 +518,7 @@ __global__ __launch_bounds__(64 * C::WK, C::WPE) void kv4_attn_kernel(Kv4AttnArg
 #pragma unroll
         for (int h = 0; h < 2; ++h)
           *reinterpret_cast<u32x4 *>(vt + (16 * h + l16) * RW + ((KvPlace<C>::unit(st, g) ^ vsw) * 16)) =
-              kv_decode8(vx[h].code(st), mx4_scale(vx[h].scale(st)));
+              kv_decode8(vx[h].code(st), mx4_scale(vx[h].scale(st) - less));
       load(vx[0], ka.vc, ka.vs, r0), load(vx[1], ka.vc, ka.vs, r1);
 
       // the softmax; of block h this lane has keys 16 h + 4 g + 0..3
@@ -535,7 +558,7 @@ __global__ __launch_bounds__(64 * C::WK, C::WPE) void kv4_attn_kernel(Kv4AttnArg
     // join the wavefronts' keys: a common maximum, scaled sums through LDS, JD dims at a time
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      l[rb] = kv_row_sum(l[rb]);
+      l[rb] = kv_row_sum(l[rb]) * __uint_as_float((127 - less) << 23);  // as the values are
       if (g == 0) {
         jml[(2 * wave) * TR + 16 * rb + l16] = m[rb];
         jml[(2 * wave + 1) * TR + 16 * rb + l16] = l[rb];

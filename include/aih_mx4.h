@@ -136,7 +136,9 @@ int aih_kv4_append(const aih_kv4_append_desc *d, const void *x, const void *wq, 
  * output. Keys and values are exact in the products, statistics and sums fp32; fp32
  * queries and probabilities enter as three bf16 terms (all their bits), f16 ones as
  * two (16 bits of a probability), bf16 probabilities are rounded to bf16 and their sum is
- * of the rounded ones. */
+ * of the rounded ones. Values of any size are averaged without leaving fp32's range, but
+ * those below 6 * 2^-122 * Lk (Lk rounded up to a power of two, 32 at least) may read as
+ * zero; what fp32 queries have below 2^-133 is lost. */
 typedef struct {
   uint32_t nseq;        /* sequences; 0 is allowed */
   uint32_t tokens;      /* rows of q and o; tokens * hq below 2^31 */
