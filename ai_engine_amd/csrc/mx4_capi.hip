@@ -116,20 +116,23 @@ int check_kv4_attn(const aih_kv4_attn_desc *d, AttnArgs *a, Kv4Plan *p) {
   if (d->nseq == 0 || d->tokens == 0) return AIH_OK;
   const uint64_t rows = (uint64_t)d->tokens * a->g;
   const uint32_t cus = device_cus();
-  // 64 rows convert the keys half as often as 32, once there are two such tiles a CU.
+  const bool few = rows <= 32ull * d->nseq;
+  // 64 rows convert the keys half as often as 32, where sequences have more than 32 of them
+  // and there are two such tiles a CU.
   // 32 | 64, bf16: four prompts of 100 to 1024 behind 2000 keys, 32/8 heads of 128
   // (1112 tiles of 64) 148 | 137 us, 4096 tokens (2048) 218 | 177, 4 x 500 behind 100, 16/4
   // heads of 96 (516) 24.5 | 21.8; f16, 8 x 720, 8/2 heads of 64 (368) 31.8 | 33.9; 4096
   // tokens, 32/8 heads, f16 of 32 111 | 118, of 64 156 | 158, of 96 266 | 213, fp32 of 96 325 |
-  // 271, of 128 552 | 472. Above 128 the registers do not hold 64 rows' results
-  const bool wide = d->d >= 64 && d->d <= 128 && (rows / 64 + d->nseq / 2) * d->hkv >= 2ull * cus;
+  // 271, of 128 552 | 472. Above 128 the registers do not hold 64 rows' results. Of 32 rows a
+  // sequence at most half of a tile of 64 is empty: 128 x 5 tokens over 500 keys, 32/8 heads of
+  // 128 bf16 27.3 | 41.1, fp32 62 | 88; 1024 tokens over 400, 32/1 heads of 128 bf16 46.3 | 53.3
+  const bool wide = !few && d->d >= 64 && d->d <= 128 && (rows / 64 + d->nseq / 2) * d->hkv >= 2ull * cus;
   p->rb = rows <= 16ull * d->nseq ? 1 : wide ? 4 : 2;
   const uint32_t bm = 16 * p->rb;
   p->tiles = d->nseq == 1 ? (rows + bm - 1) / bm : rows / bm + d->nseq;
   const uint32_t len = d->max_len ? std::min(d->max_len, a->rows) : a->rows;
   auto parts = [&](uint32_t x) { return (uint32_t)std::max<uint64_t>(1, ((uint64_t)len + (1ull << x) - 1) >> x); };
   const uint64_t base = p->tiles * d->hkv;
-  const bool few = rows <= 32ull * d->nseq;
   if (few && len > (d->d > 128 ? 512u : 1024u)) {
     p->shift = 10;
     while (p->shift > 8 && base * parts(p->shift) < 2ull * cus) --p->shift;
