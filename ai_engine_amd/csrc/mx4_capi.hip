@@ -91,7 +91,10 @@ struct Kv4Plan {
 // 16.7, 15.6, 17.4; 64 of 0 to 8192 82 | 46, 38, 31.4, 37.7; 1 x 131071, 16/4 heads f16
 // 902 | 40, 28.5, 23.3, 25.2. Prompts are cut where their tiles leave CUs without one: 1024
 // tokens, 8/2 heads of 64 (256) 11.1 | 19, 16.3; 2000 tokens, 8/4 heads of 128 f16 (500) 31 to
-// 1024 45; 2 x 300 behind 4000 keys, 8/2 heads (154) 43 | 51, 43, 35.2, 35.8.
+// 1024 45; 2 x 300 behind 4000 keys, 8/2 heads (154) 43 | 51, 43, 35.2, 35.8. Heads of more than
+// 128 take longer for a key: from 512 on whole | 512 | 256, 4 x 600 keys, 16/4 heads of 256 14.7 |
+// 16.1 | 13.5, 4 x 1000 19.4 | 16.2 | 13.6, 64 x 900, 8/2 heads of 192 18.0 | 16.0 | 15.6, unless
+// every CU has one anyway: 64 x 600, 16/4 heads of 256 16.5 | 22.9 | 23.5, 64 x 900 21.8 | 22.8 | 29.1.
 int check_kv4_attn(const aih_kv4_attn_desc *d, AttnArgs *a, Kv4Plan *p) {
   const char *fn = "aih_kv4_attn";
   if (!d) return api_fail("aih_kv4_attn: NULL descriptor");
@@ -133,7 +136,7 @@ int check_kv4_attn(const aih_kv4_attn_desc *d, AttnArgs *a, Kv4Plan *p) {
   const uint32_t len = d->max_len ? std::min(d->max_len, a->rows) : a->rows;
   auto parts = [&](uint32_t x) { return (uint32_t)std::max<uint64_t>(1, ((uint64_t)len + (1ull << x) - 1) >> x); };
   const uint64_t base = p->tiles * d->hkv;
-  if (few && len > (d->d > 128 ? 512u : 1024u)) {
+  if (few && len > (d->d > 128 && base < cus ? 512u : 1024u)) {
     p->shift = 10;
     while (p->shift > 8 && base * parts(p->shift) < 2ull * cus) --p->shift;
   } else if (!few && base < cus) {

@@ -21,3 +21,11 @@ def plan(nseq, tokens, hq, hkv, d, keys, dt=DType.BF16, **kw):
     (4, 2224, 32, 8, 256, 32), (1, 512, 32, 8, 128, 32)])
 def test_rows_of_a_tile(nseq, tokens, hq, hkv, d, bm, dt):
     assert plan(nseq, tokens, hq, hkv, d, 1000, dt).bm == bm
+
+
+@pytest.mark.parametrize("nseq, hq, hkv, d, keys, parts", [
+    # single tokens: cut from 1024 keys on, heads of more than 128 from 512 on unless every CU has one
+    (4, 16, 4, 256, 600, 3), (4, 16, 4, 256, 512, 1), (64, 16, 4, 256, 600, 1), (64, 16, 4, 256, 960, 1),
+    (64, 8, 2, 192, 960, 4), (4, 16, 4, 128, 960, 1), (1, 16, 4, 128, 131072, 128), (64, 32, 8, 128, 8192, 8)])
+def test_parts_of_the_keys(nseq, hq, hkv, d, keys, parts):
+    assert plan(nseq, nseq, hq, hkv, d, keys).parts == parts
