@@ -396,9 +396,9 @@ class Kv4AttnSpec:
         if n:
             if ws is None:
                 ws = _workspace_on(n, conv._device_of(out), stream)
-            if ws.__class__ is not int and (
-                    ws.numel() * ws.element_size() < n or not ws.is_cuda or not ws.is_contiguous()):
-                raise AihError(f"the workspace needs {n} bytes, dense and on the GPU, not "
+            if ws.__class__ is not int and (ws.numel() * ws.element_size() < n or not ws.is_cuda
+                                            or ws.get_device() != device() or not ws.is_contiguous()):
+                raise AihError(f"the workspace needs {n} bytes, dense and on the current device, not "
                                f"{ws.numel() * ws.element_size()} on {ws.device}")
         if (out.__class__ is T and out.is_cuda and out.get_device() == (dev := device()) and out.dtype is t
                 and out.is_contiguous() and out.numel() >= no
