@@ -39,8 +39,9 @@ def rotation_tables(positions: int, rot: int, theta: float = 10000.0, device="cu
 class AttnBlock:
     """weights: w_qkv [(hq + 2 hkv) d, c], b_qkv, w_out [c, hq d], b_out, and the norms' wq, wk [d] (fp32
     arrays); capacity: cache rows of a stream; causal: a token sees the tokens up to its own (else the
-    whole step's); prefix: rows kept for `share`; cache4, page: a 4-bit cache (d in whole 32s, rot in whole 16s, no
-    prefix); proj4: 4-bit projections. Steps follow one another: on one stream, or with a wait in between.
+    whole step's); prefix: rows kept for `share`; cache4, page: a 4-bit cache (d in whole 32s up to 256, rot in
+    whole 16s, no prefix) in pages of so many rows (a power of two, 16 to 4096); proj4: 4-bit projections. Steps
+    follow one another: on one stream, or with a wait in between.
 
     Besides the cache a block holds the buffers of its longest step: queries, results and the attention's workspace,
     (d + 2) fp32 values a token and query head for every part of the keys. That is large for whole prompts behind a
@@ -69,8 +70,10 @@ class AttnBlock:
             if np.prod(np.shape(weights[name])) != n:  # what packs and reads them goes by the block's sizes alone
                 raise AihError(f"{name} must hold {n} values, not {tuple(np.shape(weights[name]))}")
         self.cache4, self.proj4, self.page = cache4, proj4, page
-        if cache4 and (prefix or d % 32 or self.rot % 16):
-            raise AihError("a 4-bit cache takes heads in whole 32s, rotations in whole 16s and no shared prefix")
+        if cache4 and (prefix or d % 32 or not 32 <= d <= 256 or self.rot % 16):
+            raise AihError("a 4-bit cache takes heads in whole 32s up to 256, rotations in whole 16s and no shared prefix")
+        if cache4 and (type(page) is not int or not 16 <= page <= 4096 or page & (page - 1)):
+            raise AihError(f"a 4-bit cache takes pages of a power of two rows, 16 to 4096, not {page!r}")
         if proj4:
             self.w_qkv = self._rows4(torch.as_tensor(weights["w_qkv"]).reshape(heads * d, c).float().to(device))
             self.w_out = self._rows4(torch.as_tensor(weights["w_out"]).reshape(c, hq * d).float().to(device))
