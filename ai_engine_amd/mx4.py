@@ -22,7 +22,7 @@ refused; raw addresses are the caller's own.
 from __future__ import annotations
 
 import ctypes as C
-from dataclasses import dataclass
+from dataclasses import dataclass, fields
 
 from . import conv
 from .attn import _u32, _workspace_on
@@ -125,13 +125,20 @@ def _keep(spec, desc, sizes):
         object.__setattr__(spec, name, v)
 
 
+class _Spec:
+    """Copies and pickles of a spec are made of its fields, with a descriptor of their own."""
+
+    def __reduce__(self):
+        return type(self), tuple(getattr(self, f.name) for f in fields(self))
+
+
 def _span(rows, stride, last):
     """Values that rows `stride` apart reach over, the last one `last` long."""
     return (rows - 1) * stride + last if rows else 0
 
 
 @dataclass(frozen=True)
-class Mx4QuantSpec:
+class Mx4QuantSpec(_Spec):
     """Rows to 4 bits; fields of aih_mx4_quant_desc (x_stride in elements, 0 = dense)."""
 
     rows: int
@@ -172,7 +179,7 @@ class Mx4QuantSpec:
 
 
 @dataclass(frozen=True)
-class Mx4DequantSpec:
+class Mx4DequantSpec(_Spec):
     """4-bit rows to values; fields of aih_mx4_dequant_desc (strides: bytes of codes and scales, elements of y)."""
 
     rows: int
@@ -212,7 +219,7 @@ class Mx4DequantSpec:
 
 
 @dataclass(frozen=True)
-class Mx4PwSpec:
+class Mx4PwSpec(_Spec):
     """The 1x1 conv of 4-bit rows; fields of aih_mx4_pw_desc."""
 
     m: int
@@ -269,7 +276,7 @@ def kv4_cache(pages, page, hkv, d, device="cuda:0"):
 
 
 @dataclass(frozen=True)
-class Kv4AppendSpec:
+class Kv4AppendSpec(_Spec):
     """New tokens into a 4-bit cache; fields of aih_kv4_append_desc (strides in elements, 0 = dense)."""
 
     tokens: int
@@ -344,7 +351,7 @@ class Kv4AppendSpec:
 
 
 @dataclass(frozen=True)
-class Kv4AttnSpec:
+class Kv4AttnSpec(_Spec):
     """Attention over a 4-bit cache; fields of aih_kv4_attn_desc (strides in elements, 0 = dense; scale None =
     1 / sqrt(d))."""
 
