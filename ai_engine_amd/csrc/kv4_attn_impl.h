@@ -636,6 +636,7 @@ __global__ __launch_bounds__(64 * C::WK, C::WPE) void kv4_attn_kernel(Kv4AttnArg
 
 // Items beyond the workgroups that run at once are shared by those: where keys are
 // cut, of the items that the host counts (the longest length for all) few may exist.
+// A launch takes less than 2^32 threads.
 template <class C>
 hipError_t kv_launch_items(const Kv4AttnArgs &a, hipStream_t st) {
   static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(kv4_attn_kernel<C>),
@@ -650,7 +651,8 @@ hipError_t kv_launch_items(const Kv4AttnArgs &a, hipStream_t st) {
   }();
   uint64_t items = (uint64_t)a.at.hkv * a.at.parts * a.at.tiles;
   if (items == 0 || items > 0x7fffffffu) return hipErrorInvalidValue;
-  if (a.at.parts > 1) items = items < (uint64_t)device_cus() * occ ? items : (uint64_t)device_cus() * occ;
+  const uint64_t most = a.at.parts > 1 ? (uint64_t)device_cus() * occ : 0xffffffffu / (64 * C::WK);
+  items = items < most ? items : most;
   hipLaunchKernelGGL((kv4_attn_kernel<C>), dim3((uint32_t)items), dim3(64 * C::WK), C::LDS, st, a);
   return hipGetLastError();
 }

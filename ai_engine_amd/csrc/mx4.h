@@ -20,7 +20,7 @@ struct Mx4RowsArgs {
   uint64_t stride;     // of the values' rows, elements
   uint32_t k;          // elements of a row
   uint32_t upr;        // units of 8 elements of a row: with quant of the padded row
-  uint64_t units;      // of all rows, below 2^32
+  uint64_t units;      // of all rows, below 2^32 - 255
   uint32_t code_stride, scale_stride;  // bytes
   FastDiv by_upr;
 };

@@ -17,6 +17,9 @@ namespace {
 
 constexpr uint32_t kMaxK = 1u << 20;
 constexpr uint64_t kMaxStride = 1u << 22;
+// Workgroups of 256 threads: a launch takes less than 2^32 threads, and one of more may run a
+// few of them and report nothing.
+constexpr uint32_t kMaxGroups = 0xffffff;
 
 bool dt_ok(int32_t dt) { return dt == AIH_F32 || dt == AIH_F16 || dt == AIH_BF16; }
 std::string num(uint64_t v) { return std::to_string(v); }
@@ -136,7 +139,10 @@ int check_kv4_attn(const aih_kv4_attn_desc *d, AttnArgs *a, Kv4Plan *p) {
   const uint32_t len = d->max_len ? std::min(d->max_len, a->rows) : a->rows;
   auto parts = [&](uint32_t x) { return (uint32_t)std::max<uint64_t>(1, ((uint64_t)len + (1ull << x) - 1) >> x); };
   const uint64_t base = p->tiles * d->hkv;
-  if (few && len > (d->d > 128 && base < cus ? 512u : 1024u)) {
+  // the join's launch takes 1024 threads a row at the most; the chip is full without
+  const bool joins = (uint64_t)d->tokens * d->hq < 1u << 22;
+  if (!joins) {
+  } else if (few && len > (d->d > 128 && base < cus ? 512u : 1024u)) {
     p->shift = 10;
     while (p->shift > 8 && base * parts(p->shift) < 2ull * cus) --p->shift;
   } else if (!few && base < cus) {
@@ -168,7 +174,8 @@ extern "C" int aih_mx4_quant(const aih_mx4_quant_desc *d, const void *x, void *c
     Mx4RowsArgs a{};
     if (int rc = rows_stride(fn, "x_stride", d->x_stride, d->k, &a.stride)) return rc;
     a.k = d->k, a.upr = AIH_MX4_CODE_BYTES(d->k) / 4, a.units = (uint64_t)d->rows * a.upr;
-    if (a.units > 0xffffffffu) return api_fail("aih_mx4_quant: rows of k rounded to 128 must hold less than 2^35 elements");
+    if (a.units > 256ull * kMaxGroups)
+      return api_fail("aih_mx4_quant: rows of k rounded to 128 must hold at most 2^35 - 2048 elements");
     if (d->rows == 0) return AIH_OK;
     if (!none_null({x, codes, scales})) return api_fail("aih_mx4_quant: NULL tensor");
     if (!aligned16({x, codes, scales})) return api_fail("aih_mx4_quant: tensors must be aligned to 16 bytes");
@@ -196,7 +203,7 @@ extern "C" int aih_mx4_dequant(const aih_mx4_dequant_desc *d, const void *codes,
     if (a.scale_stride < blocks)
       return api_fail("aih_mx4_dequant: scale_stride must hold " + num(blocks) + " blocks, not " + num(d->scale_stride));
     a.k = d->k, a.upr = (d->k + 7) / 8, a.units = (uint64_t)d->rows * a.upr;
-    if (a.units > 0xffffffffu) return api_fail("aih_mx4_dequant: rows must hold less than 2^35 elements");
+    if (a.units > 256ull * kMaxGroups) return api_fail("aih_mx4_dequant: rows must hold at most 2^35 - 2048 elements");
     if (d->rows == 0) return AIH_OK;
     if (!none_null({codes, scales, y})) return api_fail("aih_mx4_dequant: NULL tensor");
     if (!aligned16({codes, y})) return api_fail("aih_mx4_dequant: tensors must be aligned to 16 bytes");
@@ -215,7 +222,7 @@ extern "C" int aih_mx4_pw(const aih_mx4_pw_desc *d, const void *x_codes, const v
     if (int rc = k_ok(fn, d->k)) return rc;
     if (d->cout == 0 || d->cout % 4 || d->cout > kMaxK)
       return api_fail("aih_mx4_pw: cout must be a multiple of 4, 4 to " + num(kMaxK) + ", not " + num(d->cout));
-    if (d->m > 0x7fffffffu) return api_fail("aih_mx4_pw: m must be below 2^31");
+    if (d->m > 0x7fffff00u) return api_fail("aih_mx4_pw: m must be at most 2^31 - 256");
     if (d->act < AIH_ACT_NONE || d->act > AIH_ACT_RECIP) return api_fail("aih_mx4_pw: unknown activation " + std::to_string(d->act));
     if (d->residual != 0 && d->residual != 1) return api_fail("aih_mx4_pw: residual must be 0 or 1");
     if (d->m == 0) return AIH_OK;
@@ -251,6 +258,9 @@ extern "C" int aih_kv4_append(const aih_kv4_append_desc *d, const void *x, const
       return api_fail("aih_kv4_append: the tables need 1 to 2^31 - 1 rows");
     const uint64_t heads = (uint64_t)d->hq + 2 * (uint64_t)d->hkv;
     if (d->tokens * heads > 0x7fffffffu) return api_fail("aih_kv4_append: tokens * (hq + 2 hkv) must be below 2^31");
+    // a workgroup takes four wavefronts of 64 / (d / 8) heads
+    if ((d->tokens * heads + 4 * (512 / d->d) - 1) / (4 * (512 / d->d)) > kMaxGroups)
+      return api_fail("aih_kv4_append: tokens * (hq + 2 hkv) must be at most (2^24 - 1) * 4 * (512 / d)");
     Kv4AppendArgs a{};
     if (int rc = heads_stride(fn, "x_stride", d->x_stride, heads * d->d, d->dt, &a.xs)) return rc;
     if (int rc = heads_stride(fn, "q_stride", d->q_stride, (uint64_t)d->hq * d->d, d->dt, &a.qs)) return rc;

@@ -404,7 +404,7 @@ hipError_t launch_tile(Mx4PwArgs a, hipStream_t st) {
                                                      hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
   if (attr != hipSuccess) return attr;
   a.mtiles = (a.m + C::BM - 1) / C::BM, a.ntiles = (a.cout + C::BN - 1) / C::BN;
-  if ((uint64_t)a.mtiles * a.ntiles > 0x7fffffffu) return hipErrorInvalidValue;
+  if ((uint64_t)a.mtiles * a.ntiles * (64 * C::NW) > 0xffffffffu) return hipErrorInvalidValue;
   hipLaunchKernelGGL((mx4_pw_kernel<DT, C>), dim3(a.mtiles * a.ntiles), dim3(64 * C::NW), C::LDS, st, a);
   return hipGetLastError();
 }
@@ -432,7 +432,8 @@ hipError_t launch_dt(const Mx4PwArgs &a, hipStream_t st) {
   auto tiles = [&](uint32_t bm, uint32_t bn) { return (uint64_t)((a.m + bm - 1) / bm) * ((a.cout + bn - 1) / bn); };
   const uint64_t cus = device_cus(), big = tiles(256, 256), mid = tiles(128, 128);
   if (a.nst < 16) {
-    if (a.cout > 64 && mid >= cus) return launch_tile<DT, MxTile<2, 2, 2, 2, 2, 4>>(a, st);
+    // a launch takes less than 2^24 workgroups of 256 threads
+    if ((a.cout > 64 && mid >= cus) || tiles(64, 64) >> 24) return launch_tile<DT, MxTile<2, 2, 2, 2, 2, 4>>(a, st);
     return launch_tile<DT, MxTile<2, 2, 1, 1, 2, 4>>(a, st);
   }
   // rounds of tiles; one of 128 x 128, two a CU, takes 0.6 of one of 256 x 256

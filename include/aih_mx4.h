@@ -50,7 +50,7 @@ extern "C" {
 #define AIH_MX4_SCALE_BYTES(k) (((k) + 511) / 512 * 16)
 
 typedef struct {
-  uint32_t rows;
+  uint32_t rows;     /* rows of k rounded up to 128 hold at most 2^35 - 2048 elements */
   uint32_t k;        /* elements of a row: a multiple of 4, at most 2^20 */
   int32_t dt;        /* enum aih_dtype of x */
   uint64_t x_stride; /* elements, a multiple of 4, at most 2^22; 0 = k */
@@ -60,7 +60,7 @@ typedef struct {
 int aih_mx4_quant(const aih_mx4_quant_desc *d, const void *x, void *codes, void *scales, aih_stream stream);
 
 typedef struct {
-  uint32_t rows;
+  uint32_t rows;         /* rows of k rounded up to 8 hold at most 2^35 - 2048 elements */
   uint32_t k;            /* as above */
   int32_t dt;            /* enum aih_dtype of y */
   uint32_t code_stride;  /* bytes between rows of codes, a multiple of 16; 0 = AIH_MX4_CODE_BYTES(k) */
@@ -76,7 +76,7 @@ int aih_mx4_dequant(const aih_mx4_dequant_desc *d, const void *codes, const void
 /* y[i][n] = act(sum_k x[i][k] w[n][k] + bias[n]) + res[i][n]; sums in fp32, one
  * rounding at the store. */
 typedef struct {
-  uint32_t m;       /* pixels (rows) of x and y */
+  uint32_t m;       /* pixels (rows) of x and y, at most 2^31 - 256 */
   uint32_t k;       /* input channels: a multiple of 4, at most 2^20 */
   uint32_t cout;    /* output channels: a multiple of 4, at most 2^20 */
   int32_t act;      /* enum aih_act */
@@ -103,7 +103,7 @@ int aih_mx4_pw(const aih_mx4_pw_desc *d, const void *x_codes, const void *x_scal
  * rotated. Queries are rounded to q; keys and values (as they are in x) become row
  * slots[t] of the cache. */
 typedef struct {
-  uint32_t tokens;    /* rows of x and q; tokens * (hq + 2 hkv) below 2^31 */
+  uint32_t tokens;    /* rows of x and q; tokens * (hq + 2 hkv) at most (2^24 - 1) * 4 * (512 / d) */
   uint32_t hq, hkv;   /* heads; hq may be 0, hkv not */
   uint32_t d;         /* elements of a head: a multiple of 32, at most 256 */
   uint32_t rot;       /* rotated dims: a multiple of 16, at most d; 0 = none */

@@ -8,8 +8,9 @@ from ai_engine_amd.conv import DType
 
 def plan(nseq, tokens, hq, hkv, d, keys, dt=DType.BF16, **kw):
     width = -(-keys // 64)
-    return mx4.Kv4AttnSpec(nseq=nseq, tokens=tokens, hq=hq, hkv=hkv, d=d, page=64, pages=nseq * width, table_width=width,
-                           dt=dt, max_len=keys, **kw).plan()
+    return mx4.Kv4AttnSpec(**{**dict(
+        nseq=nseq, tokens=tokens, hq=hq, hkv=hkv, d=d, page=64, pages=nseq * width, table_width=width, dt=dt,
+        max_len=keys), **kw}).plan()
 
 
 @pytest.mark.parametrize("dt", list(DType))
