@@ -635,8 +635,12 @@ __global__ __launch_bounds__(64 * C::WK, C::WPE) void kv4_attn_kernel(Kv4AttnArg
 }
 
 // Items beyond the workgroups that run at once are shared by those: where keys are
-// cut, of the items that the host counts (the longest length for all) few may exist.
-// A launch takes less than 2^32 threads.
+// cut, of the items that the host counts (the longest length for all) few may exist; and
+// where there are many sequences, which every workgroup counts up to its first item (single
+// tokens over 40 keys, 32/8 heads of 64, a workgroup for each item | shared: 256 sequences
+// 13.8 | 11.6 us, 1024 84 | 38, 65536 214000 | 2318). Fewer ones of different lengths are better
+// off without (100 prompts of 16 to 1024 472 | 478, of 512 behind 512 207 | 225). A launch takes
+// less than 2^32 threads.
 template <class C>
 hipError_t kv_launch_items(const Kv4AttnArgs &a, hipStream_t st) {
   static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(kv4_attn_kernel<C>),
@@ -651,7 +655,8 @@ hipError_t kv_launch_items(const Kv4AttnArgs &a, hipStream_t st) {
   }();
   uint64_t items = (uint64_t)a.at.hkv * a.at.parts * a.at.tiles;
   if (items == 0 || items > 0x7fffffffu) return hipErrorInvalidValue;
-  const uint64_t most = a.at.parts > 1 ? (uint64_t)device_cus() * occ : 0xffffffffu / (64 * C::WK);
+  const bool shared = a.at.parts > 1 || a.at.nseq > 256;
+  const uint64_t most = shared ? (uint64_t)device_cus() * occ : 0xffffffffu / (64 * C::WK);
   items = items < most ? items : most;
   hipLaunchKernelGGL((kv4_attn_kernel<C>), dim3((uint32_t)items), dim3(64 * C::WK), C::LDS, st, a);
   return hipGetLastError();
