@@ -41,9 +41,10 @@ __device__ __forceinline__ void turn_pairs(float (&f)[8], f32x4 c, f32x4 s) {
 // All of a lane's loads go out before anything is computed, the tables' as soon as the
 // position is there, none of them behind a branch that a wait would follow: the
 // rotation is computed by all lanes and taken by those it is for. 46080 tokens of 8 + 2 + 2
-// f16 heads of 64 take 32 us with adjacent pairs (3.9 TB/s), 35 with halves, 26.5 without
-// rotation, where a large copy would take 24; 16384 of 32 + 8 + 8 bf16 heads of 128 78.
-// With the loads behind branches it was 38, 41 and 95. NORM and MODE apart, so that an
+// f16 heads of 64 take 32 us with adjacent pairs (3.9 TB/s), 36 with halves, 26.5 without
+// rotation, where a large copy would take 24; 16384 of 32 + 8 + 8 bf16 heads of 128 70 and 78.
+// With the loads behind branches it was 38, 41 and, with halves, 95. Head norms, whose sums
+// cross the lanes of a head: 34 and 41, 81 and 99. NORM and MODE apart, so that an
 // append carries what it needs.
 enum : int { MODE_NONE = 0, MODE_HALVES = 1, MODE_PAIRS = 2 };
 template <int DT, bool NORM, int MODE>

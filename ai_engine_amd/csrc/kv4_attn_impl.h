@@ -23,8 +23,8 @@
 // of it.
 //
 // Single tokens are bound by memory between a start and an end: 64 sequences of 0 to 8192
-// keys, 32/8 bf16 heads of 128, 23.5 us and 4.5 to join their parts (94 MB: 18.4 us at a
-// large copy's 5.1 TB/s), one of 131071 keys, 16/4 f16 heads of 128, 19.3 and 4.8 (71 MB:
+// keys, 32/8 bf16 heads of 128, 23.7 us and 4.2 to join their parts (94 MB: 18.4 us at a
+// large copy's 5.1 TB/s), one of 131071 keys, 16/4 f16 heads of 128, 19.8 and 4.7 (71 MB:
 // 14). The first loads (lengths, table, codes) follow each other, 3 us. With 32x32x16
 // products, whose tile a token's rows fill an eighth of, and addresses of each lane's own
 // it was 38 and 28. Prompts are bound by vector instructions (conversions, softmax) and
@@ -102,8 +102,12 @@ struct KvCfg {
   static_assert(LDS <= 160 * 1024, "LDS");
   // registers that a wavefront cannot do without: queries, results, scores, probabilities, codes
   static constexpr int NEED = (QL ? 0 : 4 * NT * NB * RB) + 8 * NB * RB + 8 * RB + 4 * NT * RB + 5 * NB;
-  // wavefronts of a SIMD: a few registers that spill cost less than one of them (4096 tokens, 32/8
-  // fp32 heads of 96, one 405 us, two 271)
+  // wavefronts of a SIMD: a few registers that spill cost less than one of them. One | two, where the
+  // limits decide (us; 64 rows: 4 x 1000 tokens behind 500 keys, 32/8 heads; 32 rows: 8 x 500 behind 500,
+  // 8/2 heads; 16 rows: 64 tokens over 1000, 16/4 heads): 64 rows of 128 bf16 177 | 112, f16 229 | 163,
+  // fp32 285 | 373, of 96 fp32 245 | 168; 32 rows of 256 bf16 88 | 118, f16 111 | 133, of 128 fp32 75.6 | 56.1
+  // (which the limits miss); 16 rows of 256 fp32 28.5 | 37.7. Two | four, 16 rows: one workgroup a CU, 128 bf16 12.2
+  // | 14.3; several, 64 tokens over 0 to 8192 keys, 32.8 | 32.4; one of 131071 keys, 128 f16, 23.5 | 32.5
   static constexpr int WPE = NEED <= 80 && 4 * LDS <= 160 * 1024 ? 4 : NEED <= (NT == 3 ? 195 : 215) && 2 * LDS <= 160 * 1024 ? 2 : 1;
 };
 

@@ -98,6 +98,11 @@ struct Kv4Plan {
 // 128 take longer for a key: from 512 on whole | 512 | 256, 4 x 600 keys, 16/4 heads of 256 14.7 |
 // 16.1 | 13.5, 4 x 1000 19.4 | 16.2 | 13.6, 64 x 900, 8/2 heads of 192 18.0 | 16.0 | 15.6, unless
 // every CU has one anyway: 64 x 600, 16/4 heads of 256 16.5 | 22.9 | 23.5, 64 x 900 21.8 | 22.8 | 29.1.
+//
+// Prompts whose tiles fill the CUs are never cut, as the host does not know which of them
+// are long: cut to 16384 keys, 4 x 500 tokens behind 20000, 32/8 heads of 128, take 952 for 733,
+// 4 x 2000 behind 30000 4683 for 4227. Single tokens among them pay for it: 7 of 131072 keys
+// beside a prompt of 2000 2016 (cut 431), in calls of their own 228 and 67.
 int check_kv4_attn(const aih_kv4_attn_desc *d, AttnArgs *a, Kv4Plan *p) {
   const char *fn = "aih_kv4_attn";
   if (!d) return api_fail("aih_kv4_attn: NULL descriptor");

@@ -75,8 +75,10 @@ __device__ __forceinline__ void mx_store4(const Mx4PwArgs &a, const Act &act, ui
 
 // ---------------------------------------------------------------- few pixels
 //
-// Up to 32 pixels: bound by the weights' bytes (16 x 8192 x 8192 17 us, 2.1 TB/s) or, with
-// few of those, by one chain of loads, products and the join (8 x 4096 x 4096 5.6 us). A workgroup owns 16 channels, its W
+// Up to 32 pixels: the weights' bytes are the floor, but what bounds it is waiting for them:
+// 16 x 8192 x 8192 takes 17 us, 2.1 TB/s where a large copy reaches 5.1, 8 x 4096 x 4096 5.7
+// with wavefronts waiting for 69 % of their time (half a cache line a row and stage, two stages
+// on their way, a load for every byte of scales). A workgroup owns 16 channels, its W
 // wavefronts take turns at the stages of 128 elements, operands straight into registers
 // (a lane: channel lane % 16, block lane / 16 of the stage, 64 contiguous bytes a row),
 // and the partial sums are joined in LDS in the wavefronts' order.
@@ -129,15 +131,16 @@ __global__ __launch_bounds__(64 * W) void mx4_pw_few_kernel(Mx4PwArgs a) {
 //
 // WM x WN wavefronts of TM x TN blocks of 32 pixels x 32 channels. Stages of U
 // blocks of 32 elements (16 U bytes a row; 8 are a whole cache line) come into LDS by
-// DMA, up to NST of them ahead; the scales of 16 blocks a row with every 16 / U-th
-// one. Unit u of tile row r is at slot u ^ mx_swz(r), which spreads 16 rows' units over
-// the banks.
+// DMA: while a stage is worked on the next NST - 1 are in LDS or on their way; the scales
+// of 16 blocks a row come with every 16 / U-th one. Unit u of tile row r is at slot
+// u ^ mx_swz(r), which spreads 16 rows' units over the banks.
 //
 // A stage is U / 2 products of 64 elements. The operands of each are read while the
 // one before it runs, those of the next stage's first too, so that the matrix unit has a
 // product's work in registers when the wavefronts meet. 8192 cubed takes 285 us, 3.85
 // PFLOP/s, where the matrix unit alone reaches 7.1; without the copies it took 230, without
-// the products 236: both pipes are busy most of the time. With the products of a stage
+// the products 236: neither alone is the bound, and the reads from LDS (six operands for eight
+// products of a wavefront) keep the matrix unit from its rate even without copies. With the products of a stage
 // behind its barrier, and half a cache line a row, it took 353.
 template <int WM_, int WN_, int TM_, int TN_, int NST_, int U_>
 struct MxTile {
@@ -417,7 +420,7 @@ hipError_t launch_few(const Mx4PwArgs &a, hipStream_t st) {
   return hipGetLastError();
 }
 
-// Measured, bf16, us: 8192 cubed with tiles of 256 x 256 289, 128 x 128 356, 64 x 128 483;
+// Measured, bf16, us, calls in a row: 8192 cubed with tiles of 256 x 256 289, 128 x 128 356, 64 x 128 483;
 // 4096 cubed 40.6 | 48 | 63; 2048 cubed 20 | 12.0 | 11.0, 64 x 64 12.0; 1024 x 4096 x 4096 32 |
 // 17.9 | 17.7 | 20.1; 3000 x 4096 x 4096 34.8 | 39 | 48; 5000 x 8192 x 1000 54 | 39 | 48; 300 x
 // 4096 x 4096 31 | 15.5 | 13.0 | 11.6. A short sum gives little

@@ -150,7 +150,10 @@ typedef struct {
   float scale;          /* finite, 1e-20 to 1e20; 0 = 1 / sqrt(d) */
   int32_t dt;           /* enum aih_dtype: q, o */
   uint32_t max_len;     /* the longest k_len, as far as known (0: all that a table row holds); steers
-                           how the keys are split, results hold for any lengths */
+                           how the keys are split, results hold for any lengths. A call is planned
+                           by its average sequence: where that has more than 32 (query, head of a
+                           group) rows and the tiles fill the chip, no keys are split, so single
+                           tokens over long caches beside prompts belong in a call of their own */
   uint64_t q_stride, o_stride; /* elements, whole 16-byte units; 0 = dense */
 } aih_kv4_attn_desc;
 
