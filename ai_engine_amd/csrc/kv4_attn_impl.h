@@ -4,7 +4,11 @@
 // bf16, and the matrix instructions run in bf16 for every type: fp32 queries and
 // probabilities are taken as three bf16 terms, which hold all their 24 bits, f16
 // ones as two (all 11 bits of a query, 16 of a probability), whose products are
-// summed in fp32.
+// summed in fp32. bf16 probabilities are rounded to bf16, and their sum is of the rounded
+// ones, so that the roundings cancel where one key has most of it: results are off by 2.3e-3
+// (four prompts behind 2000 keys) and 1.4e-3 (64 tokens over 0 to 8192), by 1.7e-3 and
+// 1.3e-3, which is their own rounding, with a second term, for 160 us instead of 136 and 36.8
+// instead of 31.3.
 //
 // As in attn_impl.h the scores are S^T = K Q^T and the result O^T += V^T P^T, here
 // with 16x16x32 instructions and 16 RB (query, head of the group) rows a
