@@ -146,8 +146,7 @@ int check_kv4_attn(const aih_kv4_attn_desc *d, AttnArgs *a, Kv4Plan *p) {
   const uint64_t base = p->tiles * d->hkv;
   // the join's launch takes 1024 threads a row at the most; the chip is full without
   const bool joins = (uint64_t)d->tokens * d->hq < 1u << 22;
-  if (!joins) {
-  } else if (few && len > (d->d > 128 && base < cus ? 512u : 1024u)) {
+  if (joins && few && len > (d->d > 128 && base < cus ? 512u : 1024u)) {
     p->shift = 10;
     while (p->shift > 8 && base * parts(p->shift) < 2ull * cus) --p->shift;
   } else if (!few && base < cus) {
